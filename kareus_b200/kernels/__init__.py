@@ -161,6 +161,26 @@ def gemm(a, b, trans_a=False, trans_b=True, out_dtype=None, accumulate=None, out
     return r
 
 
+# ----------------------------------------------------------------------------- 8-bit floating point
+def fp8_quantize(x, rows=True, cols=False, square=False, fmt="e4m3"):
+    """``(r, c)``: the matrix ``x`` in 8 bits for a product along its rows, and its transpose for a product along its columns
+    (:class:`.fp8.Fp8Matrix`; ``None`` for the one that is not wanted), both from one pass over ``x``.
+
+    A piece of 1 x 128 elements along the contraction (activations, gradients), or of 128 x 128 with ``square`` (weights), is held
+    as ``q * 2^E`` with the smallest whole ``E`` under which it fits the format (``"e4m3"``: 448, ``"e5m2"``: 57344) and ``q``
+    rounded to nearest even.  A piece with an infinity or a NaN stands for NaN as a whole."""
+    from .fp8 import quantize
+    return quantize(x, rows, cols, square, fmt)
+
+
+def fp8_gemm(a, b, out_dtype=None, accumulate=None, out=None):
+    """``a @ b.T`` of two :class:`.fp8.Fp8Matrix`, summed in fp32; bf16 unless ``out_dtype`` or ``out`` says fp32.  ``accumulate``
+    is an fp32 tensor that receives ``+=``.  With ``(xr, xc) = fp8_quantize(x, cols=True)``, the same of ``dy`` and, square, of
+    ``w``, a linear layer is ``y = fp8_gemm(xr, wr)``, ``dx = fp8_gemm(dr, wc)``, ``fp8_gemm(dc, xc, accumulate=dw)``."""
+    from .fp8 import gemm as f
+    return f(a, b, out_dtype, accumulate, out)
+
+
 # ----------------------------------------------------------------------------- attention
 def _peer_guard(q, what: str) -> None:
     """A call that announces peer-memory operands may only reach this package's own kernels."""

@@ -1,0 +1,212 @@
+// bf16 → 8-bit floating point with power-of-two scales, along the rows, along the columns, or both in one pass.
+//
+// A piece of 128 elements along the contraction (of 128 x 128 for a weight, so that the same values serve as the weight and as its
+// transpose) is held as q * 2^E: E is the smallest integer with |x| <= max * 2^E over the piece (max: 448 for e4m3, 57344 for
+// e5m2), q the nearest value of the format, ties to even.  A scale is one byte, E + 127; it is read off the bits of the largest
+// |x|, so nothing here is rounded but q itself: x * 2^-E is exact in fp32.  A piece of zeros has the byte 0.  A piece with an
+// infinity or a NaN has the byte 255 (NaN) and stands for NaN as a whole: an overflow stays visible and does not become a large
+// number.
+//
+// Scales are laid out as the product's tensor memory takes them (gemm_fp8_sm100.cu): 128 rows x 4 pieces are 512 bytes, row r of
+// them at (r % 32) * 16 + (r / 32) * 4; [ceil(rows / 128)][ceil(pieces / 4)] such blocks.  Bytes past the edge are 0.
+//
+// What bounds it: memory.  A block of 256 threads takes a 128 x 128 tile, reads it once (16 lanes a row, 16 bytes each), writes the
+// rows' bytes from registers and the columns' by way of shared memory, 32 tokens (one sector) of a column a thread.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+#include "launch.h"
+#include "pdl.cuh"
+
+namespace kb {
+
+struct Fp8Quantize {
+  const __nv_bfloat16* x;
+  long ld;                      // elements from row to row
+  int rows, cols;
+  uint8_t *q, *s;               // [rows, ldq] and its scales; null: not wanted
+  uint8_t *qt, *st;             // [cols, ldqt] (the transpose) and its scales; null: not wanted
+  long ldq, ldqt;
+  int tiles_c;                  // 128-column tiles
+  bool vec;                     // rows start on 16 bytes and hold whole 16-byte units
+};
+
+constexpr int FQ_THREADS = 256;
+constexpr int FQ_PITCH = 68;    // words from row to row of the staged tile: rows start on 16 bytes, units of a row on other banks
+
+// Scale byte of a piece whose largest |x| has these bf16 bits; TOP: the format's largest value is 0.875 * 2^TOP.
+template <int TOP>
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
+  const int e = static_cast<int>(amax >> 7);
+  if (e == 255) return 255u;
+  const int b = e + 1 - TOP + ((amax & 127u) > 96u ? 1 : 0);    // 1.mmmmmmm > 1.75 does not fit any more
+  return b > 0 ? static_cast<uint32_t>(b) : 0u;
+}
+// 2^-E
+__device__ __forceinline__ float inverse_scale(uint32_t byte) {
+  return __uint_as_float(byte == 255u ? 0x7fc00000u : (254u - byte) << 23);
+}
+// Two bf16 (packed), scaled, as two bytes; the low half goes to the low byte.
+template <bool E5M2>
+__device__ __forceinline__ uint32_t quantize2(uint32_t v, float inv) {
+  const float lo = __uint_as_float(v << 16) * inv, hi = __uint_as_float(v & 0xffff0000u) * inv;
+  uint16_t r;
+  if constexpr (E5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// The same for two values of one column that come from two packed pairs.
+template <bool E5M2, bool HIGH>
+__device__ __forceinline__ uint32_t quantize_col(uint32_t a, uint32_t b, float inv) {
+  const uint32_t v = __byte_perm(a, b, HIGH ? 0x7632 : 0x5410);
+  return quantize2<E5M2>(v, inv);
+}
+
+// Where the scale of (row, piece) lies.
+__device__ __forceinline__ size_t scale_at(int row, int piece, int groups) {
+  return (static_cast<size_t>(row >> 7) * groups + (piece >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (piece & 3);
+}
+// Writes it; the last piece also clears what is left of its group of four.
+__device__ __forceinline__ void put_scale(uint8_t* s, int row, int piece, int pieces, uint32_t byte) {
+  const int groups = (pieces + 3) >> 2;
+  s[scale_at(row, piece, groups)] = static_cast<uint8_t>(byte);
+  if (piece == pieces - 1)
+    for (int p = pieces; p & 3; ++p) s[scale_at(row, p, groups)] = 0;
+}
+
+template <bool E5M2, bool SQUARE>
+__global__ void __launch_bounds__(FQ_THREADS) fp8_quantize_kernel(const Fp8Quantize p) {
+  __shared__ __align__(16) uint32_t tile[128 * FQ_PITCH];
+  __shared__ uint32_t part[4][128];
+  __shared__ uint32_t whole[FQ_THREADS / 32];
+  constexpr int TOP = E5M2 ? 16 : 9;
+  pdl_begin();
+  const int tr = blockIdx.x / p.tiles_c, tc = blockIdx.x - tr * p.tiles_c;
+  const int r0 = tr * 128, c0 = tc * 128;
+  const int tid = threadIdx.x, unit = tid & 15, rsub = tid >> 4;
+  const int col = c0 + unit * 8;
+  uint4 v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int row = r0 + i * 16 + rsub;
+    v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < p.rows && col < p.cols) {
+      const __nv_bfloat16* src = p.x + row * p.ld + col;
+      if (p.vec) {
+        v[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+      } else {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (col + j < p.cols) w[j >> 1] |= static_cast<uint32_t>(__bfloat16_as_ushort(src[j])) << (j & 1 ? 16 : 0);
+        v[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  }
+  constexpr uint32_t ABS = 0x7fff7fffu;
+  uint32_t block_byte = 0;
+  if constexpr (SQUARE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      m = __vmaxu2(__vmaxu2(__vmaxu2(m, v[i].x & ABS), __vmaxu2(v[i].y & ABS, v[i].z & ABS)), v[i].w & ABS);
+    m = max(m & 0xffffu, m >> 16);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((tid & 31) == 0) whole[tid >> 5] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < FQ_THREADS / 32; ++i) m = max(m, whole[i]);
+    block_byte = scale_byte<TOP>(m);
+  }
+  if (p.q) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = r0 + i * 16 + rsub;
+      uint32_t byte = block_byte;
+      if constexpr (!SQUARE) {
+        uint32_t m = __vmaxu2(__vmaxu2(v[i].x & ABS, v[i].y & ABS), __vmaxu2(v[i].z & ABS, v[i].w & ABS));
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, s));
+        byte = scale_byte<TOP>(max(m & 0xffffu, m >> 16));
+      }
+      if (row < p.rows && col < p.ldq) {
+        const float inv = inverse_scale(byte);
+        uint2 o;
+        o.x = quantize2<E5M2>(v[i].x, inv) | quantize2<E5M2>(v[i].y, inv) << 16;
+        o.y = quantize2<E5M2>(v[i].z, inv) | quantize2<E5M2>(v[i].w, inv) << 16;
+        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = o;
+      }
+      if (unit == 0) put_scale(p.s, row, tc, p.tiles_c, row < p.rows ? byte : 0u);
+    }
+  }
+  if (!p.qt) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    *reinterpret_cast<uint4*>(tile + (i * 16 + rsub) * FQ_PITCH + unit * 4) = v[i];
+  }
+  __syncthreads();
+  const int pair = tid & 63, rg = tid >> 6;             // two columns, 32 rows
+  uint32_t w[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) w[j] = tile[(rg * 32 + j) * FQ_PITCH + pair];
+  uint32_t b0 = block_byte, b1 = block_byte;
+  const int tiles_r = (p.rows + 127) >> 7;
+  if constexpr (!SQUARE) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) m = __vmaxu2(m, w[j] & ABS);
+    part[rg][pair] = m;
+    __syncthreads();
+    m = __vmaxu2(__vmaxu2(part[0][pair], part[1][pair]), __vmaxu2(part[2][pair], part[3][pair]));
+    b0 = scale_byte<TOP>(m & 0xffffu);
+    b1 = scale_byte<TOP>(m >> 16);
+  }
+  const int c = c0 + 2 * pair, r = r0 + rg * 32;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float inv = inverse_scale(h ? b1 : b0);
+    uint32_t o[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      o[j] = h ? quantize_col<E5M2, true>(w[4 * j], w[4 * j + 1], inv) | quantize_col<E5M2, true>(w[4 * j + 2], w[4 * j + 3], inv) << 16
+               : quantize_col<E5M2, false>(w[4 * j], w[4 * j + 1], inv) | quantize_col<E5M2, false>(w[4 * j + 2], w[4 * j + 3], inv) << 16;
+    if (c + h < p.cols) {
+      uint8_t* dst = p.qt + (c + h) * p.ldqt + r;       // ldqt is a multiple of 16: 16-byte units are whole or outside
+      if (r < p.ldqt) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+      if (r + 16 < p.ldqt) *reinterpret_cast<uint4*>(dst + 16) = make_uint4(o[4], o[5], o[6], o[7]);
+    }
+    if (rg == 0) put_scale(p.st, c + h, tr, tiles_r, c + h < p.cols ? (h ? b1 : b0) : 0u);
+  }
+}
+
+}  // namespace kb
+
+// x: [rows, cols] bf16, `ld` elements from row to row.  q [rows, ldq] / s and qt [cols, ldqt] / st: see above, either pair null.
+// ldq and ldqt are multiples of 16, at least cols / rows; what lies between the two is nobody's.  fmt: 0 e4m3, 1 e5m2.
+extern "C" int kb_fp8_quantize(const void* x, long rows, long cols, long ld, void* q, long ldq, void* s, void* qt, long ldqt,
+                               void* st, int square, int fmt, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0 || rows >= 1L << 31 || cols >= 1L << 31 || ld < cols || (!q && !qt) || (fmt & ~1)) return 7;
+  if (q && (!s || ldq < cols || ldq % 16 || reinterpret_cast<uintptr_t>(q) % 16)) return 7;
+  if (qt && (!st || ldqt < rows || ldqt % 16 || reinterpret_cast<uintptr_t>(qt) % 16)) return 7;
+  kb::Fp8Quantize p;
+  p.x = static_cast<const __nv_bfloat16*>(x);
+  p.ld = ld;
+  p.rows = static_cast<int>(rows);
+  p.cols = static_cast<int>(cols);
+  p.q = static_cast<uint8_t*>(q);
+  p.s = static_cast<uint8_t*>(s);
+  p.qt = static_cast<uint8_t*>(qt);
+  p.st = static_cast<uint8_t*>(st);
+  p.ldq = ldq;
+  p.ldqt = ldqt;
+  p.tiles_c = static_cast<int>((cols + 127) / 128);
+  p.vec = cols % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  const long blocks = (rows + 127) / 128 * p.tiles_c;
+  if (blocks >= 1L << 31) return 7;
+  auto kern = fmt ? (square ? kb::fp8_quantize_kernel<true, true> : kb::fp8_quantize_kernel<true, false>)
+                  : (square ? kb::fp8_quantize_kernel<false, true> : kb::fp8_quantize_kernel<false, false>);
+  KB_LAUNCH_PDL(kern, static_cast<unsigned>(blocks), kb::FQ_THREADS, 0, stream, p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
+}

@@ -96,6 +96,8 @@ def _declare(L) -> None:
         "kb_ce_stats": [P, P, P, P, P, LNG, I, LNG, P],
         "kb_ce_grad": [P, P, P, P, P, LNG, I, LNG, P],
         "kb_adamw": [P, P, P, P, P, LNG, F, F, F, F, F, F, F, P, F, P],
+        "kb_fp8_quantize": [P, LNG, LNG, LNG, P, LNG, P, P, LNG, P, I, I, P],
+        "kb_gemm_fp8": [P, P, I, LNG, P, P, I, LNG, P, LNG, I, I, I, I, I, P, P],
         "kb_sumsq": [P, LNG, I, P, P],
         "kb_clip_scale": [P, F, P, P],
     }
@@ -157,6 +159,22 @@ def _no_recording(what: str) -> None:
     """Guard of wrapper paths that launch PyTorch kernels (invisible to a launch-list recording)."""
     from . import replay
     replay.require_recordable(what)
+
+
+def require_current_device(what: str, *tensors) -> None:
+    """Kernels are enqueued on the current device's stream: tensors of another one are refused."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t.device.index != cur:
+            raise KernelError(f"{what}: a tensor on {t.device} while cuda:{cur} is the current device")
+
+
+def _rows_readable(t: torch.Tensor, what: str) -> torch.Tensor:
+    """``t`` if its rows are contiguous and do not overlap, else a copy."""
+    if t.stride(1) == 1 and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]) or t.shape[1] == 1 and t.is_contiguous():
+        return t
+    _no_recording(f"making the operand of {what} contiguous")
+    return t.contiguous()
 
 
 # per-device status word that kernels with bounded waits write to

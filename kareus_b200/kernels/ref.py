@@ -332,3 +332,64 @@ def embedding_bwd(dout, tokens, grad_weight, vocab_start: int):
     d = dout.reshape(-1, dout.shape[-1]).to(grad_weight.dtype) * inside.unsqueeze(-1).to(grad_weight.dtype)
     grad_weight.index_add_(0, local.clamp(0, v - 1), d)
     return grad_weight
+
+
+# ----------------------------------------------------------------------------- 8-bit floating point
+#: format -> (torch type, e of its largest value 0.875 * 2^e)
+FP8_FORMATS = {"e4m3": (torch.float8_e4m3fn, 9), "e5m2": (torch.float8_e5m2, 16)}
+
+
+def exact_power_of_two(e):
+    """``2.0 ** e`` (float64) of whole exponents, exactly."""
+    return ((e.to(torch.int64) + 1023) << 52).view(torch.float64)
+
+
+def fp8_pack_scales(byte):
+    """Scale bytes ``[rows, pieces]`` in the order of the 8-bit product: blocks of 128 rows x 4 pieces, ``[row blocks, piece
+    blocks, 32, 4, 4]``, row ``r`` of a block at ``[r % 32, r // 32]``; 0 past the edge."""
+    r, p = byte.shape
+    rt, pt = -(-r // 128), -(-p // 4)
+    full = torch.zeros(rt * 128, pt * 4, dtype=torch.uint8, device=byte.device)
+    full[:r, :p] = byte
+    return full.view(rt, 4, 32, pt, 4).permute(0, 3, 2, 1, 4).contiguous()
+
+
+def fp8_unpack_scales(scales, rows: int, pieces: int):
+    """The reverse of :func:`fp8_pack_scales`."""
+    rt, pt = scales.shape[:2]
+    return scales.permute(0, 3, 2, 1, 4).reshape(rt * 128, pt * 4)[:rows, :pieces]
+
+
+def fp8_quantize(x, fmt="e4m3", square=False):
+    """Rows of ``x`` in 8 bits: ``(data [rows, cols], scales as fp8_pack_scales lays them out)``.  A piece of 128 columns (and 128
+    rows, if ``square``) stands for ``data * 2^E`` with the smallest whole ``E >= -127`` under which it fits; a piece with an
+    infinity or a NaN is NaN as a whole."""
+    dtype, top = FP8_FORMATS[fmt]
+    rows, cols = x.shape
+    pieces = -(-cols // 128)
+    pad = torch.zeros(-(-rows // 128) * 128 if square else rows, pieces * 128, dtype=torch.float64, device=x.device)
+    pad[:rows, :cols] = x
+    amax = pad.view(-1, 128 if square else 1, pieces, 128).abs().amax(dim=(1, 3))
+    finite = torch.isfinite(amax)
+    m, e = torch.frexp(torch.where(finite, amax, 0))
+    e = torch.where(amax > 0, e - top + (m > 0.875).to(e.dtype), -127).clamp(min=-127)
+    if square:
+        e, finite = e.repeat_interleave(128, 0)[:rows], finite.repeat_interleave(128, 0)[:rows]
+    q = pad[:rows].view(rows, pieces, 128) * exact_power_of_two(-e)[:, :, None]
+    q = torch.where(finite[:, :, None], q, float("nan")).to(torch.float32).to(dtype)
+    byte = torch.where(finite, e + 127, 255).to(torch.uint8)
+    return q.view(rows, -1)[:, :cols].contiguous(), fp8_pack_scales(byte)
+
+
+def fp8_dequantize(data, scales, dtype=torch.float32):
+    rows, cols = data.shape
+    byte = fp8_unpack_scales(scales, rows, -(-cols // 128))
+    scale = torch.where(byte == 255, float("nan"), exact_power_of_two(byte.to(torch.int64) - 127))
+    return (data.to(torch.float64) * scale.repeat_interleave(128, 1)[:, :cols]).to(dtype)
+
+
+def fp8_gemm(a, b, out_dtype=torch.bfloat16, accumulate=None):
+    """``a @ b.T`` of ``(data, scales)`` pairs."""
+    acc = torch.float64 if torch.float64 in (out_dtype, None if accumulate is None else accumulate.dtype) else torch.float32
+    y = fp8_dequantize(*a, dtype=acc) @ fp8_dequantize(*b, dtype=acc).t()
+    return y.to(out_dtype) if accumulate is None else accumulate.add_(y.to(accumulate.dtype))
