@@ -312,6 +312,30 @@ def adamw_step(p, g, m, v, master, lr, beta1, beta2, eps, wd, step, grad_scale=1
     return ref.adamw_step(p, g, m, v, master, lr, beta1, beta2, eps, wd, step, grad_scale)
 
 
+def orthogonalize(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """The last two dimensions of ``x`` after ``steps`` Newton-Schulz products, as bf16: ``X = x / (|x|_F + eps)``, then ``G = X Xt;
+    X = a X + (b G + c G G) X``.  Singular vectors stay, singular values go to about 1 (0.7 to 1.2 with these coefficients and five
+    steps); ones below about 1e-3 of the largest stay small.  The products run in fp16 with fp32 sums.  A matrix with an infinity or
+    a NaN becomes NaN, one of zeros stays zero.  ``coefficients`` that let the iterates leave the range of fp16 are refused."""
+    from .muon import orthogonalize as f
+    return f(x, steps, coefficients, eps)
+
+
+def muon_step(p, g, m, master, lr, momentum=0.95, weight_decay=0.0, scale=None, nesterov=True, steps=5,
+              coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, grad_scale_tensor=None):
+    """One Muon step of a weight matrix, in place; returns the orthogonalised update (bf16)::
+
+        m = momentum * m + s * g                                 s: the value of grad_scale_tensor, 1 without it
+        o = orthogonalize(s * g + momentum * m if nesterov else m)
+        master = master * (1 - lr * weight_decay) - lr * scale * o
+        p = master rounded to bf16
+
+    ``g``, ``m`` and ``master`` are fp32.  ``scale`` (default ``0.2 * sqrt(max(rows, columns))``) gives the update the root mean
+    square that an AdamW update has, so that learning rate and weight decay of that optimizer serve both."""
+    from .muon import muon_step as f
+    return f(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, steps, coefficients, eps, grad_scale_tensor)
+
+
 def sumsq(t):
     if is_cuda(t):
         return _cuda().sumsq(t)

@@ -1,0 +1,710 @@
+// Orthogonalising matrices by Newton-Schulz products, and the optimizer step built on it (Muon).
+//
+// X_0 = U / (|U|_F + eps), then a number of times
+//     G = X Xt,   P = b G + c G G,   X <- a X + P X          (matrices with more rows than columns: G = Xt X, X <- a X + X P)
+// which takes the singular values s of X to a s + b s^3 + c s^5 and leaves the singular vectors.
+//
+// Types.  The products run on the tensor cores in fp16 with fp32 sums: their operands are bounded by the singular values, so fp16
+// with a common power of two (`scale`, chosen by the host so that the largest possible entry fits) has 11 bits for everything that
+// counts where bf16 has 8; five steps are then 1e-3 off in the 2-norm instead of 1e-2.  The largest single rounding error would be
+// that of P's diagonal (about -2.6 beside entries near 0), so the diagonal stays in fp32, outside P: X <- (a + diag P) X + (P - diag
+// P) X.  Norms are summed in fp32 per thread and fp64 beyond, in a fixed order.
+//
+// G and P are symmetric: only the tiles on and above the diagonal are computed, the others are written as their transposes.
+//
+// One 256 x BN tile per two-CTA cluster (tcgen05 cta_group::2), roles as in gemm_pair_sm100.cu:
+//   warp 0      TMA producer of this CTA's halves
+//   warp 1      MMA issuer (leader CTA only); allocates TMEM in both CTAs
+//   warps 2..9  epilogue: accumulator and the tile of G or X that is added to it, which is fetched while the main loop runs
+#include <cuda_fp16.h>
+#include "sm100.cuh"
+#include "launch.h"
+#include "pdl.cuh"
+#include "host_utils.h"
+
+namespace kb {
+
+constexpr int NS_BM = 256;                     // rows of a tile (128 per CTA)
+constexpr int NS_BK = 64;
+constexpr int NS_MAX_STAGES = 8;
+constexpr int NS_EPI_WARPS = 8;                // 4 TMEM lane quarters x 2 sets of column slabs
+constexpr int NS_THREADS = (2 + NS_EPI_WARPS) * 32;
+constexpr int NS_A_BYTES = 128 * NS_BK * 2;
+constexpr int NS_RING = 5 * (NS_A_BYTES + 128 * NS_BK * 2);
+constexpr int NS_STG_BYTES = NS_EPI_WARPS * 8192;          // two 4 KB slabs a warp
+constexpr int NS_SMEM = NS_RING + NS_STG_BYTES + 256 + 1024;
+static_assert(NS_SMEM <= 227 * 1024, "shared memory per CTA");
+
+enum NsMode : int {
+  NS_GRAM = 0,       // G = X Xt
+  NS_POLY = 1,       // P = b G + c G G; diagonal apart
+  NS_UPDATE = 2,     // X <- (a + d) X + P X
+  NS_UPDATE_T = 3,   // X <- X (a + d) + X P
+};
+
+struct NsWork {
+  int batch, tiles_m, tiles_n, per_matrix, nk;
+  int ratio;                                   // column tiles per 256 rows, where only the upper tiles are computed; else 0
+  int group_m;
+  __device__ __forceinline__ int units() const { return batch * per_matrix; }
+  __device__ __forceinline__ void decode(int u, int& z, int& tm, int& tn) const {
+    z = u / per_matrix;
+    int t = u - z * per_matrix;
+    if (ratio) {                               // row after row of the upper triangle
+      tm = 0;
+      for (int len = tiles_n; t >= len; len -= ratio) { t -= len; ++tm; }
+      tn = tm * ratio + t;
+    } else {
+      const int per_group = group_m * tiles_n;
+      const int g = t / per_group, first_m = g * group_m, gsz = min(group_m, tiles_m - first_m), r = t - g * per_group;
+      tm = first_m + r % gsz;
+      tn = r / gsz;
+    }
+  }
+};
+
+struct NsEpilogue {
+  const __half* e;           // tile that is added (G or X): [batch][M][lde]
+  long e_batch;
+  int lde, e_cols;           // e_cols: columns to read, a multiple of 8
+  float alpha, coef;         // accumulator's factor, e's factor
+  float* diag;               // [batch][diag_len]: diagonal of P, written by NS_POLY, read by the updates
+  int diag_len;
+  float unit;                // 1 / scale
+  __nv_bfloat16* out;        // last update: the result, [batch][M][N]
+  bool last;
+};
+
+// D[tmem] (+)= A * B in fp16: the instruction descriptor's formats are 0.
+__host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(M >> 4) << 24);
+}
+__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ float2 f16_pair(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+template <bool A_MN, bool B_MN, int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NS_THREADS, 1)
+newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmM, const NsWork w, const int M,
+                     const int N, const int bn, const NsEpilogue ep, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + NS_RING + NS_STG_BYTES);   // used in the leader
+  uint64_t* empty = full + NS_MAX_STAGES;
+  uint64_t* tfull = empty + NS_MAX_STAGES;  // [2]
+  uint64_t* tempty = tfull + 2;             // [2] used in the leader
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int units = w.units();
+  const int half_n = bn >> 1;
+  const int b_bytes = B_MN ? ((half_n + 63) / 64) * 64 * NS_BK * 2 : half_n * NS_BK * 2, stage_bytes = NS_A_BYTES + b_bytes;
+  const int stages = min(NS_MAX_STAGES, NS_RING / stage_bytes);
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS_MAX_STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&tfull[i], 1);
+      mbar_init(&tempty[i], 2 * NS_EPI_WARPS);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                       // the peer's barriers exist before anything arrives on them
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_begin();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ producer (each CTA: its own halves)
+    if (elect_one()) {
+      prefetch_tmap(&tmA);
+      prefetch_tmap(&tmB);
+      const int b_chunks = (half_n + 63) >> 6;
+      const uint32_t full0 = cluster_addr(full, 0);
+      int s = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      for (int u = first; u < units && ok; u += step) {
+        int z, tm, tn;
+        w.decode(u, z, tm, tn);
+        const int m0 = tm * NS_BM + rank * 128, n0 = tn * bn + rank * half_n;
+        for (int kb_ = 0; kb_ < w.nk; ++kb_) {
+          if (!mbar_wait(&empty[s], ph, abort_flag, status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
+          uint8_t* a_dst = smem + s * stage_bytes;
+          uint8_t* b_dst = a_dst + NS_A_BYTES;
+          const uint32_t bar = full0 + s * 8;
+          if (rank == 0) mbar_expect_tx(&full[s], 2u * stage_bytes);
+          const int k0 = kb_ * NS_BK;
+          if constexpr (!A_MN) {
+            tma_load_3d_pair(a_dst, &tmA, bar, k0, m0, z);
+          } else {
+            tma_load_3d_pair(a_dst, &tmA, bar, m0, k0, z);
+            tma_load_3d_pair(a_dst + 8192, &tmA, bar, m0 + 64, k0, z);
+          }
+          if constexpr (!B_MN) {
+            tma_load_3d_pair(b_dst, &tmB, bar, k0, n0, z);
+          } else {
+            tma_load_3d_pair(b_dst, &tmB, bar, n0, k0, z);
+            if (b_chunks > 1) tma_load_3d_pair(b_dst + 8192, &tmB, bar, n0 + 64, k0, z);
+          }
+          if (++s == stages) { s = 0; ph ^= 1u; }
+        }
+      }
+      if (!ok) {
+        // leave no copy in flight: tile loads land within microseconds, give them 200 us
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 200000ull) {}
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (leader)
+    if (rank == 0 && elect_one()) {
+      const uint32_t idesc = make_idesc_f16(NS_BM, bn, A_MN, B_MN);
+      const uint32_t smem0 = smem_u32(smem);
+      const uint64_t ad0 = A_MN ? make_smem_desc(smem0, 8192, 1024) : make_smem_desc(smem0, 16, 1024);
+      const uint64_t bd0 = B_MN ? make_smem_desc(smem0 + NS_A_BYTES, 8192, 1024) : make_smem_desc(smem0 + NS_A_BYTES, 16, 1024);
+      constexpr uint64_t ka = (A_MN ? 2048 : 32) >> 4, kb = (B_MN ? 2048 : 32) >> 4;   // descriptor step of 16 in K
+      uint32_t tile_i = 0;
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int u = first; u < units && ok; u += step, ++tile_i) {
+        const uint32_t buf = tile_i & 1u;
+        if (!mbar_wait(&tempty[buf], ((tile_i >> 1) & 1u) ^ 1u, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * 256;
+        for (int kb_ = 0; kb_ < w.nk; ++kb_) {
+          if (!mbar_wait(&full[s], ph, abort_flag, status, ST_TIMEOUT_FULL)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t ad = ad0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
+          const uint64_t bd = bd0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
+#pragma unroll
+          for (int k = 0; k < NS_BK / 16; ++k)
+            umma_ss_pair(d_tmem, ad + k * ka, bd + k * kb, idesc, (kb_ > 0 || k > 0) ? 1u : 0u);
+          umma_commit_pair(&empty[s]);
+          if (kb_ == w.nk - 1) umma_commit_pair(&tfull[buf]);
+          if (++s == stages) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3;                   // TMEM lane quarter
+    const int h = (warp - 2) >> 2;            // this warp takes the 64-column slabs h, h + 2, ...
+    uint8_t* const stg0 = smem + NS_RING + (warp - 2) * 8192;
+    const int slabs = bn / 64;
+    constexpr bool ADDS = MODE != NS_GRAM, SYMMETRIC = MODE == NS_GRAM || MODE == NS_POLY;
+    uint4 v[8];                               // the tile that is added: 32 rows x 64 columns, on its way
+    auto fetch = [&](int u, int c) {
+      int z, tm, tn;
+      w.decode(u, z, tm, tn);
+      const int row0 = tm * NS_BM + rank * 128 + q * 32, col = tn * bn + c * 64 + (lane & 7) * 8;
+      const __half* src = ep.e + z * ep.e_batch + col;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = row0 + i * 4 + (lane >> 3);
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < M && col < ep.e_cols) v[i] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(r) * ep.lde);
+      }
+    };
+    if (ADDS && first < units && h < slabs) fetch(first, h);
+    uint32_t tile_i = 0, slab_i = 0;
+    for (int u = first; u < units; u += step, ++tile_i) {
+      int z, tm, tn;
+      w.decode(u, z, tm, tn);
+      const uint32_t buf = tile_i & 1u;
+      const int row0 = tm * NS_BM + rank * 128 + q * 32, row = row0 + lane;
+      float coef = ep.coef;
+      if constexpr (MODE == NS_UPDATE) {
+        if (row < M) coef += ep.diag[static_cast<size_t>(z) * ep.diag_len + row];
+      }
+      __syncwarp();
+      if (!mbar_wait_warp(&tfull[buf], (tile_i >> 1) & 1u, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + buf * 256 + (static_cast<uint32_t>(q * 32) << 16);
+      const bool mirror = SYMMETRIC && tn * bn / NS_BM > tm;
+#pragma unroll 1
+      for (int c = h; c < slabs; c += 2, ++slab_i) {
+        // Symmetric outputs use one buffer for the tile and one for its transpose, the others two in turn.
+        uint8_t* const stg = SYMMETRIC ? stg0 : stg0 + (slab_i & 1u) * 4096;
+        uint8_t* const stg_row = stg + lane * 128;
+        if (lane == 0) {
+          if constexpr (SYMMETRIC) tma_store_wait_read<0>();
+          else tma_store_wait_read<1>();
+        }
+        __syncwarp();
+        if constexpr (ADDS) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            *reinterpret_cast<uint4*>(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = v[i];
+          }
+          __syncwarp();
+          if (c + 2 < slabs) fetch(u, c + 2);
+          else if (u + step < units) fetch(u + step, h);
+          __syncwarp();
+        }
+        const int col0 = tn * bn + c * 64;
+        uint32_t o[32];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t a[32];
+          __syncwarp();                               // TMEM is read by whole warps: what lanes did on their own before ends here
+          tmem_ld_32x32(taddr + c * 64 + half * 32, a);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int unit = half * 4 + j;
+            uint4 e4 = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (ADDS) e4 = *reinterpret_cast<const uint4*>(stg_row + ((unit ^ (lane & 7)) << 4));
+            const uint32_t e[4] = {e4.x, e4.y, e4.z, e4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float x = __uint_as_float(a[8 * j + 2 * i]) * ep.alpha, y = __uint_as_float(a[8 * j + 2 * i + 1]) * ep.alpha;
+              if constexpr (ADDS) {
+                const float2 p = f16_pair(e[i]);
+                float c0 = coef, c1 = coef;
+                if constexpr (MODE == NS_UPDATE_T) {
+                  const int col = col0 + unit * 8 + 2 * i;
+                  const float* d = ep.diag + static_cast<size_t>(z) * ep.diag_len;
+                  if (col < N) c0 += d[col];
+                  if (col + 1 < N) c1 += d[col + 1];
+                }
+                x = fmaf(c0, p.x, x);
+                y = fmaf(c1, p.y, y);
+              }
+              if constexpr (MODE == NS_POLY) {
+                const int d = row - (col0 + unit * 8 + 2 * i);      // the diagonal is held apart
+                if (d == 0 || d == 1) {
+                  if (row < M) ep.diag[static_cast<size_t>(z) * ep.diag_len + row] = (d ? y : x) * ep.unit;
+                  if (d) y = 0.f;
+                  else x = 0.f;
+                }
+              }
+              o[unit * 4 + i] = ep.last ? pack_bf16x2(x * ep.unit, y * ep.unit) : pack_f16x2(x, y);
+            }
+          }
+        }
+        if (c + 2 >= slabs) {
+          // this warp's last read of the accumulator: hand it back before the stores go out
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+        }
+        __syncwarp();
+        if (!SYMMETRIC && ep.last && (N & 7)) {      // rows of the result start anywhere
+          __nv_bfloat16* dst = ep.out + (static_cast<size_t>(z) * M + row) * N + col0;
+          if (row < M) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j)
+              if (col0 + j < N) dst[j] = __ushort_as_bfloat16(static_cast<unsigned short>(o[j >> 1] >> (j & 1 ? 16 : 0)));
+          }
+          continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          st_shared_v4(smem_u32(stg_row) + ((j ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        if (mirror) {                                // [64 columns][32 rows]
+          uint16_t* t = reinterpret_cast<uint16_t*>(stg0 + 4096) + lane;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            t[(2 * j) * 32] = static_cast<uint16_t>(o[j]);
+            t[(2 * j + 1) * 32] = static_cast<uint16_t>(o[j] >> 16);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (row0 < M && col0 < N) {                // the tensor maps clip what crosses the edge
+            tma_store_3d(&tmC, stg, col0, row0, z);
+            if (mirror) tma_store_3d(&tmM, stg0 + 4096, row0, col0, z);
+          }
+          tma_store_commit();
+        }
+      }
+      if (slabs <= h) {                              // no slab for this warp (narrow tile): release all the same
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+      }
+    }
+    if (lane == 0) tma_store_wait<0>();              // nothing in flight out of shared memory at exit
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// ----------------------------------------------------------------------------- the passes around the products
+constexpr int NS_SUM_THREADS = 256;
+constexpr int NS_SUM_BLOCKS = 592;             // most blocks that share a matrix' sum of squares
+
+__device__ __forceinline__ double block_sum(double s) {
+  __shared__ double sh[NS_SUM_THREADS / 32];
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) s += __shfl_xor_sync(0xffffffffu, s, i);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = 0.;
+#pragma unroll
+  for (int i = 0; i < NS_SUM_THREADS / 32; ++i) s += sh[i];
+  return s;
+}
+
+// The matrix that is orthogonalised, read where it lies: of fp32 or bf16 values, or of a gradient and its momentum.
+struct NsSource {
+  const void* x;             // fp32 or bf16 values; the gradient of an optimizer step
+  float* m;                  // momentum, or null
+  const float* grad_scale;   // the gradient's factor on the device, or null
+  float beta;
+  bool bf16, nesterov;
+  // eight values from element `at` on (`n` of them exist), `whole`: aligned and all there
+  template <bool STEP>
+  __device__ __forceinline__ void load(long at, int n, bool whole, float gs, float (&u)[8]) const {
+    float g[8];
+    if (bf16) {
+      const __nv_bfloat16* p = static_cast<const __nv_bfloat16*>(x) + at;
+      if (whole) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          g[2 * j] = __uint_as_float(w[j] << 16);
+          g[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] = j < n ? __bfloat162float(p[j]) : 0.f;
+      }
+    } else {
+      load8(static_cast<const float*>(x) + at, n, whole, g);
+    }
+    if (!m) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] = g[j];
+      return;
+    }
+    float mo[8];
+    load8(m + at, n, whole, mo);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      g[j] *= gs;
+      if (STEP) mo[j] = fmaf(beta, mo[j], g[j]);
+      u[j] = nesterov ? fmaf(beta, mo[j], g[j]) : mo[j];
+    }
+    if (STEP) {
+      if (whole) {
+        *reinterpret_cast<float4*>(m + at) = make_float4(mo[0], mo[1], mo[2], mo[3]);
+        *reinterpret_cast<float4*>(m + at + 4) = make_float4(mo[4], mo[5], mo[6], mo[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < n) m[at + j] = mo[j];
+      }
+    }
+  }
+  static __device__ __forceinline__ void load8(const float* p, int n, bool whole, float (&g)[8]) {
+    if (whole) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+      g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = j < n ? p[j] : 0.f;
+    }
+  }
+};
+
+// Momentum step (where there is one) and sum of squares: part[matrix][block], in a fixed order.
+__global__ void __launch_bounds__(NS_SUM_THREADS)
+ns_sumsq_kernel(const NsSource src, long count, bool aligned, double* __restrict__ part) {
+  pdl_begin();
+  const float gs = src.grad_scale ? *src.grad_scale : 1.f;
+  const long base = blockIdx.y * count, vecs = (count + 7) / 8;
+  float s = 0.f;
+  double total = 0.;
+  int n = 0;
+  for (long i = static_cast<long>(blockIdx.x) * NS_SUM_THREADS + threadIdx.x; i < vecs; i += static_cast<long>(gridDim.x) * NS_SUM_THREADS) {
+    const int left = static_cast<int>(count - i * 8 < 8 ? count - i * 8 : 8);
+    float u[8];
+    src.load<true>(base + i * 8, left, aligned && left == 8, gs, u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(u[j], u[j], s);
+    if (++n == 32) {                           // short fp32 sums, added up in fp64
+      total += s;
+      s = 0.f;
+      n = 0;
+    }
+  }
+  total = block_sum(total + s);
+  if (threadIdx.x == 0) part[static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x] = total;
+}
+
+// X_0 in fp16: rows of ldx elements, zeros behind the columns.
+__global__ void __launch_bounds__(NS_SUM_THREADS)
+ns_normalize_kernel(const NsSource src, int rows, int cols, int ldx, bool aligned, const double* __restrict__ part, int parts, float eps,
+                    float scale, __half* __restrict__ x) {
+  pdl_begin();
+  double sq = 0.;
+  for (int i = threadIdx.x; i < parts; i += NS_SUM_THREADS) sq += part[static_cast<size_t>(blockIdx.y) * parts + i];
+  const double norm = sqrt(block_sum(sq)) + static_cast<double>(eps);
+  // a norm that fp32 squares cannot hold, or a matrix with an infinity, gives NaN and not zeros
+  const float f = isinf(norm) ? __int_as_float(0x7fc00000) : static_cast<float>(static_cast<double>(scale) / norm);
+  const float gs = src.grad_scale ? *src.grad_scale : 1.f;
+  const int vecs = ldx >> 3;
+  const long total = static_cast<long>(rows) * vecs;
+  const long base = blockIdx.y * static_cast<long>(rows) * cols;
+  x += blockIdx.y * static_cast<long>(rows) * ldx;
+  for (long i = static_cast<long>(blockIdx.x) * NS_SUM_THREADS + threadIdx.x; i < total; i += static_cast<long>(gridDim.x) * NS_SUM_THREADS) {
+    const long r = i / vecs;
+    const int c = static_cast<int>(i - r * vecs) * 8, left = min(8, cols - c);
+    float u[8];
+    src.load<false>(base + r * cols + c, left, aligned && left == 8, gs, u);
+    uint4 o;
+    o.x = pack_f16x2(u[0] * f, u[1] * f);
+    o.y = pack_f16x2(u[2] * f, u[3] * f);
+    o.z = pack_f16x2(u[4] * f, u[5] * f);
+    o.w = pack_f16x2(u[6] * f, u[7] * f);
+    *reinterpret_cast<uint4*>(x + i * 8) = o;
+  }
+}
+
+// master <- master * keep - step * o;  p = bf16(master)
+__global__ void __launch_bounds__(256)
+muon_apply_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ p, const __nv_bfloat16* __restrict__ o, long n, bool aligned,
+                  float keep, float step) {
+  pdl_begin();
+  const long vecs = aligned ? n / 8 : 0;
+  for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < vecs; i += static_cast<long>(gridDim.x) * 256) {
+    const uint4 r = reinterpret_cast<const uint4*>(o)[i];
+    float4 a = reinterpret_cast<float4*>(master)[2 * i], b = reinterpret_cast<float4*>(master)[2 * i + 1];
+    a.x = fmaf(-step, __uint_as_float(r.x << 16), a.x * keep);
+    a.y = fmaf(-step, __uint_as_float(r.x & 0xffff0000u), a.y * keep);
+    a.z = fmaf(-step, __uint_as_float(r.y << 16), a.z * keep);
+    a.w = fmaf(-step, __uint_as_float(r.y & 0xffff0000u), a.w * keep);
+    b.x = fmaf(-step, __uint_as_float(r.z << 16), b.x * keep);
+    b.y = fmaf(-step, __uint_as_float(r.z & 0xffff0000u), b.y * keep);
+    b.z = fmaf(-step, __uint_as_float(r.w << 16), b.z * keep);
+    b.w = fmaf(-step, __uint_as_float(r.w & 0xffff0000u), b.w * keep);
+    reinterpret_cast<float4*>(master)[2 * i] = a;
+    reinterpret_cast<float4*>(master)[2 * i + 1] = b;
+    reinterpret_cast<uint4*>(p)[i] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+  }
+  for (long i = vecs * 8 + static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long>(gridDim.x) * 256) {
+    const float a = fmaf(-step, __bfloat162float(o[i]), master[i] * keep);
+    master[i] = a;
+    p[i] = __float2bfloat16(a);
+  }
+}
+
+// ----------------------------------------------------------------------------- host side
+struct NsLayout {
+  int rows, cols, side;      // side: the smaller of the two
+  long ldx, ldg;             // row strides in elements (multiples of 8)
+  long x, g, diag, part, total;                // bytes
+  NsLayout(int batch, int m, int n) : rows(m), cols(n), side(m < n ? m : n) {
+    const auto up = [](long b) { return (b + 255) / 256 * 256; };
+    ldx = (n + 7L) / 8 * 8;
+    ldg = (side + 7L) / 8 * 8;
+    x = up(2L * batch * m * ldx);
+    g = up(2L * batch * side * ldg);
+    diag = up(4L * batch * side);
+    part = up(8L * batch * NS_SUM_BLOCKS);
+    total = 2 * x + 2 * g + diag + part;
+  }
+};
+
+static int ns_map(CUtensorMap* map, const void* base, long inner, long rows, long batch, long ld, uint32_t box_inner, uint32_t box_rows,
+                  int swizzle) {
+  const uint64_t dims[3] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)batch};
+  const uint64_t str[2] = {(uint64_t)ld * 2, (uint64_t)ld * rows * 2};
+  const uint32_t box[3] = {box_inner, box_rows, 1};
+  return make_tmap(map, base, 2, 3, dims, str, box, swizzle);
+}
+
+// C [M, N] of each matrix of the batch from A and B: [rows][ld] matrices whose rows run along K (K-major) or along M / N.
+template <bool A_MN, bool B_MN, int MODE>
+static int ns_product(const void* A, long lda, const void* B, long ldb, void* C, long ldc, int batch, int M, int N, int K,
+                      const NsEpilogue& ep, int* status, cudaStream_t stream) {
+  constexpr bool SYMMETRIC = MODE == NS_GRAM || MODE == NS_POLY;
+  const int pairs = device_sm_count() / 2;
+  NsWork w;
+  w.batch = batch;
+  w.tiles_m = (M + NS_BM - 1) / NS_BM;
+  w.nk = (K + NS_BK - 1) / NS_BK;
+  // Width of the tiles: as for the other products on pairs of SMs, clocks of a step of 64 are the larger of the tensor cores' (2 a
+  // column) and of the loads' (64 bytes a clock reach an SM).
+  int bn = 0;
+  double best = 0;
+  for (int b = 256; b >= 64; b -= 64) {
+    if (SYMMETRIC && 256 % b) continue;        // rows of tiles start on the diagonal
+    const int tn = (N + b - 1) / b;
+    long tiles = 0;
+    if (SYMMETRIC) for (int i = 0; i < w.tiles_m; ++i) tiles += tn - i * (256 / b);
+    else tiles = (long)w.tiles_m * tn;
+    const long waves = (tiles * batch + pairs - 1) / pairs;
+    const double cost = (double)waves * (w.nk * (double)(2 * b > 256 + b ? 2 * b : 256 + b) + 1500.0);
+    if (!bn || cost < best * 0.97) {
+      best = cost;
+      bn = b;
+      w.tiles_n = tn;
+      w.per_matrix = (int)tiles;
+    }
+  }
+  w.ratio = SYMMETRIC ? 256 / bn : 0;
+  long gm = (24L << 20) / ((long)NS_BM * K * 2);
+  gm = gm < 8 ? 8 : gm > 16 ? 16 : gm;
+  w.group_m = gm < w.tiles_m ? (int)gm : w.tiles_m;
+  CUtensorMap tmA, tmB, tmC, tmM;
+  int rc;
+  // operands: zeros past the edge of K and of the rows, so that padding never counts
+  if (!A_MN) rc = ns_map(&tmA, A, K, M, batch, lda, NS_BK, 128, 3);
+  else       rc = ns_map(&tmA, A, M, K, batch, lda, 64, NS_BK, 3);
+  if (rc) return rc;
+  if (!B_MN) rc = ns_map(&tmB, B, K, N, batch, ldb, NS_BK, bn / 2, 3);
+  else       rc = ns_map(&tmB, B, N, K, batch, ldb, 64, NS_BK, 3);
+  if (rc) return rc;
+  // the output's rows in whole 16-byte units (the padding of the workspace takes zeros); a result with other rows is not stored by TMA
+  tmC = tmA;
+  if (ldc % 8 == 0 && (rc = ns_map(&tmC, C, ldc, M, batch, ldc, 64, 32, 3))) return rc;
+  tmM = tmC;
+  if (SYMMETRIC && (rc = ns_map(&tmM, C, ldc, M, batch, ldc, 32, 64, 0))) return rc;
+  auto kern = newton_schulz_kernel<A_MN, B_MN, MODE>;
+  static bool configured[64] = {};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return 7;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM);
+    if (e != cudaSuccess) return 1000 + static_cast<int>(e);
+    configured[dev] = true;
+  }
+  const long units = (long)batch * w.per_matrix;
+  if (units >= 1L << 30) return 7;
+  const int grid = 2 * (int)(units < pairs ? units : pairs);
+  KB_LAUNCH_PDL(kern, grid, NS_THREADS, NS_SMEM, stream, tmA, tmB, tmC, tmM, w, M, N, bn, ep, status);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
+}
+
+static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
+                         void* out, uint8_t* work, int* status, cudaStream_t stream) {
+  const NsLayout lay(batch, m, n);
+  uint8_t* x[2] = {work, work + lay.x};
+  uint8_t* const g = work + 2 * lay.x;
+  uint8_t* const p = g + lay.g;
+  float* const diag = reinterpret_cast<float*>(p + lay.g);
+  double* const part = reinterpret_cast<double*>(p + lay.g + lay.diag);
+  const long count = (long)m * n;
+  const auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  const long per_block = 8L * NS_SUM_THREADS;
+  {
+    const bool aligned = al(src.x) && al(src.m) && (batch == 1 || count % 8 == 0);
+    long blocks = (count + 4 * per_block - 1) / (4 * per_block);
+    const long most = NS_SUM_BLOCKS / batch > 1 ? NS_SUM_BLOCKS / batch : 1;
+    blocks = blocks < 1 ? 1 : blocks > most ? most : blocks;
+    KB_LAUNCH_PDL(ns_sumsq_kernel, dim3((unsigned)blocks, batch), NS_SUM_THREADS, 0, stream, src, count, aligned, part);
+    const bool rows_aligned = al(src.x) && al(src.m) && n % 8 == 0;
+    long nblocks = (m * (lay.ldx / 8) + NS_SUM_THREADS - 1) / NS_SUM_THREADS;
+    nblocks = nblocks > 148 * 8 ? 148 * 8 : nblocks;
+    KB_LAUNCH_PDL(ns_normalize_kernel, dim3((unsigned)nblocks, batch), NS_SUM_THREADS, 0, stream, src, m, n, (int)lay.ldx, rows_aligned,
+                  (const double*)part, (int)blocks, eps, scale, reinterpret_cast<__half*>(x[0]));
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return 2000 + static_cast<int>(e);
+  }
+  const bool tall = m > n;
+  const int side = lay.side;
+  const float unit = 1.f / scale;              // a power of two
+  for (int i = 0; i < steps; ++i) {
+    const bool last = i == steps - 1;
+    void* const xi = x[i & 1];
+    void* const xo = last ? out : x[(i + 1) & 1];
+    const long ldo = last ? n : lay.ldx;
+    NsEpilogue eg{nullptr, 0, 0, 0, unit, 0.f, nullptr, 0, unit, nullptr, false};
+    NsEpilogue epo{reinterpret_cast<const __half*>(g), side * lay.ldg, (int)lay.ldg, (int)lay.ldg, c * unit, b, diag, side, unit, nullptr, false};
+    NsEpilogue eu{reinterpret_cast<const __half*>(xi), m * lay.ldx, (int)lay.ldx, (int)lay.ldx, unit, a, diag, side, unit,
+                  static_cast<__nv_bfloat16*>(out), last};
+    int rc = tall ? ns_product<true, true, NS_GRAM>(xi, lay.ldx, xi, lay.ldx, g, lay.ldg, batch, side, side, m, eg, status, stream)
+                  : ns_product<false, false, NS_GRAM>(xi, lay.ldx, xi, lay.ldx, g, lay.ldg, batch, side, side, n, eg, status, stream);
+    if (rc) return rc;
+    rc = ns_product<false, false, NS_POLY>(g, lay.ldg, g, lay.ldg, p, lay.ldg, batch, side, side, side, epo, status, stream);
+    if (rc) return rc;
+    rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, lay.ldx, p, lay.ldg, xo, ldo, batch, m, n, side, eu, status, stream)
+              : ns_product<false, true, NS_UPDATE>(p, lay.ldg, xi, lay.ldx, xo, ldo, batch, m, n, side, eu, status, stream);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+static bool ns_sizes_ok(long batch, long m, long n) {
+  return batch >= 1 && m >= 1 && n >= 1 && batch < 1L << 16 && m < 1L << 24 && n < 1L << 24;
+}
+
+}  // namespace kb
+
+// Bytes of workspace (256-byte aligned) of the calls below, negative for sizes that they refuse.
+extern "C" long kb_newton_schulz_bytes(long batch, long m, long n) {
+  return kb::ns_sizes_ok(batch, m, n) ? kb::NsLayout((int)batch, (int)m, (int)n).total : -1;
+}
+// out [batch, m, n] (bf16, 16-byte aligned) = x (fp32 or bf16, contiguous) after `steps` Newton-Schulz steps.  scale: a power of
+// two under which every entry of the iterates, of G and of P fits into fp16.
+extern "C" int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n, float a, float b, float c, int steps, float eps,
+                                float scale, void* out, void* work, int* status, cudaStream_t stream) {
+  if (!kb::ns_sizes_ok(batch, m, n) || steps < 1 || !x || !out || !work || reinterpret_cast<uintptr_t>(out) % 16 ||
+      reinterpret_cast<uintptr_t>(work) % 256)
+    return 7;
+  const kb::NsSource src{x, nullptr, nullptr, 0.f, bf16 != 0, false};
+  return kb::newton_schulz(src, batch, m, n, a, b, c, steps, eps, scale, out, static_cast<uint8_t*>(work), status, stream);
+}
+// One optimizer step of a [m, n] matrix: mom <- beta mom + gs g;  o = Newton-Schulz of (nesterov: gs g + beta mom) or mom;
+// master <- keep * master - step * o;  p = bf16(master).  gs: *grad_scale, 1 where that is null.
+extern "C" int kb_muon_step(const float* g, float* mom, float* master, void* p, void* o, int m, int n, float beta, int nesterov,
+                            float keep, float step, const float* grad_scale, float a, float b, float c, int steps, float eps, float scale,
+                            void* work, int* status, cudaStream_t stream) {
+  if (!kb::ns_sizes_ok(1, m, n) || steps < 1 || !g || !mom || !master || !p || !o || !work || reinterpret_cast<uintptr_t>(o) % 16 ||
+      reinterpret_cast<uintptr_t>(work) % 256)
+    return 7;
+  const kb::NsSource src{g, mom, grad_scale, beta, false, nesterov != 0};
+  const int rc = kb::newton_schulz(src, 1, m, n, a, b, c, steps, eps, scale, o, static_cast<uint8_t*>(work), status, stream);
+  if (rc) return rc;
+  const long count = (long)m * n;
+  const auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
+  long blocks = (count / 8 + 255) / 256;
+  blocks = blocks < 1 ? 1 : blocks > 148 * 8 ? 148 * 8 : blocks;
+  KB_LAUNCH_PDL(kb::muon_apply_kernel, (unsigned)blocks, 256, 0, stream, master, static_cast<__nv_bfloat16*>(p),
+                static_cast<const __nv_bfloat16*>(o), count, al(master) && al(p), keep, step);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
+}

@@ -98,6 +98,8 @@ def _declare(L) -> None:
         "kb_adamw": [P, P, P, P, P, LNG, F, F, F, F, F, F, F, P, F, P],
         "kb_fp8_quantize": [P, LNG, LNG, LNG, P, LNG, P, P, LNG, P, I, I, P],
         "kb_gemm_fp8": [P, P, I, LNG, P, P, I, LNG, P, LNG, I, I, I, I, I, P, P],
+        "kb_newton_schulz": [P, I, I, I, I, F, F, F, I, F, F, P, P, P, P],
+        "kb_muon_step": [P, P, P, P, P, I, I, F, I, F, F, P, F, F, F, I, F, F, P, P, P],
         "kb_sumsq": [P, LNG, I, P, P],
         "kb_clip_scale": [P, F, P, P],
     }
@@ -107,6 +109,8 @@ def _declare(L) -> None:
         fn.restype = c_int
     L.kb_rmsnorm_bwd_scratch_elems.argtypes = [I, I]
     L.kb_rmsnorm_bwd_scratch_elems.restype = c_long
+    L.kb_newton_schulz_bytes.argtypes = [LNG, LNG, LNG]
+    L.kb_newton_schulz_bytes.restype = c_long
     L.kb_gemm_row_stats_floats.argtypes = [I, I, I]
     L.kb_gemm_row_stats_floats.restype = c_long
     L.kb_gemm_scratch_floats.argtypes = [I, I, I, I, I]

@@ -1,0 +1,106 @@
+"""Orthogonalised matrices by Newton-Schulz products and the optimizer step built on them (``csrc/newton_schulz_sm100.cu``).
+
+The contract of the calls is at :func:`kareus_b200.kernels.orthogonalize` and :func:`kareus_b200.kernels.muon_step`."""
+from __future__ import annotations
+
+import functools
+import math
+
+import torch
+
+from . import ref
+from .cuda import KernelError, _check, _count, _no_recording, _stream, lib, require_current_device, status_word
+
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+@functools.lru_cache(maxsize=64)
+def fp16_scale(steps: int, coefficients: tuple) -> float:
+    """The power of two (at most 2^14) under which the entries of X, of G = X Xt and of P = b G + c G G fit into fp16 in every step.
+    Entries are at most the largest singular value, which starts at 1 or below; the range that a step can reach is sampled."""
+    a, b, c = coefficients
+    bound, worst = 1.0, 1.0
+    for _ in range(steps):
+        s = torch.linspace(0.0, bound * 1.01, 8193, dtype=torch.float64)       # 1 %: what rounding adds
+        t = s * s
+        poly = b * t + c * t * t
+        worst = max(worst, t.max().item(), poly.abs().max().item())
+        bound = (s * (a + poly)).abs().max().item()
+        worst = max(worst, bound)
+        if not worst < 1e3:
+            raise KernelError(f"Newton-Schulz coefficients {coefficients} let the iterates grow without bound")
+    return 2.0 ** min(14, math.floor(math.log2(65000.0 / worst)))
+
+
+def _parameters(steps, coefficients, eps):
+    steps, coefficients, eps = int(steps), tuple(float(v) for v in coefficients), float(eps)
+    if steps < 1 or len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients) or not eps >= 0:
+        raise KernelError(f"Newton-Schulz: at least one step, three finite coefficients and eps >= 0, got {steps}, {coefficients}, {eps}")
+    return steps, coefficients, eps
+
+
+def _workspace(batch, m, n, device):
+    size = lib().kb_newton_schulz_bytes(batch, m, n)
+    if size < 0:
+        raise KernelError(f"Newton-Schulz: {batch} matrices of {m} x {n} are too many or too large")
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _launches(steps: int) -> int:
+    return 2 + 3 * steps
+
+
+def orthogonalize(x, steps, coefficients, eps):
+    steps, coefficients, eps = _parameters(steps, coefficients, eps)
+    if x.dim() < 2 or not x.is_floating_point():
+        raise KernelError(f"orthogonalize takes matrices of floating-point numbers, got {x.dtype} of shape {tuple(x.shape)}")
+    if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32)):
+        return ref.orthogonalize(x, steps, coefficients, eps)
+    require_current_device("orthogonalize", x)
+    scale = fp16_scale(steps, coefficients)
+    out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+    if not x.numel():
+        return out
+    if not x.is_contiguous():
+        _no_recording("making the matrices of a Newton-Schulz iteration contiguous")
+        x = x.contiguous()
+    m, n = x.shape[-2:]
+    batch = x.numel() // (m * n)
+    work = _workspace(batch, m, n, x.device)
+    _check(lib().kb_newton_schulz(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, batch, m, n, *coefficients, steps, eps, scale,
+                                  out.data_ptr(), work.data_ptr(), status_word(x.device).data_ptr(), _stream()),
+           f"orthogonalize {batch} x {m} x {n}")
+    _count(_launches(steps))
+    return out
+
+
+def muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, steps, coefficients, eps, grad_scale_tensor):
+    steps, coefficients, eps = _parameters(steps, coefficients, eps)
+    if g.dim() != 2 or any(t.shape != g.shape for t in (p, m, master)):
+        raise KernelError("muon_step takes one matrix: weight, gradient, momentum and master of one shape, got "
+                          + ", ".join(str(tuple(t.shape)) for t in (p, g, m, master)))
+    if any(t.device != g.device for t in (p, m, master)):
+        raise KernelError(f"muon_step: tensors on several devices: {[str(t.device) for t in (p, g, m, master)]}")
+    if scale is None:
+        scale = 0.2 * math.sqrt(max(g.shape))
+    if not (g.is_cuda and g.dtype == torch.float32 and p.dtype == torch.bfloat16):
+        gs = 1.0 if grad_scale_tensor is None else grad_scale_tensor.to(g.dtype)
+        return ref.muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, steps, coefficients, eps, gs)
+    require_current_device("muon_step", g)
+    if m.dtype != torch.float32 or master.dtype != torch.float32 or not all(t.is_contiguous() for t in (p, g, m, master)):
+        raise KernelError("muon_step: momentum and master have to be fp32, all tensors contiguous")
+    if grad_scale_tensor is not None and (grad_scale_tensor.dtype != torch.float32 or grad_scale_tensor.numel() != 1
+                                          or grad_scale_tensor.device != g.device):
+        raise KernelError("muon_step: the gradient's factor is one fp32 value on the gradient's device")
+    o = torch.empty(g.shape, dtype=torch.bfloat16, device=g.device)
+    if not g.numel():
+        return o
+    rows, cols = g.shape
+    work = _workspace(1, rows, cols, g.device)
+    _check(lib().kb_muon_step(g.data_ptr(), m.data_ptr(), master.data_ptr(), p.data_ptr(), o.data_ptr(), rows, cols, float(momentum),
+                              1 if nesterov else 0, 1.0 - lr * weight_decay, lr * scale,
+                              0 if grad_scale_tensor is None else grad_scale_tensor.data_ptr(), *coefficients, steps, eps,
+                              fp16_scale(steps, coefficients), work.data_ptr(), status_word(g.device).data_ptr(), _stream()),
+           f"muon_step {rows} x {cols}")
+    _count(_launches(steps) + 1)
+    return o

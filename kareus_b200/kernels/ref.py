@@ -393,3 +393,29 @@ def fp8_gemm(a, b, out_dtype=torch.bfloat16, accumulate=None):
     acc = torch.float64 if torch.float64 in (out_dtype, None if accumulate is None else accumulate.dtype) else torch.float32
     y = fp8_dequantize(*a, dtype=acc) @ fp8_dequantize(*b, dtype=acc).t()
     return y.to(out_dtype) if accumulate is None else accumulate.add_(y.to(accumulate.dtype))
+
+
+# ----------------------------------------------------------------------------- Newton-Schulz
+def orthogonalize(x, steps, coefficients, eps):
+    """``X_0 = x / (|x|_F + eps)``, then ``steps`` times ``G = X Xt; X = a X + (b G + c G G) X`` for the last two dimensions."""
+    a, b, c = coefficients
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    y = x.to(acc)
+    norm = y.square().sum(dim=(-2, -1), keepdim=True).sqrt() + eps
+    y = y / torch.where(torch.isinf(norm), float("nan"), norm)
+    tall = y.shape[-2] > y.shape[-1]
+    y = y.mT if tall else y
+    for _ in range(steps):
+        g = y @ y.mT
+        y = a * y + (b * g + c * (g @ g)) @ y
+    y = y.mT if tall else y
+    return y.contiguous().to(acc if acc == torch.float64 else torch.bfloat16)
+
+
+def muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, steps, coefficients, eps, grad_scale=1.0):
+    g = g * grad_scale
+    m.mul_(momentum).add_(g)
+    o = orthogonalize(g + momentum * m if nesterov else m, steps, coefficients, eps)
+    master.mul_(1.0 - lr * weight_decay).sub_(o.to(master.dtype), alpha=lr * scale)
+    p.copy_(master.to(p.dtype))
+    return o
