@@ -293,16 +293,21 @@ def cross_entropy_finish(logits, targets, vocab_start, gmax, gsum, grad_scale):
 
 
 # ----------------------------------------------------------------------------- embedding
-def embedding_fwd(tokens, weight, vocab_start):
+def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
+    """``scale`` times the rows of ``weight`` for tokens in ``[vocab_start, vocab_start + rows)``, zeros for others; the product is
+    rounded once to the table's type."""
     if is_cuda(weight):
-        return _cuda().embedding_fwd(tokens, weight, vocab_start)
-    return ref.embedding_fwd(tokens, weight, vocab_start)
+        return _cuda().embedding_fwd(tokens, weight, vocab_start, scale)
+    return ref.embedding_fwd(tokens, weight, vocab_start, scale)
 
 
-def embedding_bwd(dout, tokens, grad_weight, vocab_start):
+def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"):
+    """``grad_weight[id] += scale *`` the sum of ``dout`` over the tokens ``id``.  ``order="sorted"``: the rows of a token are summed
+    in the order of the tokens and added once, so the same inputs give the same bits, and tokens that fill much of a batch (padding)
+    cost no more than others; ``"any"``: as they come, with atomic additions (a ``scale`` other than 1 sorts too)."""
     if is_cuda(dout):
-        return _cuda().embedding_bwd(dout, tokens, grad_weight, vocab_start)
-    return ref.embedding_bwd(dout, tokens, grad_weight, vocab_start)
+        return _cuda().embedding_bwd(dout, tokens, grad_weight, vocab_start, scale, order)
+    return ref.embedding_bwd(dout, tokens, grad_weight, vocab_start, scale, order)
 
 
 # ----------------------------------------------------------------------------- optimizer

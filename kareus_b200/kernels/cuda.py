@@ -100,6 +100,8 @@ def _declare(L) -> None:
         "kb_gemm_fp8": [P, P, I, LNG, P, P, I, LNG, P, LNG, I, I, I, I, I, P, P],
         "kb_newton_schulz": [P, I, I, I, I, F, F, F, I, F, F, P, P, P, P],
         "kb_muon_step": [P, P, P, P, P, I, I, F, I, F, F, P, F, F, F, I, F, F, P, P, P],
+        "kb_embedding_fwd_scaled": [P, P, P, LNG, I, LNG, LNG, F, P],
+        "kb_embedding_bwd_sorted": [P, P, P, LNG, I, LNG, LNG, F, P, P],
         "kb_sumsq": [P, LNG, I, P, P],
         "kb_clip_scale": [P, F, P, P],
     }
@@ -109,6 +111,8 @@ def _declare(L) -> None:
         fn.restype = c_int
     L.kb_rmsnorm_bwd_scratch_elems.argtypes = [I, I]
     L.kb_rmsnorm_bwd_scratch_elems.restype = c_long
+    L.kb_embedding_sorted_bytes.argtypes = [LNG, I]
+    L.kb_embedding_sorted_bytes.restype = c_long
     L.kb_newton_schulz_bytes.argtypes = [LNG, LNG, LNG]
     L.kb_newton_schulz_bytes.restype = c_long
     L.kb_gemm_row_stats_floats.argtypes = [I, I, I]
@@ -720,27 +724,61 @@ def cross_entropy_finish(logits, targets, vocab_start, gmax, gsum, grad_scale):
 
 
 # ----------------------------------------------------------------------------- embedding
-def embedding_fwd(tokens, weight, vocab_start):
+def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
     if not _bf16(weight):
-        return ref.embedding_fwd(tokens, weight, vocab_start)
+        return ref.embedding_fwd(tokens, weight, vocab_start, scale)
+    _embedding_args("embedding_fwd", tokens, weight)
     tokens = tokens.contiguous()
     H = weight.shape[1]
     out = torch.empty(tuple(tokens.shape) + (H,), dtype=weight.dtype, device=weight.device)
-    _check(lib().kb_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
-                                  int(vocab_start), weight.shape[0], _stream()), "embedding_fwd")
+    if not out.numel():
+        return out
+    if scale == 1.0 and H % 8 == 0 and weight.data_ptr() % 16 == 0:
+        _check(lib().kb_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
+                                      int(vocab_start), weight.shape[0], _stream()), "embedding_fwd")
+    else:
+        _check(lib().kb_embedding_fwd_scaled(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
+                                             int(vocab_start), weight.shape[0], float(scale), _stream()), "embedding_fwd")
     _count()
     return out
 
 
-def embedding_bwd(dout, tokens, grad_weight, vocab_start):
+def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"):
+    if order not in EMBEDDING_ORDERS:
+        raise KernelError(f"unknown order {order!r} of embedding gradients; known: {EMBEDDING_ORDERS}")
     if not _bf16(dout) or grad_weight.dtype != torch.float32:
-        return ref.embedding_bwd(dout, tokens, grad_weight, vocab_start)
+        return ref.embedding_bwd(dout, tokens, grad_weight, vocab_start, scale, order)
+    _embedding_args("embedding_bwd", tokens, grad_weight, dout)
+    if dout.dim() < 1 or dout.shape[-1] != grad_weight.shape[1] or dout.numel() != tokens.numel() * grad_weight.shape[1]:
+        raise KernelError(f"embedding_bwd: {tuple(tokens.shape)} tokens and rows of {grad_weight.shape[1]} have no gradient of shape "
+                          f"{tuple(dout.shape)}")
     dout, tokens = dout.contiguous(), tokens.contiguous()
-    H = grad_weight.shape[1]
-    _check(lib().kb_embedding_bwd(tokens.data_ptr(), dout.data_ptr(), grad_weight.data_ptr(), tokens.numel(), H,
+    H, n = grad_weight.shape[1], tokens.numel()
+    if not dout.numel():
+        return grad_weight
+    L = lib()
+    if order == "sorted" or scale != 1.0:
+        work = torch.empty(L.kb_embedding_sorted_bytes(n, H), dtype=torch.uint8, device=dout.device)
+        _check(L.kb_embedding_bwd_sorted(tokens.data_ptr(), dout.data_ptr(), grad_weight.data_ptr(), n, H, int(vocab_start),
+                                         grad_weight.shape[0], float(scale), work.data_ptr(), _stream()), "embedding_bwd")
+        _count(3 * -(-n // EMBEDDING_CHUNK))
+    else:
+        _check(L.kb_embedding_bwd(tokens.data_ptr(), dout.data_ptr(), grad_weight.data_ptr(), n, H,
                                   int(vocab_start), grad_weight.shape[0], _stream()), "embedding_bwd")
-    _count()
+        _count()
     return grad_weight
+
+
+EMBEDDING_ORDERS = ("any", "sorted")
+EMBEDDING_CHUNK = 65536       # tokens that csrc/embedding_sorted.cu sorts at once
+
+
+def _embedding_args(what, tokens, table, *more):
+    if tokens.dtype != torch.int64:
+        raise KernelError(f"{what}: tokens have to be int64, got {tokens.dtype}")
+    if table.dim() != 2 or not table.is_contiguous():
+        raise KernelError(f"{what}: the table has to be a contiguous matrix, got strides {tuple(table.stride())}")
+    require_current_device(what, tokens, table, *more)
 
 
 # ----------------------------------------------------------------------------- optimizer

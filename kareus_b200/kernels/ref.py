@@ -316,21 +316,31 @@ def sumsq(t) -> torch.Tensor:
 
 
 # ----------------------------------------------------------------------------- embedding
-def embedding_fwd(tokens, weight, vocab_start: int):
-    """Rows of ``weight`` for tokens in ``[vocab_start, vocab_start+V_local)``, zeros elsewhere."""
+def embedding_fwd(tokens, weight, vocab_start: int, scale: float = 1.0):
+    """``scale`` times the rows of ``weight`` for tokens in ``[vocab_start, vocab_start+V_local)``, zeros elsewhere."""
     v = weight.shape[0]
     local = tokens - vocab_start
     inside = (local >= 0) & (local < v)
     out = weight[local.clamp(0, v - 1)]
+    if scale != 1.0:
+        out = (out.to(torch.promote_types(out.dtype, torch.float32)) * scale).to(out.dtype)
+        return torch.where(inside.unsqueeze(-1), out, 0)
     return out * inside.unsqueeze(-1).to(out.dtype)
 
 
-def embedding_bwd(dout, tokens, grad_weight, vocab_start: int):
+def embedding_bwd(dout, tokens, grad_weight, vocab_start: int, scale: float = 1.0, order: str = "any"):
     v = grad_weight.shape[0]
     local = (tokens - vocab_start).reshape(-1)
     inside = (local >= 0) & (local < v)
+    if order not in ("any", "sorted"):
+        raise ValueError(f"unknown order {order!r} of embedding gradients")
+    if order == "sorted":
+        at = torch.nonzero(inside).flatten()
+        d = dout.reshape(-1, dout.shape[-1])[at].to(grad_weight.dtype)
+        grad_weight.index_put_((local[at],), d * scale, accumulate=True)      # adds by sorted index
+        return grad_weight
     d = dout.reshape(-1, dout.shape[-1]).to(grad_weight.dtype) * inside.unsqueeze(-1).to(grad_weight.dtype)
-    grad_weight.index_add_(0, local.clamp(0, v - 1), d)
+    grad_weight.index_add_(0, local.clamp(0, v - 1), d if scale == 1.0 else d * scale)
     return grad_weight
 
 

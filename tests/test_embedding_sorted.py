@@ -1,0 +1,212 @@
+"""Embedding lookup with a scale and its gradient by sorted tokens, against plain statements in 64 bits.
+
+A looked-up value is one product in fp32 (2^-24) rounded to bf16 (2^-8).  The gradient of a row is a sum of n rows in fp32, each
+addition off by at most 2^-24 of the sum of their sizes, times the scale, plus the addition to what was there."""
+import pytest
+import torch
+
+from kareus_b200 import kernels as K
+from kareus_b200.kernels.cuda import KernelError
+
+gpu = pytest.mark.gpu
+
+
+def reference(tokens, weight, dout, grad, start, scale):
+    """(out, grad, number of tokens of each row, sum of the sizes) in 64 bits."""
+    v, H = weight.shape
+    ids = (tokens.reshape(-1) - start)
+    keep = torch.nonzero((ids >= 0) & (ids < v)).flatten()
+    out = torch.zeros(ids.numel(), H, dtype=torch.float64, device=weight.device)
+    out[keep] = weight.double()[ids[keep]] * scale
+    d = dout.reshape(-1, H).double()[keep] * scale
+    g, size = grad.double(), grad.double().abs()
+    g.index_put_((ids[keep],), d, accumulate=True)
+    size.index_put_((ids[keep],), d.abs(), accumulate=True)
+    n = torch.bincount(ids[keep], minlength=v)
+    return out.view(tuple(tokens.shape) + (H,)), g, n, size
+
+
+def check(tokens, weight, start, scale, seed=1):
+    gen = torch.Generator().manual_seed(seed)
+    H = weight.shape[1]
+    dout = torch.randn(tuple(tokens.shape) + (H,), generator=gen).bfloat16().to(weight.device)
+    grad = torch.randn(weight.shape, generator=gen).to(weight.device)
+    out, want, n, size = reference(tokens, weight, dout, grad, start, scale)
+    got = K.embedding_fwd(tokens, weight, start, scale=scale)
+    assert got.dtype == weight.dtype and bool(((got.double() - out).abs() <= 2.0 ** -8 * 1.0001 * out.abs()).all())
+    runs = []
+    for _ in range(2):
+        g = grad.clone()
+        assert K.embedding_bwd(dout, tokens, g, start, scale=scale, order="sorted") is g
+        runs.append(g)
+    assert torch.equal(*runs)                                      # the same bits every time
+    limit = 2.0 ** -24 * (n[:, None].double() + 3) * size
+    off = ((runs[0].double() - want).abs() - limit).max().item()
+    assert off <= 0, off
+    assert torch.equal(runs[0][n == 0], grad[n == 0])              # rows without tokens as they were
+
+
+def table(v, H, device="cuda", seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(v, H, generator=g).bfloat16().to(device)
+
+
+def draw(n, total, skew=1.0, seed=2, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    return ((torch.rand(n, generator=g, dtype=torch.float64) ** skew) * total).long().to(device)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("n, v, H", [(1, 1, 8), (1, 5, 1), (7, 3, 24), (64, 10, 136), (33, 100, 64)])
+@pytest.mark.parametrize("scale", [1.0, 64.0, 1.3])
+def test_small(device, n, v, H, scale):
+    check(draw(n, v, device=device), table(v, H, device), 0, scale)
+    check(draw(n, 3 * v, device=device).view(1, n, 1), table(v, H, device), v, scale)      # middle one of three shards
+
+
+@gpu
+@pytest.mark.parametrize("n", [2, 31, 32, 33, 255, 257, 1000, 4097, 8192, 30001, 65536, 65537, 150000])
+def test_lengths(n):
+    check(draw(n, 500, 2), table(500, 16), 0, 1.0)
+
+
+@gpu
+@pytest.mark.parametrize("v", [1, 2, 255, 256, 257, 511, 65535, 65536, 128256])
+def test_vocabularies(v):
+    """Every number of digits of the sort, each with keys at both ends."""
+    t = draw(3000, v, 3)
+    t[5], t[6], t[-1] = v - 1, 0, v - 1
+    check(t, table(v, 8), 0, 2.0)
+
+
+@gpu
+@pytest.mark.parametrize("H", [1, 7, 8, 72, 520, 1020, 1024, 1032, 2048, 4096])
+def test_widths(H):
+    check(draw(700, 90), table(90, H), 0, 1.0)
+    check(draw(700, 90, seed=4).view(100, 7), table(30, H), 30, 0.5)
+
+
+@gpu
+@pytest.mark.parametrize("n", [63, 64, 65, 128, 700, 5000, 20000])
+@pytest.mark.parametrize("share", [0.5, 0.97, 1.0])
+def test_one_token_many_times(n, share):
+    """Padding: runs that cross windows, fill them, end at their borders."""
+    t = draw(n, 40)
+    t[: int(n * share)] = 17
+    t = t[torch.randperm(n, generator=torch.Generator().manual_seed(3)).to(t.device)]
+    check(t, table(40, 264), 0, 1.0)
+    check(torch.full((n,), 39, device="cuda"), table(40, 264), 0, 3.0)
+
+
+@gpu
+def test_runs_of_every_length():
+    """Sorted tokens whose runs start and end at every place of a window."""
+    runs = torch.arange(1, 200)
+    t = torch.repeat_interleave(torch.arange(199), runs).cuda()
+    check(t, table(199, 2048), 0, 1.0)
+    check(t.flip(0), table(199, 24), 0, 1.0)
+
+
+@gpu
+def test_tokens_of_no_row():
+    w = table(50, 64)
+    for t in (torch.full((300,), 50), torch.full((300,), -1), torch.tensor([-2 ** 62, 2 ** 62, 49, 0, 2 ** 32 + 3])):
+        check(t.cuda(), w, 0, 1.0)
+    check(draw(100, 50), w, 2 ** 40, 1.0)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """A gradient of more than 2^32 bytes: the last rows of a large table."""
+    v, H = 300000, 4096
+    t = torch.tensor([v - 1, 5, v - 1, v - 2, 262144], device="cuda")
+    dout = torch.randn(5, H, device="cuda").bfloat16()
+    grad = torch.zeros(v, H, device="cuda")
+    K.embedding_bwd(dout, t, grad, 0, order="sorted")
+    d = dout.float()
+    for row, want in ((v - 1, d[0] + d[2]), (5, d[1]), (v - 2, d[3]), (262144, d[4])):
+        assert torch.equal(grad[row], want)
+        grad[row] = 0
+    assert not bool(grad.any())
+
+
+@gpu
+def test_views_and_streams():
+    base = torch.randn(300, 1, 80, device="cuda").bfloat16()
+    t = draw(300, 20).view(300, 1)
+    w = table(20, 64)
+    g0 = torch.zeros(20, 64, device="cuda")
+    K.embedding_bwd(base[..., 8:72].contiguous(), t, g0, 0, order="sorted")
+    g1 = torch.zeros(20, 64, device="cuda")
+    K.embedding_bwd(base[..., 8:72], t, g1, 0, order="sorted")     # a strided gradient
+    assert torch.equal(g0, g1)
+    flat = torch.zeros(20 * 64 + 1, device="cuda")
+    g2 = flat[1:].view(20, 64)                                     # a gradient that starts on no 16-byte boundary
+    K.embedding_bwd(base[..., 8:72], t, g2, 0, order="sorted")
+    assert torch.equal(g0, g2) and flat[0].item() == 0
+    torch.cuda.synchronize()
+    outs = []
+    for s in (torch.cuda.Stream(), torch.cuda.Stream()):
+        with torch.cuda.stream(s):
+            g = torch.zeros(20, 64, device="cuda")
+            K.embedding_bwd(base[..., 8:72].contiguous(), t, g, 0, order="sorted")
+            outs.append(g)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, g0) for g in outs)
+    grad, d, tok = torch.zeros(20, 64, device="cuda"), base[..., 8:72].contiguous(), t.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.embedding_bwd(d, tok, grad, 0, order="sorted")
+    for seed in (5, 6):
+        tok.copy_(draw(300, 20, seed=seed).view(300, 1))
+        grad.zero_()
+        graph.replay()
+        want = torch.zeros(20, 64, device="cuda")
+        K.embedding_bwd(d, tok, want, 0, order="sorted")
+        assert torch.equal(grad, want)
+
+
+@gpu
+def test_not_finite():
+    t = torch.tensor([3, 4, 3, 9], device="cuda")
+    d = torch.ones(4, 16, device="cuda").bfloat16()
+    d[2, 5], d[1, 0], d[3, 2] = float("inf"), float("nan"), float("nan")
+    g = torch.zeros(9, 16, device="cuda")
+    K.embedding_bwd(d, t, g, 0, order="sorted")                    # the last token belongs to another shard
+    assert g[3, 5].isinf() and g[4, 0].isnan() and torch.isfinite(g).sum() == 9 * 16 - 2
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_gradient_is_that_of_the_lookup(device):
+    """<dout, lookup(W + E) - lookup(W)> = <gradient, E>: the lookup is linear in its table."""
+    t = draw(200, 30, device=device)
+    dout, e = table(200, 24, device, 3), table(20, 24, device, 4)
+    g = torch.zeros(20, 24, device=device)
+    K.embedding_bwd(dout, t, g, 5, scale=2.0, order="sorted")
+    left = (dout.double() * K.embedding_fwd(t, e, 5, scale=2.0).double()).sum()        # times 2 is exact in bf16
+    assert (left - (g.double() * e.double()).sum()).abs() < 1e-5 * left.abs() + 1e-3
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_empty_and_refusals(device):
+    w, g = table(10, 16, device), torch.zeros(10, 16, device=device)
+    none = torch.empty(0, dtype=torch.int64, device=device)
+    assert tuple(K.embedding_fwd(none, w, 0, scale=2.0).shape) == (0, 16)
+    K.embedding_bwd(torch.empty(0, 16, dtype=torch.bfloat16, device=device), none, g, 0, order="sorted")
+    assert not bool(g.any())
+    with pytest.raises((KernelError, ValueError), match="order"):
+        K.embedding_bwd(w[:3].contiguous(), torch.zeros(3, dtype=torch.int64, device=device), g, 0, order="random")
+
+
+@gpu
+def test_gpu_refusals():
+    w, g = table(10, 16), torch.zeros(10, 16, device="cuda")
+    t = torch.zeros(3, dtype=torch.int64, device="cuda")
+    with pytest.raises(KernelError, match="int64"):
+        K.embedding_fwd(t.int(), w, 0, scale=2.0)
+    with pytest.raises(KernelError, match="gradient of shape"):
+        K.embedding_bwd(w[:2].contiguous(), t, g, 0, order="sorted")
+    with pytest.raises(KernelError, match="contiguous"):
+        K.embedding_bwd(w[:3].contiguous(), t, torch.zeros(16, 10, device="cuda").t(), 0, order="sorted")
+    with pytest.raises(KernelError, match="current device"):
+        K.embedding_fwd(t.cpu(), w, 0, scale=2.0)
