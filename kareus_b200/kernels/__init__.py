@@ -24,9 +24,10 @@ import torch
 from . import ref
 
 _LAUNCHES = [0]
-# The native calls of csrc/torch/fastcall.cpp, once the library is loaded.  Each returns None for a call that it leaves to
-# the statements below it.
+# The native calls of csrc/torch/fastcall.cpp and opcalls.cpp, once the library is loaded.  Each returns None for a call that it
+# leaves to the statements below it.
 _FAST = None
+_OPS = None
 
 
 def launch_count() -> int:
@@ -162,6 +163,11 @@ def gemm(a, b, trans_a=False, trans_b=True, out_dtype=None, accumulate=None, out
 
 
 # ----------------------------------------------------------------------------- 8-bit floating point
+def _fp8():
+    from . import fp8
+    return fp8
+
+
 def fp8_quantize(x, rows=True, cols=False, square=False, fmt="e4m3"):
     """``(r, c)``: the matrix ``x`` in 8 bits for a product along its rows, and its transpose for a product along its columns
     (:class:`.fp8.Fp8Matrix`; ``None`` for the one that is not wanted), both from one pass over ``x``.
@@ -169,16 +175,14 @@ def fp8_quantize(x, rows=True, cols=False, square=False, fmt="e4m3"):
     A piece of 1 x 128 elements along the contraction (activations, gradients), or of 128 x 128 with ``square`` (weights), is held
     as ``q * 2^E`` with the smallest whole ``E`` under which it fits the format (``"e4m3"``: 448, ``"e5m2"``: 57344) and ``q``
     rounded to nearest even.  A piece with an infinity or a NaN stands for NaN as a whole."""
-    from .fp8 import quantize
-    return quantize(x, rows, cols, square, fmt)
+    return _fp8().quantize(x, rows, cols, square, fmt)
 
 
 def fp8_gemm(a, b, out_dtype=None, accumulate=None, out=None):
     """``a @ b.T`` of two :class:`.fp8.Fp8Matrix`, summed in fp32; bf16 unless ``out_dtype`` or ``out`` says fp32.  ``accumulate``
     is an fp32 tensor that receives ``+=``.  With ``(xr, xc) = fp8_quantize(x, cols=True)``, the same of ``dy`` and, square, of
     ``w``, a linear layer is ``y = fp8_gemm(xr, wr)``, ``dx = fp8_gemm(dr, wc)``, ``fp8_gemm(dc, xc, accumulate=dw)``."""
-    from .fp8 import gemm as f
-    return f(a, b, out_dtype, accumulate, out)
+    return _fp8().gemm(a, b, out_dtype, accumulate, out)
 
 
 # ----------------------------------------------------------------------------- attention
@@ -296,6 +300,10 @@ def cross_entropy_finish(logits, targets, vocab_start, gmax, gsum, grad_scale):
 def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
     """``scale`` times the rows of ``weight`` for tokens in ``[vocab_start, vocab_start + rows)``, zeros for others; the product is
     rounded once to the table's type."""
+    if _OPS is not None:
+        r = _OPS.embedding_fwd(tokens, weight, vocab_start, scale)
+        if r is not None:
+            return r
     if is_cuda(weight):
         return _cuda().embedding_fwd(tokens, weight, vocab_start, scale)
     return ref.embedding_fwd(tokens, weight, vocab_start, scale)

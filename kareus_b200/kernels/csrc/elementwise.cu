@@ -7,6 +7,7 @@
 //   fused AdamW over flat buffers, sum of squares (reference: TE/Apex multi_tensor kernels)
 #include <cuda_bf16.h>
 #include "launch.h"
+#include "native_ops.h"
 #include "pdl.cuh"
 #include "host_utils.h"
 #include <cuda_runtime.h>

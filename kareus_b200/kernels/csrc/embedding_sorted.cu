@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 #include "sm100.cuh"
 #include "launch.h"
+#include "native_ops.h"
 #include "pdl.cuh"
 #include "host_utils.h"
 

@@ -16,6 +16,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include "launch.h"
+#include "native_ops.h"
 #include "pdl.cuh"
 
 namespace kb {

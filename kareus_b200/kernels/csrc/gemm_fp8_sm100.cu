@@ -16,6 +16,7 @@
 // soon as they are read.
 #include "sm100.cuh"
 #include "launch.h"
+#include "native_ops.h"
 #include "pdl.cuh"
 #include "host_utils.h"
 

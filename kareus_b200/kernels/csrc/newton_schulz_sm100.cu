@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 #include "sm100.cuh"
 #include "launch.h"
+#include "native_ops.h"
 #include "pdl.cuh"
 #include "host_utils.h"
 

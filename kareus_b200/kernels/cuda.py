@@ -9,6 +9,7 @@ library is missing: there is no PyTorch fallback for bf16 CUDA tensors.  fp32/fp
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 from ctypes import c_float, c_int, c_long, c_uint, c_void_p
 from pathlib import Path
@@ -40,29 +41,30 @@ def lib() -> ctypes.CDLL:
                 "(bf16 CUDA tensors have no PyTorch fallback)")
         L = ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
         _declare(L)
-        _load_fastcall()
+        _load_modules()
         _LIB = L
     return _LIB
 
 
-def _load_fastcall() -> None:
-    """The extension module that takes plain GEMM and attention calls without the statements of this file.  They run all calls
-    where it is missing or was built for another PyTorch."""
+def _load_modules() -> None:
+    """The extension modules that take plain calls without the statements of this package's Python files.  Those run all calls
+    where a module is missing or was built for another PyTorch."""
     import kareus_b200.kernels as K
-    try:
-        from . import _fastcall
-        built_for = getattr(_fastcall, "torch_version", "of another version")
-        if built_for != torch.__version__:
-            raise ImportError(f"built for PyTorch {built_for}, this is {torch.__version__}")
-    except ImportError as e:
-        import warnings
-        warnings.warn(f"{_HERE / '_fastcall.so'} cannot be loaded ({e}): GEMM and attention calls take more host time; build it "
-                      "with `python -m kareus_b200.kernels.build`", RuntimeWarning, stacklevel=3)
-        return
-    _fastcall.init(K._LAUNCHES, _check)
-    for idx, t in _STATUS.items():
-        _fastcall.set_status(idx, t.data_ptr())
-    K._FAST = _fastcall
+    for name, slot, calls in (("_fastcall", "_FAST", "GEMM and attention"), ("_opcalls", "_OPS", "8-bit, Newton-Schulz and embedding")):
+        try:
+            module = importlib.import_module(f"{__package__}.{name}")
+            built_for = getattr(module, "torch_version", "of another version")
+            if built_for != torch.__version__:
+                raise ImportError(f"built for PyTorch {built_for}, this is {torch.__version__}")
+        except ImportError as e:
+            import warnings
+            warnings.warn(f"{_HERE / name}.so cannot be loaded ({e}): {calls} calls take more host time; build it "
+                          "with `python -m kareus_b200.kernels.build`", RuntimeWarning, stacklevel=3)
+            continue
+        module.init(K._LAUNCHES, _check)
+        for idx, t in _STATUS.items():
+            module.set_status(idx, t.data_ptr())
+        setattr(K, slot, module)
 
 
 def is_loaded() -> bool:
@@ -197,9 +199,10 @@ def status_word(device) -> torch.Tensor:
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=f"cuda:{idx}")
         _STATUS[idx] = t
-        from . import _FAST
-        if _FAST is not None:
-            _FAST.set_status(idx, t.data_ptr())
+        from . import _FAST, _OPS
+        for module in (_FAST, _OPS):
+            if module is not None:
+                module.set_status(idx, t.data_ptr())
     return t
 
 
@@ -728,6 +731,7 @@ def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
     if not _bf16(weight):
         return ref.embedding_fwd(tokens, weight, vocab_start, scale)
     _embedding_args("embedding_fwd", tokens, weight)
+    status_word(weight.device)                # the native call takes over from the next one on
     tokens = tokens.contiguous()
     H = weight.shape[1]
     out = torch.empty(tuple(tokens.shape) + (H,), dtype=weight.dtype, device=weight.device)
@@ -746,6 +750,12 @@ def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
 def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"):
     if order not in EMBEDDING_ORDERS:
         raise KernelError(f"unknown order {order!r} of embedding gradients; known: {EMBEDDING_ORDERS}")
+    if order == "sorted":
+        from . import _OPS
+        if _OPS is not None:
+            r = _OPS.embedding_bwd_sorted(dout, tokens, grad_weight, vocab_start, scale, 3 * -(-tokens.numel() // EMBEDDING_CHUNK))
+            if r is not None:
+                return r
     if not _bf16(dout) or grad_weight.dtype != torch.float32:
         return ref.embedding_bwd(dout, tokens, grad_weight, vocab_start, scale, order)
     _embedding_args("embedding_bwd", tokens, grad_weight, dout)
@@ -758,6 +768,7 @@ def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"
         return grad_weight
     L = lib()
     if order == "sorted" or scale != 1.0:
+        status_word(dout.device)              # the native call takes over from the next one on
         work = torch.empty(L.kb_embedding_sorted_bytes(n, H), dtype=torch.uint8, device=dout.device)
         _check(L.kb_embedding_bwd_sorted(tokens.data_ptr(), dout.data_ptr(), grad_weight.data_ptr(), n, H, int(vocab_start),
                                          grad_weight.shape[0], float(scale), work.data_ptr(), _stream()), "embedding_bwd")

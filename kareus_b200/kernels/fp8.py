@@ -4,24 +4,28 @@ The contract of both calls is at :func:`kareus_b200.kernels.fp8_quantize` and :f
 ``csrc/fp8_quantize.cu`` and ``csrc/gemm_fp8_sm100.cu``, the PyTorch statements are in :mod:`.ref`."""
 from __future__ import annotations
 
-from dataclasses import dataclass
-
 import torch
+
+import kareus_b200.kernels as _entry
 
 from . import ref
 from .cuda import KernelError, _check, _count, _rows_readable, _stream, lib, require_current_device, status_word
 
 _FORMAT_CODE = {"e4m3": 0, "e5m2": 1}
+_DTYPE = {fmt: ref.FP8_FORMATS[fmt][0] for fmt in _FORMAT_CODE}
 
 
-@dataclass(frozen=True)
 class Fp8Matrix:
     """``data`` (``[rows, cols]``, one byte each) times the powers of two in ``scales`` (uint8, ``[row blocks, piece blocks, 32, 4,
     4]``: see :func:`.ref.fp8_pack_scales`).  Pieces run along the rows, which is the direction that a product contracts."""
 
-    data: torch.Tensor
-    scales: torch.Tensor
-    fmt: str = "e4m3"
+    __slots__ = ("data", "scales", "fmt")
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor, fmt: str = "e4m3"):
+        self.data, self.scales, self.fmt = data, scales, fmt
+
+    def __repr__(self):
+        return f"Fp8Matrix({tuple(self.data.shape)}, {self.fmt}, {self.data.device})"
 
     @property
     def shape(self):
@@ -52,6 +56,10 @@ def _empty(rows: int, cols: int, fmt: str, device) -> Fp8Matrix:
 
 
 def quantize(x, rows: bool = True, cols: bool = False, square: bool = False, fmt: str = "e4m3"):
+    if _entry._OPS is not None and fmt in _FORMAT_CODE:
+        r = _entry._OPS.fp8_quantize(x, rows, cols, square, _FORMAT_CODE[fmt])
+        if r is not None:
+            return (None if r[0] is None else Fp8Matrix(r[0], r[1], fmt)), (None if r[2] is None else Fp8Matrix(r[2], r[3], fmt))
     if fmt not in _FORMAT_CODE:
         raise KernelError(f"unknown 8-bit format {fmt!r}; known: {sorted(_FORMAT_CODE)}")
     if x.dim() != 2 or not x.is_floating_point():
@@ -64,6 +72,7 @@ def quantize(x, rows: bool = True, cols: bool = False, square: bool = False, fmt
         return (Fp8Matrix(*ref.fp8_quantize(x, fmt, square), fmt) if rows else None,
                 Fp8Matrix(*ref.fp8_quantize(x.t(), fmt, square), fmt) if cols else None)
     require_current_device("fp8_quantize", x)
+    status_word(x.device)                     # the native call takes over from the next one on
     M, N = x.shape
     r = _empty(M, N, fmt, x.device) if rows else None
     c = _empty(N, M, fmt, x.device) if cols else None
@@ -88,6 +97,11 @@ def _operand(m: Fp8Matrix, what: str):
 
 
 def gemm(a: Fp8Matrix, b: Fp8Matrix, out_dtype=None, accumulate=None, out=None):
+    if (_entry._OPS is not None and out is None and out_dtype is None and type(a) is Fp8Matrix and type(b) is Fp8Matrix
+            and _DTYPE.get(a.fmt) is a.data.dtype and _DTYPE.get(b.fmt) is b.data.dtype):
+        r = _entry._OPS.fp8_gemm(a.data, a.scales, b.data, b.scales, accumulate)
+        if r is not None:
+            return r
     _check_matrix(a, "fp8_gemm a")
     _check_matrix(b, "fp8_gemm b")
     (M, K), (N, Kb) = a.shape, b.shape

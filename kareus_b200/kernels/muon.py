@@ -8,6 +8,8 @@ import math
 
 import torch
 
+import kareus_b200.kernels as _entry
+
 from . import ref
 from .cuda import KernelError, _check, _count, _no_recording, _stream, lib, require_current_device, status_word
 
@@ -52,6 +54,10 @@ def _launches(steps: int) -> int:
 
 def orthogonalize(x, steps, coefficients, eps):
     steps, coefficients, eps = _parameters(steps, coefficients, eps)
+    if _entry._OPS is not None and x.is_cuda:
+        r = _entry._OPS.orthogonalize(x, *coefficients, steps, eps, fp16_scale(steps, coefficients), _launches(steps))
+        if r is not None:
+            return r
     if x.dim() < 2 or not x.is_floating_point():
         raise KernelError(f"orthogonalize takes matrices of floating-point numbers, got {x.dtype} of shape {tuple(x.shape)}")
     if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32)):
