@@ -47,20 +47,22 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
 __device__ __forceinline__ float inverse_scale(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : (254u - byte) << 23);
 }
-// Two bf16 (packed), scaled, as two bytes; the low half goes to the low byte.
+// Two values as two bytes; `lo` goes to the low one.
 template <bool E5M2>
-__device__ __forceinline__ uint32_t quantize2(uint32_t v, float inv) {
-  const float lo = __uint_as_float(v << 16) * inv, hi = __uint_as_float(v & 0xffff0000u) * inv;
+__device__ __forceinline__ uint32_t quantize2(float lo, float hi) {
   uint16_t r;
   if constexpr (E5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// The same for two values of one column that come from two packed pairs.
-template <bool E5M2, bool HIGH>
-__device__ __forceinline__ uint32_t quantize_col(uint32_t a, uint32_t b, float inv) {
-  const uint32_t v = __byte_perm(a, b, HIGH ? 0x7632 : 0x5410);
-  return quantize2<E5M2>(v, inv);
+// The two bf16 of a word, each times its factor.
+__device__ __forceinline__ float2 scaled(uint32_t v, float2 inv) {
+  return __fmul2_rn(make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)), inv);
+}
+// Larger |x| of two pairs of bf16, element by element; a NaN stays one.
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
+  return *reinterpret_cast<const uint32_t*>(&m);
 }
 
 // Where the scale of (row, piece) lies.
@@ -76,17 +78,18 @@ __device__ __forceinline__ void put_scale(uint8_t* s, int row, int piece, int pi
 }
 
 template <bool E5M2, bool SQUARE>
-__global__ void __launch_bounds__(FQ_THREADS) fp8_quantize_kernel(const Fp8Quantize p) {
+__global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Quantize p) {
   __shared__ __align__(16) uint32_t tile[128 * FQ_PITCH];
-  __shared__ uint32_t part[4][128];
+  __shared__ uint32_t part[4][64];
   __shared__ uint32_t whole[FQ_THREADS / 32];
+  __shared__ uint8_t row_byte[128], col_byte[128];
   constexpr int TOP = E5M2 ? 16 : 9;
   pdl_begin();
   const int tr = blockIdx.x / p.tiles_c, tc = blockIdx.x - tr * p.tiles_c;
   const int r0 = tr * 128, c0 = tc * 128;
   const int tid = threadIdx.x, unit = tid & 15, rsub = tid >> 4;
   const int col = c0 + unit * 8;
-  uint4 v[8];
+  uint4 v[8];                                   // rows r0 + rsub + 16 i, columns col .. col + 7
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = r0 + i * 16 + rsub;
@@ -104,14 +107,12 @@ __global__ void __launch_bounds__(FQ_THREADS) fp8_quantize_kernel(const Fp8Quant
       }
     }
   }
-  constexpr uint32_t ABS = 0x7fff7fffu;
   uint32_t block_byte = 0;
   if constexpr (SQUARE) {
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      m = __vmaxu2(__vmaxu2(__vmaxu2(m, v[i].x & ABS), __vmaxu2(v[i].y & ABS, v[i].z & ABS)), v[i].w & ABS);
-    m = max(m & 0xffffu, m >> 16);
+    for (int i = 0; i < 8; ++i) m = max_abs2(m, max_abs2(max_abs2(v[i].x, v[i].y), max_abs2(v[i].z, v[i].w)));
+    m = max(m & 0x7fffu, m >> 16);
     m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) whole[tid >> 5] = m;
     __syncthreads();
@@ -121,63 +122,82 @@ __global__ void __launch_bounds__(FQ_THREADS) fp8_quantize_kernel(const Fp8Quant
     block_byte = scale_byte<TOP>(m);
   }
   if (p.q) {
+    uint32_t byte[8];
+    if constexpr (!SQUARE) {
+      // two rows' maxima in a word, over the 16 lanes that hold the rows
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const uint32_t a = max_abs2(max_abs2(v[i].x, v[i].y), max_abs2(v[i].z, v[i].w));
+        const uint32_t b = max_abs2(max_abs2(v[i + 1].x, v[i + 1].y), max_abs2(v[i + 1].z, v[i + 1].w));
+        uint32_t m = max_abs2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+        for (int s = 8; s > 0; s >>= 1) m = max_abs2(m, __shfl_xor_sync(0xffffffffu, m, s));
+        byte[i] = scale_byte<TOP>(m & 0x7fffu);
+        byte[i + 1] = scale_byte<TOP>(m >> 16);
+      }
+    }
+    uint8_t* dst = p.q + (r0 + rsub) * p.ldq + col;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int row = r0 + i * 16 + rsub;
-      uint32_t byte = block_byte;
-      if constexpr (!SQUARE) {
-        uint32_t m = __vmaxu2(__vmaxu2(v[i].x & ABS, v[i].y & ABS), __vmaxu2(v[i].z & ABS, v[i].w & ABS));
-#pragma unroll
-        for (int s = 8; s > 0; s >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, s));
-        byte = scale_byte<TOP>(max(m & 0xffffu, m >> 16));
-      }
-      if (row < p.rows && col < p.ldq) {
-        const float inv = inverse_scale(byte);
-        uint2 o;
-        o.x = quantize2<E5M2>(v[i].x, inv) | quantize2<E5M2>(v[i].y, inv) << 16;
-        o.y = quantize2<E5M2>(v[i].z, inv) | quantize2<E5M2>(v[i].w, inv) << 16;
-        *reinterpret_cast<uint2*>(p.q + row * p.ldq + col) = o;
-      }
-      if (unit == 0) put_scale(p.s, row, tc, p.tiles_c, row < p.rows ? byte : 0u);
+      if constexpr (SQUARE) byte[i] = block_byte;
+      const float f = inverse_scale(byte[i]);
+      const float2 inv = make_float2(f, f);
+      const float2 a = scaled(v[i].x, inv), b = scaled(v[i].y, inv), c = scaled(v[i].z, inv), d = scaled(v[i].w, inv);
+      const uint2 o = make_uint2(quantize2<E5M2>(a.x, a.y) | quantize2<E5M2>(b.x, b.y) << 16,
+                                 quantize2<E5M2>(c.x, c.y) | quantize2<E5M2>(d.x, d.y) << 16);
+      if (r0 + i * 16 + rsub < p.rows && col < p.ldq) *reinterpret_cast<uint2*>(dst) = o;
+      dst += 16 * p.ldq;
+      if (unit == 0) row_byte[i * 16 + rsub] = static_cast<uint8_t>(byte[i]);
     }
   }
-  if (!p.qt) return;
+  if (p.qt) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    *reinterpret_cast<uint4*>(tile + (i * 16 + rsub) * FQ_PITCH + unit * 4) = v[i];
+    for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(tile + (i * 16 + rsub) * FQ_PITCH + unit * 4) = v[i];
+    __syncthreads();
+    const int pair = tid & 63, rg = tid >> 6;             // two columns, 32 rows
+    uint32_t w[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) w[j] = tile[(rg * 32 + j) * FQ_PITCH + pair];
+    uint32_t b0 = block_byte, b1 = block_byte;
+    if constexpr (!SQUARE) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) m = max_abs2(m, w[j]);
+      part[rg][pair] = m;
+      __syncthreads();
+      m = max_abs2(max_abs2(part[0][pair], part[1][pair]), max_abs2(part[2][pair], part[3][pair]));
+      b0 = scale_byte<TOP>(m & 0x7fffu);
+      b1 = scale_byte<TOP>(m >> 16);
+    }
+    if (rg == 0) {
+      col_byte[2 * pair] = static_cast<uint8_t>(b0);
+      col_byte[2 * pair + 1] = static_cast<uint8_t>(b1);
+    }
+    const float2 inv = make_float2(inverse_scale(b0), inverse_scale(b1));
+    const int c = c0 + 2 * pair, r = r0 + rg * 32;
+    uint8_t* dst = p.qt + c * p.ldqt + r;                 // ldqt is a multiple of 16: 16-byte units are whole or outside
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t lo[4], hi[4];                              // 16 rows of either column
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t* x = w + half * 16 + 4 * j;
+        const float2 e = scaled(x[0], inv), f = scaled(x[1], inv), g = scaled(x[2], inv), h = scaled(x[3], inv);
+        lo[j] = quantize2<E5M2>(e.x, f.x) | quantize2<E5M2>(g.x, h.x) << 16;
+        hi[j] = quantize2<E5M2>(e.y, f.y) | quantize2<E5M2>(g.y, h.y) << 16;
+      }
+      if (r + half * 16 < p.ldqt) {
+        if (c < p.cols) *reinterpret_cast<uint4*>(dst + half * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (c + 1 < p.cols) *reinterpret_cast<uint4*>(dst + p.ldqt + half * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      }
+    }
   }
   __syncthreads();
-  const int pair = tid & 63, rg = tid >> 6;             // two columns, 32 rows
-  uint32_t w[32];
-#pragma unroll
-  for (int j = 0; j < 32; ++j) w[j] = tile[(rg * 32 + j) * FQ_PITCH + pair];
-  uint32_t b0 = block_byte, b1 = block_byte;
-  const int tiles_r = (p.rows + 127) >> 7;
-  if constexpr (!SQUARE) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) m = __vmaxu2(m, w[j] & ABS);
-    part[rg][pair] = m;
-    __syncthreads();
-    m = __vmaxu2(__vmaxu2(part[0][pair], part[1][pair]), __vmaxu2(part[2][pair], part[3][pair]));
-    b0 = scale_byte<TOP>(m & 0xffffu);
-    b1 = scale_byte<TOP>(m >> 16);
-  }
-  const int c = c0 + 2 * pair, r = r0 + rg * 32;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const float inv = inverse_scale(h ? b1 : b0);
-    uint32_t o[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      o[j] = h ? quantize_col<E5M2, true>(w[4 * j], w[4 * j + 1], inv) | quantize_col<E5M2, true>(w[4 * j + 2], w[4 * j + 3], inv) << 16
-               : quantize_col<E5M2, false>(w[4 * j], w[4 * j + 1], inv) | quantize_col<E5M2, false>(w[4 * j + 2], w[4 * j + 3], inv) << 16;
-    if (c + h < p.cols) {
-      uint8_t* dst = p.qt + (c + h) * p.ldqt + r;       // ldqt is a multiple of 16: 16-byte units are whole or outside
-      if (r < p.ldqt) *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-      if (r + 16 < p.ldqt) *reinterpret_cast<uint4*>(dst + 16) = make_uint4(o[4], o[5], o[6], o[7]);
-    }
-    if (rg == 0) put_scale(p.st, c + h, tr, tiles_r, c + h < p.cols ? (h ? b1 : b0) : 0u);
+  const int i = tid & 127;
+  if (tid < 128) {
+    if (p.q) put_scale(p.s, r0 + i, tc, p.tiles_c, r0 + i < p.rows ? row_byte[i] : 0u);
+  } else if (p.qt) {
+    put_scale(p.st, c0 + i, tr, (p.rows + 127) >> 7, c0 + i < p.cols ? col_byte[i] : 0u);
   }
 }
 

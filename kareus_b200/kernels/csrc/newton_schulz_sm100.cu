@@ -10,7 +10,15 @@
 // that of P's diagonal (about -2.6 beside entries near 0), so the diagonal stays in fp32, outside P: X <- (a + diag P) X + (P - diag
 // P) X.  Norms are summed in fp32 per thread and fp64 beyond, in a fixed order.
 //
-// G and P are symmetric: only the tiles on and above the diagonal are computed, the others are written as their transposes.
+// Long matrices.  X_{k+1} = Q_k X_k with Q_k = a I + P_k, and G_{k+1} = Q_k G_k Q_k, where everything but X is as small as the shorter
+// side.  Where the longer side is at least 1.5 times the shorter one and that is long enough to be bound by arithmetic, G is carried from step to step so (T = Q G, G' = Q T), the Q are
+// multiplied up, and X is read twice per segment of two or three steps instead of twice per step: five steps of a matrix with
+// sides m and r m take 6 r + 14 units of m^3 multiplications instead of 15 r + 5.  G of a carried step is off by the roundings
+// before it, and small singular values suffer most from that; with segments of three and two steps (the singular values grow in
+// the first, settle in the second) the result is as exact as step by step, with one of five it would not be.
+//
+// G, P, T and the products of the Q are symmetric: only the tiles on and above the diagonal are computed, the others are written as
+// their transposes.
 //
 // One 256 x BN tile per two-CTA cluster (tcgen05 cta_group::2), roles as in gemm_pair_sm100.cu:
 //   warp 0      TMA producer of this CTA's halves
@@ -38,19 +46,25 @@ static_assert(NS_SMEM <= 227 * 1024, "shared memory per CTA");
 
 enum NsMode : int {
   NS_GRAM = 0,       // G = X Xt
-  NS_POLY = 1,       // P = b G + c G G; diagonal apart
+  NS_POLY = 1,       // P = b G + c G G; diagonal d apart
   NS_UPDATE = 2,     // X <- (a + d) X + P X
   NS_UPDATE_T = 3,   // X <- X (a + d) + X P
+  NS_CARRY = 4,      // Y <- (a + d) Y + P Y for symmetric Y that P commutes with
+  NS_APPLY = 5,      // X <- Q X or X Q
 };
+__host__ __device__ constexpr bool ns_symmetric(int mode) { return mode == NS_GRAM || mode == NS_POLY || mode == NS_CARRY; }
+__host__ __device__ constexpr bool ns_adds(int mode) { return mode != NS_GRAM && mode != NS_APPLY; }
 
 struct NsWork {
-  int batch, tiles_m, tiles_n, per_matrix, nk;
+  int batch, pairs, tiles_m, tiles_n, per_matrix, nk;      // pairs: matrices per item of the batch (NS_CARRY takes G and Q at once)
   int ratio;                                   // column tiles per 256 rows, where only the upper tiles are computed; else 0
   int group_m;
-  __device__ __forceinline__ int units() const { return batch * per_matrix; }
-  __device__ __forceinline__ void decode(int u, int& z, int& tm, int& tn) const {
+  __device__ __forceinline__ int units() const { return pairs * batch * per_matrix; }
+  __device__ __forceinline__ void decode(int u, int& pair, int& z, int& tm, int& tn) const {
     z = u / per_matrix;
     int t = u - z * per_matrix;
+    pair = z / batch;
+    z -= pair * batch;
     if (ratio) {                               // row after row of the upper triangle
       tm = 0;
       for (int len = tiles_n; t >= len; len -= ratio) { t -= len; ++tm; }
@@ -65,13 +79,15 @@ struct NsWork {
 };
 
 struct NsEpilogue {
-  const __half* e;           // tile that is added (G or X): [batch][M][lde]
-  long e_batch;
+  const __half* e;           // matrix that is added (G, X or Y): [pairs][batch][M][lde]
+  long e_batch, e_pair;
   int lde, e_cols;           // e_cols: columns to read, a multiple of 8
   float alpha, coef;         // accumulator's factor, e's factor
   float* diag;               // [batch][diag_len]: diagonal of P, written by NS_POLY, read by the updates
   int diag_len;
   float unit;                // 1 / scale
+  float coef2;               // a * scale
+  float also;                // NS_POLY: a I + P times this goes to a second matrix; 0: not wanted
   __nv_bfloat16* out;        // last update: the result, [batch][M][N]
   bool last;
 };
@@ -81,16 +97,11 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn, b
   return (1u << 4) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | (static_cast<uint32_t>(N >> 3) << 17) |
          (static_cast<uint32_t>(M >> 4) << 24);
 }
-__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z) {
+__device__ __forceinline__ void tma_load_4d_pair(void* dst, const CUtensorMap* map, uint32_t cluster_bar, int x, int y, int z, int w) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z)
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(cluster_bar), "r"(x), "r"(y), "r"(z), "r"(w)
       : "memory");
-}
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
-               ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
-               : "memory");
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
@@ -101,7 +112,8 @@ __device__ __forceinline__ float2 f16_pair(uint32_t v) { return __half22float2(*
 template <bool A_MN, bool B_MN, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NS_THREADS, 1)
 newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmM, const NsWork w, const int M,
+                     const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmM,
+                     const __grid_constant__ CUtensorMap tmC2, const __grid_constant__ CUtensorMap tmM2, const NsWork w, const int M,
                      const int N, const int bn, const NsEpilogue ep, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -138,21 +150,25 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   cluster_sync_all();                       // the peer's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    prefetch_tmap(&tmC);
+  }
   pdl_begin();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer (each CTA: its own halves)
     if (elect_one()) {
-      prefetch_tmap(&tmA);
-      prefetch_tmap(&tmB);
       const int b_chunks = (half_n + 63) >> 6;
       const uint32_t full0 = cluster_addr(full, 0);
       int s = 0;
       uint32_t ph = 1;
       bool ok = true;
       for (int u = first; u < units && ok; u += step) {
-        int z, tm, tn;
-        w.decode(u, z, tm, tn);
+        int pair, z, tm, tn;
+        w.decode(u, pair, z, tm, tn);
+        const int pa = MODE == NS_CARRY ? 0 : pair;      // P serves both
         const int m0 = tm * NS_BM + rank * 128, n0 = tn * bn + rank * half_n;
         for (int kb_ = 0; kb_ < w.nk; ++kb_) {
           if (!mbar_wait(&empty[s], ph, abort_flag, status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
@@ -162,16 +178,16 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           if (rank == 0) mbar_expect_tx(&full[s], 2u * stage_bytes);
           const int k0 = kb_ * NS_BK;
           if constexpr (!A_MN) {
-            tma_load_3d_pair(a_dst, &tmA, bar, k0, m0, z);
+            tma_load_4d_pair(a_dst, &tmA, bar, k0, m0, z, pa);
           } else {
-            tma_load_3d_pair(a_dst, &tmA, bar, m0, k0, z);
-            tma_load_3d_pair(a_dst + 8192, &tmA, bar, m0 + 64, k0, z);
+            tma_load_4d_pair(a_dst, &tmA, bar, m0, k0, z, pa);
+            tma_load_4d_pair(a_dst + 8192, &tmA, bar, m0 + 64, k0, z, pa);
           }
           if constexpr (!B_MN) {
-            tma_load_3d_pair(b_dst, &tmB, bar, k0, n0, z);
+            tma_load_4d_pair(b_dst, &tmB, bar, k0, n0, z, pair);
           } else {
-            tma_load_3d_pair(b_dst, &tmB, bar, n0, k0, z);
-            if (b_chunks > 1) tma_load_3d_pair(b_dst + 8192, &tmB, bar, n0 + 64, k0, z);
+            tma_load_4d_pair(b_dst, &tmB, bar, n0, k0, z, pair);
+            if (b_chunks > 1) tma_load_4d_pair(b_dst + 8192, &tmB, bar, n0 + 64, k0, z, pair);
           }
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
@@ -221,13 +237,13 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     const int h = (warp - 2) >> 2;            // this warp takes the 64-column slabs h, h + 2, ...
     uint8_t* const stg0 = smem + NS_RING + (warp - 2) * 8192;
     const int slabs = bn / 64;
-    constexpr bool ADDS = MODE != NS_GRAM, SYMMETRIC = MODE == NS_GRAM || MODE == NS_POLY;
+    constexpr bool ADDS = ns_adds(MODE), SYMMETRIC = ns_symmetric(MODE);
     uint4 v[8];                               // the tile that is added: 32 rows x 64 columns, on its way
     auto fetch = [&](int u, int c) {
-      int z, tm, tn;
-      w.decode(u, z, tm, tn);
+      int pair, z, tm, tn;
+      w.decode(u, pair, z, tm, tn);
       const int row0 = tm * NS_BM + rank * 128 + q * 32, col = tn * bn + c * 64 + (lane & 7) * 8;
-      const __half* src = ep.e + z * ep.e_batch + col;
+      const __half* src = ep.e + pair * ep.e_pair + z * ep.e_batch + col;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int r = row0 + i * 4 + (lane >> 3);
@@ -238,12 +254,12 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     if (ADDS && first < units && h < slabs) fetch(first, h);
     uint32_t tile_i = 0, slab_i = 0;
     for (int u = first; u < units; u += step, ++tile_i) {
-      int z, tm, tn;
-      w.decode(u, z, tm, tn);
+      int pair, z, tm, tn;
+      w.decode(u, pair, z, tm, tn);
       const uint32_t buf = tile_i & 1u;
       const int row0 = tm * NS_BM + rank * 128 + q * 32, row = row0 + lane;
       float coef = ep.coef;
-      if constexpr (MODE == NS_UPDATE) {
+      if constexpr (MODE == NS_UPDATE || MODE == NS_CARRY) {
         if (row < M) coef += ep.diag[static_cast<size_t>(z) * ep.diag_len + row];
       }
       __syncwarp();
@@ -274,6 +290,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
         const int col0 = tn * bn + c * 64;
         uint32_t o[32];
+        uint32_t o2[MODE == NS_POLY ? 32 : 1];           // a I + P
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t a[32];
@@ -303,6 +320,10 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
               }
               if constexpr (MODE == NS_POLY) {
                 const int d = row - (col0 + unit * 8 + 2 * i);      // the diagonal is held apart
+                if (ep.also != 0.f) {
+                  const float full = ep.coef2;
+                  o2[unit * 4 + i] = pack_f16x2((d == 0 ? x + full : x) * ep.also, (d == 1 ? y + full : y) * ep.also);
+                }
                 if (d == 0 || d == 1) {
                   if (row < M) ep.diag[static_cast<size_t>(z) * ep.diag_len + row] = (d ? y : x) * ep.unit;
                   if (d) y = 0.f;
@@ -329,25 +350,36 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           }
           continue;
         }
+        const bool here = row0 < M && col0 < N;      // the tensor maps clip what crosses the edge
+        auto put = [&](const uint32_t* v, const CUtensorMap* direct, const CUtensorMap* transposed) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          st_shared_v4(smem_u32(stg_row) + ((j ^ (lane & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-        if (mirror) {                                // [64 columns][32 rows]
-          uint16_t* t = reinterpret_cast<uint16_t*>(stg0 + 4096) + lane;
+          for (int j = 0; j < 8; ++j)
+            st_shared_v4(smem_u32(stg_row) + ((j ^ (lane & 7)) << 4), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          if (mirror) {                              // [64 columns][32 rows]
+            uint16_t* t = reinterpret_cast<uint16_t*>(stg0 + 4096) + lane;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            t[(2 * j) * 32] = static_cast<uint16_t>(o[j]);
-            t[(2 * j + 1) * 32] = static_cast<uint16_t>(o[j] >> 16);
+            for (int j = 0; j < 32; ++j) {
+              t[(2 * j) * 32] = static_cast<uint16_t>(v[j]);
+              t[(2 * j + 1) * 32] = static_cast<uint16_t>(v[j] >> 16);
+            }
           }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          if (row0 < M && col0 < N) {                // the tensor maps clip what crosses the edge
-            tma_store_3d(&tmC, stg, col0, row0, z);
-            if (mirror) tma_store_3d(&tmM, stg0 + 4096, row0, col0, z);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (here) {
+              tma_store_4d(direct, stg, col0, row0, z, pair);
+              if (mirror) tma_store_4d(transposed, stg0 + 4096, row0, col0, z, pair);
+            }
+            tma_store_commit();
           }
-          tma_store_commit();
+        };
+        put(o, &tmC, &tmM);
+        if constexpr (MODE == NS_POLY) {
+          if (ep.also != 0.f) {
+            if (lane == 0) tma_store_wait_read<0>();
+            __syncwarp();
+            put(o2, &tmC2, &tmM2);
+          }
         }
       }
       if (slabs <= h) {                              // no slab for this warp (narrow tile): release all the same
@@ -531,10 +563,12 @@ muon_apply_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ p, con
 }
 
 // ----------------------------------------------------------------------------- host side
+constexpr int NS_G = 0, NS_T = 1, NS_Q = 2, NS_P = 4, NS_SLOTS = 5;      // square matrices of the workspace: G, T, two Q, P
+
 struct NsLayout {
   int rows, cols, side;      // side: the smaller of the two
   long ldx, ldg;             // row strides in elements (multiples of 8)
-  long x, g, diag, part, total;                // bytes
+  long x, g, diag, part, total;                // bytes; g: one square matrix of every item
   NsLayout(int batch, int m, int n) : rows(m), cols(n), side(m < n ? m : n) {
     const auto up = [](long b) { return (b + 255) / 256 * 256; };
     ldx = (n + 7L) / 8 * 8;
@@ -543,26 +577,35 @@ struct NsLayout {
     g = up(2L * batch * side * ldg);
     diag = up(4L * batch * side);
     part = up(8L * batch * NS_SUM_BLOCKS);
-    total = 2 * x + 2 * g + diag + part;
+    total = 2 * x + NS_SLOTS * g + diag + part;
   }
 };
 
-static int ns_map(CUtensorMap* map, const void* base, long inner, long rows, long batch, long ld, uint32_t box_inner, uint32_t box_rows,
+// Matrices of one product: [pairs][batch][rows][ld]; pair_bytes: from the first of a pair to the second.
+struct NsMatrix {
+  void* p;
+  long ld;
+  long pair_bytes;
+};
+
+static int ns_map(CUtensorMap* map, const NsMatrix& m, long inner, long rows, long batch, int pairs, uint32_t box_inner, uint32_t box_rows,
                   int swizzle) {
-  const uint64_t dims[3] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)batch};
-  const uint64_t str[2] = {(uint64_t)ld * 2, (uint64_t)ld * rows * 2};
-  const uint32_t box[3] = {box_inner, box_rows, 1};
-  return make_tmap(map, base, 2, 3, dims, str, box, swizzle);
+  const uint64_t item = (uint64_t)m.ld * rows * 2;
+  const uint64_t dims[4] = {(uint64_t)inner, (uint64_t)rows, (uint64_t)batch, (uint64_t)pairs};
+  const uint64_t str[3] = {(uint64_t)m.ld * 2, item, pairs > 1 ? (uint64_t)m.pair_bytes : item * batch};
+  const uint32_t box[4] = {box_inner, box_rows, 1, 1};
+  return make_tmap(map, m.p, 2, 4, dims, str, box, swizzle);
 }
 
 // C [M, N] of each matrix of the batch from A and B: [rows][ld] matrices whose rows run along K (K-major) or along M / N.
 template <bool A_MN, bool B_MN, int MODE>
-static int ns_product(const void* A, long lda, const void* B, long ldb, void* C, long ldc, int batch, int M, int N, int K,
+static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, const NsMatrix& C2, int batch, int pairs, int M, int N, int K,
                       const NsEpilogue& ep, int* status, cudaStream_t stream) {
-  constexpr bool SYMMETRIC = MODE == NS_GRAM || MODE == NS_POLY;
-  const int pairs = device_sm_count() / 2;
+  constexpr bool SYMMETRIC = ns_symmetric(MODE);
+  const int sms = device_sm_count() / 2;
   NsWork w;
   w.batch = batch;
+  w.pairs = pairs;
   w.tiles_m = (M + NS_BM - 1) / NS_BM;
   w.nk = (K + NS_BK - 1) / NS_BK;
   // Width of the tiles: as for the other products on pairs of SMs, clocks of a step of 64 are the larger of the tensor cores' (2 a
@@ -575,7 +618,7 @@ static int ns_product(const void* A, long lda, const void* B, long ldb, void* C,
     long tiles = 0;
     if (SYMMETRIC) for (int i = 0; i < w.tiles_m; ++i) tiles += tn - i * (256 / b);
     else tiles = (long)w.tiles_m * tn;
-    const long waves = (tiles * batch + pairs - 1) / pairs;
+    const long waves = (tiles * batch * pairs + sms - 1) / sms;
     const double cost = (double)waves * (w.nk * (double)(2 * b > 256 + b ? 2 * b : 256 + b) + 1500.0);
     if (!bn || cost < best * 0.97) {
       best = cost;
@@ -588,20 +631,26 @@ static int ns_product(const void* A, long lda, const void* B, long ldb, void* C,
   long gm = (24L << 20) / ((long)NS_BM * K * 2);
   gm = gm < 8 ? 8 : gm > 16 ? 16 : gm;
   w.group_m = gm < w.tiles_m ? (int)gm : w.tiles_m;
-  CUtensorMap tmA, tmB, tmC, tmM;
+  CUtensorMap tmA, tmB, tmC, tmM, tmC2, tmM2;
   int rc;
+  const int pairs_a = MODE == NS_CARRY ? 1 : pairs;
   // operands: zeros past the edge of K and of the rows, so that padding never counts
-  if (!A_MN) rc = ns_map(&tmA, A, K, M, batch, lda, NS_BK, 128, 3);
-  else       rc = ns_map(&tmA, A, M, K, batch, lda, 64, NS_BK, 3);
+  if (!A_MN) rc = ns_map(&tmA, A, K, M, batch, pairs_a, NS_BK, 128, 3);
+  else       rc = ns_map(&tmA, A, M, K, batch, pairs_a, 64, NS_BK, 3);
   if (rc) return rc;
-  if (!B_MN) rc = ns_map(&tmB, B, K, N, batch, ldb, NS_BK, bn / 2, 3);
-  else       rc = ns_map(&tmB, B, N, K, batch, ldb, 64, NS_BK, 3);
+  if (!B_MN) rc = ns_map(&tmB, B, K, N, batch, pairs, NS_BK, bn / 2, 3);
+  else       rc = ns_map(&tmB, B, N, K, batch, pairs, 64, NS_BK, 3);
   if (rc) return rc;
   // the output's rows in whole 16-byte units (the padding of the workspace takes zeros); a result with other rows is not stored by TMA
   tmC = tmA;
-  if (ldc % 8 == 0 && (rc = ns_map(&tmC, C, ldc, M, batch, ldc, 64, 32, 3))) return rc;
+  if (C.ld % 8 == 0 && (rc = ns_map(&tmC, C, C.ld, M, batch, pairs, 64, 32, 3))) return rc;
   tmM = tmC;
-  if (SYMMETRIC && (rc = ns_map(&tmM, C, ldc, M, batch, ldc, 32, 64, 0))) return rc;
+  if (SYMMETRIC && (rc = ns_map(&tmM, C, C.ld, M, batch, pairs, 32, 64, 0))) return rc;
+  tmC2 = tmC;
+  tmM2 = tmM;
+  if (MODE == NS_POLY && C2.p && ((rc = ns_map(&tmC2, C2, C2.ld, M, batch, pairs, 64, 32, 3)) ||
+                                  (rc = ns_map(&tmM2, C2, C2.ld, M, batch, pairs, 32, 64, 0))))
+    return rc;
   auto kern = newton_schulz_kernel<A_MN, B_MN, MODE>;
   static bool configured[64] = {};
   int dev = 0;
@@ -612,22 +661,34 @@ static int ns_product(const void* A, long lda, const void* B, long ldb, void* C,
     if (e != cudaSuccess) return 1000 + static_cast<int>(e);
     configured[dev] = true;
   }
-  const long units = (long)batch * w.per_matrix;
+  const long units = (long)pairs * batch * w.per_matrix;
   if (units >= 1L << 30) return 7;
-  const int grid = 2 * (int)(units < pairs ? units : pairs);
-  KB_LAUNCH_PDL(kern, grid, NS_THREADS, NS_SMEM, stream, tmA, tmB, tmC, tmM, w, M, N, bn, ep, status);
+  const int grid = 2 * (int)(units < sms ? units : sms);
+  KB_LAUNCH_PDL(kern, grid, NS_THREADS, NS_SMEM, stream, tmA, tmB, tmC, tmM, tmC2, tmM2, w, M, N, bn, ep, status);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }
 
+// Whether G is carried from step to step (see the head of this file).  One B200, us step by step / carried: 14336 x 4096 3650 / 2560,
+// 6144 x 4096 1842 / 1675.  Below a side of 1024 a product is over before its launch and its epilogue are, and there are no fewer of
+// them: 2048 x 512 139 / 143, three of 333 x 1000 126 / 138.
+static bool ns_carries(int m, int n, int steps) {
+  const long side = m < n ? m : n, other = m < n ? n : m;
+  return steps > 1 && side >= 1024 && 2 * other >= 3 * side;
+}
+// Steps of the segment that begins with `left` steps to go: three and then two, or only two.
+static int ns_segment(int m, int n, int steps, int left) {
+  if (!ns_carries(m, n, steps)) return 1;
+  return left % 2 == 1 && left > 1 ? 3 : left < 2 ? left : 2;
+}
+
 static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
-                         void* out, uint8_t* work, int* status, cudaStream_t stream) {
+                         float scale_q, void* out, uint8_t* work, int* status, cudaStream_t stream) {
   const NsLayout lay(batch, m, n);
-  uint8_t* x[2] = {work, work + lay.x};
-  uint8_t* const g = work + 2 * lay.x;
-  uint8_t* const p = g + lay.g;
-  float* const diag = reinterpret_cast<float*>(p + lay.g);
-  double* const part = reinterpret_cast<double*>(p + lay.g + lay.diag);
+  uint8_t* const x[2] = {work, work + lay.x};
+  uint8_t* const square = work + 2 * lay.x;
+  float* const diag = reinterpret_cast<float*>(square + NS_SLOTS * lay.g);
+  double* const part = reinterpret_cast<double*>(square + NS_SLOTS * lay.g + lay.diag);
   const long count = (long)m * n;
   const auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   const long per_block = 8L * NS_SUM_THREADS;
@@ -647,24 +708,87 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
   }
   const bool tall = m > n;
   const int side = lay.side;
-  const float unit = 1.f / scale;              // a power of two
-  for (int i = 0; i < steps; ++i) {
-    const bool last = i == steps - 1;
-    void* const xi = x[i & 1];
-    void* const xo = last ? out : x[(i + 1) & 1];
-    const long ldo = last ? n : lay.ldx;
-    NsEpilogue eg{nullptr, 0, 0, 0, unit, 0.f, nullptr, 0, unit, nullptr, false};
-    NsEpilogue epo{reinterpret_cast<const __half*>(g), side * lay.ldg, (int)lay.ldg, (int)lay.ldg, c * unit, b, diag, side, unit, nullptr, false};
-    NsEpilogue eu{reinterpret_cast<const __half*>(xi), m * lay.ldx, (int)lay.ldx, (int)lay.ldx, unit, a, diag, side, unit,
-                  static_cast<__nv_bfloat16*>(out), last};
-    int rc = tall ? ns_product<true, true, NS_GRAM>(xi, lay.ldx, xi, lay.ldx, g, lay.ldg, batch, side, side, m, eg, status, stream)
-                  : ns_product<false, false, NS_GRAM>(xi, lay.ldx, xi, lay.ldx, g, lay.ldg, batch, side, side, n, eg, status, stream);
+  const long ldg = lay.ldg;
+  const float unit = 1.f / scale, unit_q = 1.f / scale_q;      // powers of two
+  const auto slot = [&](int i) { return NsMatrix{square + i * lay.g, ldg, 0}; };
+  const NsMatrix none{nullptr, 0, 0};
+  int cur = 0, rc = 0;
+  for (int done = 0; done < steps;) {
+    const int len = ns_segment(m, n, steps, steps - done);
+    const bool last = done + len == steps;
+    const NsMatrix xi{x[cur], lay.ldx, 0}, xo{last ? out : x[cur ^ 1], last ? (long)n : lay.ldx, 0};
+    NsEpilogue eg{};
+    eg.alpha = eg.unit = unit;
+    rc = tall ? ns_product<true, true, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, m, eg, status, stream)
+              : ns_product<false, false, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, n, eg, status, stream);
     if (rc) return rc;
-    rc = ns_product<false, false, NS_POLY>(g, lay.ldg, g, lay.ldg, p, lay.ldg, batch, side, side, side, epo, status, stream);
+    // P of the G at hand; with `q` also a I + P
+    const auto poly = [&](bool q) {
+      NsEpilogue e{};
+      e.e = reinterpret_cast<const __half*>(square + NS_G * lay.g);
+      e.e_batch = side * ldg;
+      e.lde = e.e_cols = (int)ldg;
+      e.alpha = c * unit;
+      e.coef = b;
+      e.diag = diag;
+      e.diag_len = side;
+      e.unit = unit;
+      e.coef2 = a * scale;
+      e.also = q ? scale_q * unit : 0.f;
+      return ns_product<false, false, NS_POLY>(slot(NS_G), slot(NS_G), slot(NS_P), q ? slot(NS_Q) : none, batch, 1, side, side, side, e, status,
+                                               stream);
+    };
+    // slot `to` = (a I + P) slot `from`, with a second pair of slots where `from2` says so
+    const auto carry = [&](int from, int to, int from2, int to2) {
+      NsEpilogue e{};
+      const int pairs = from2 ? 2 : 1;
+      NsMatrix y = slot(from), z = slot(to);
+      y.pair_bytes = (from2 - from) * lay.g;
+      z.pair_bytes = (to2 - to) * lay.g;
+      e.e = static_cast<const __half*>(y.p);
+      e.e_batch = side * ldg;
+      e.e_pair = y.pair_bytes / 2;
+      e.lde = e.e_cols = (int)ldg;
+      e.alpha = unit;
+      e.coef = a;
+      e.diag = diag;
+      e.diag_len = side;
+      e.unit = unit;
+      return ns_product<false, false, NS_CARRY>(slot(NS_P), y, z, none, batch, pairs, side, side, side, e, status, stream);
+    };
+    NsEpilogue eu{};
+    eu.diag = diag;
+    eu.diag_len = side;
+    eu.out = static_cast<__nv_bfloat16*>(out);
+    eu.last = last;
+    if (len == 1) {
+      if ((rc = poly(false))) return rc;
+      eu.e = static_cast<const __half*>(xi.p);
+      eu.e_batch = m * lay.ldx;
+      eu.lde = eu.e_cols = (int)lay.ldx;
+      eu.alpha = eu.unit = unit;
+      eu.coef = a;
+      rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, slot(NS_P), xo, none, batch, 1, m, n, side, eu, status, stream)
+                : ns_product<false, true, NS_UPDATE>(slot(NS_P), xi, xo, none, batch, 1, m, n, side, eu, status, stream);
+    } else {
+      int q = NS_Q, spare = NS_Q + 1;
+      if ((rc = poly(true)) || (rc = carry(NS_G, NS_T, 0, 0)) || (rc = carry(NS_T, NS_G, 0, 0))) return rc;
+      for (int k = 1; k < len; ++k) {
+        if ((rc = poly(false))) return rc;
+        rc = k < len - 1 ? carry(NS_G, NS_T, q, spare) : carry(q, spare, 0, 0);
+        if (rc || (k < len - 1 && (rc = carry(NS_T, NS_G, 0, 0)))) return rc;
+        const int t = q;
+        q = spare;
+        spare = t;
+      }
+      eu.alpha = unit_q;
+      eu.unit = unit;
+      rc = tall ? ns_product<false, false, NS_APPLY>(xi, slot(q), xo, none, batch, 1, m, n, side, eu, status, stream)
+                : ns_product<false, true, NS_APPLY>(slot(q), xi, xo, none, batch, 1, m, n, side, eu, status, stream);
+    }
     if (rc) return rc;
-    rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, lay.ldx, p, lay.ldg, xo, ldo, batch, m, n, side, eu, status, stream)
-              : ns_product<false, true, NS_UPDATE>(p, lay.ldg, xi, lay.ldx, xo, ldo, batch, m, n, side, eu, status, stream);
-    if (rc) return rc;
+    done += len;
+    cur ^= 1;
   }
   return 0;
 }
@@ -679,26 +803,36 @@ static bool ns_sizes_ok(long batch, long m, long n) {
 extern "C" long kb_newton_schulz_bytes(long batch, long m, long n) {
   return kb::ns_sizes_ok(batch, m, n) ? kb::NsLayout((int)batch, (int)m, (int)n).total : -1;
 }
+// Kernels that a call of the functions below launches for a batch (the optimizer step: one more).
+extern "C" int kb_newton_schulz_launches(int m, int n, int steps) {
+  int launches = 2;
+  for (int done = 0; done < steps;) {
+    const int len = kb::ns_segment(m, n, steps, steps - done);
+    launches += len == 1 ? 3 : 1 + 3 + 3 * (len - 1) - 1 + 1;
+    done += len;
+  }
+  return launches;
+}
 // out [batch, m, n] (bf16, 16-byte aligned) = x (fp32 or bf16, contiguous) after `steps` Newton-Schulz steps.  scale: a power of
-// two under which every entry of the iterates, of G and of P fits into fp16.
+// two under which every entry of the iterates, of G and of P fits into fp16; scale_q: one for the products of up to three a I + P.
 extern "C" int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n, float a, float b, float c, int steps, float eps,
-                                float scale, void* out, void* work, int* status, cudaStream_t stream) {
+                                float scale, float scale_q, void* out, void* work, int* status, cudaStream_t stream) {
   if (!kb::ns_sizes_ok(batch, m, n) || steps < 1 || !x || !out || !work || reinterpret_cast<uintptr_t>(out) % 16 ||
       reinterpret_cast<uintptr_t>(work) % 256)
     return 7;
   const kb::NsSource src{x, nullptr, nullptr, 0.f, bf16 != 0, false};
-  return kb::newton_schulz(src, batch, m, n, a, b, c, steps, eps, scale, out, static_cast<uint8_t*>(work), status, stream);
+  return kb::newton_schulz(src, batch, m, n, a, b, c, steps, eps, scale, scale_q, out, static_cast<uint8_t*>(work), status, stream);
 }
 // One optimizer step of a [m, n] matrix: mom <- beta mom + gs g;  o = Newton-Schulz of (nesterov: gs g + beta mom) or mom;
 // master <- keep * master - step * o;  p = bf16(master).  gs: *grad_scale, 1 where that is null.
 extern "C" int kb_muon_step(const float* g, float* mom, float* master, void* p, void* o, int m, int n, float beta, int nesterov,
                             float keep, float step, const float* grad_scale, float a, float b, float c, int steps, float eps, float scale,
-                            void* work, int* status, cudaStream_t stream) {
+                            float scale_q, void* work, int* status, cudaStream_t stream) {
   if (!kb::ns_sizes_ok(1, m, n) || steps < 1 || !g || !mom || !master || !p || !o || !work || reinterpret_cast<uintptr_t>(o) % 16 ||
       reinterpret_cast<uintptr_t>(work) % 256)
     return 7;
   const kb::NsSource src{g, mom, grad_scale, beta, false, nesterov != 0};
-  const int rc = kb::newton_schulz(src, 1, m, n, a, b, c, steps, eps, scale, o, static_cast<uint8_t*>(work), status, stream);
+  const int rc = kb::newton_schulz(src, 1, m, n, a, b, c, steps, eps, scale, scale_q, o, static_cast<uint8_t*>(work), status, stream);
   if (rc) return rc;
   const long count = (long)m * n;
   const auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };

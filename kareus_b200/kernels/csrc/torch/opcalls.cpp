@@ -129,7 +129,7 @@ PyObject* fp8_gemm(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// orthogonalize(x, a, b, c, steps, eps, scale, launches): contiguous fp32 or bf16 matrices, checked parameters
+// orthogonalize(x, a, b, c, steps, eps, scale, scale_q): contiguous fp32 or bf16 matrices, checked parameters
 PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   if (nargs != 8) Py_RETURN_NONE;
@@ -139,8 +139,7 @@ PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!x || x->dim() < 2 || !x->is_contiguous() || !x->numel() || !current(*x)) Py_RETURN_NONE;
   const double a = PyFloat_AsDouble(args[1]), b = PyFloat_AsDouble(args[2]), c = PyFloat_AsDouble(args[3]);
   const long steps = PyLong_AsLong(args[4]);
-  const double eps = PyFloat_AsDouble(args[5]), scale = PyFloat_AsDouble(args[6]);
-  const long launches = PyLong_AsLong(args[7]);
+  const double eps = PyFloat_AsDouble(args[5]), scale = PyFloat_AsDouble(args[6]), scale_q = PyFloat_AsDouble(args[7]);
   if (PyErr_Occurred()) return nullptr;
   const int64_t m = x->size(-2), n = x->size(-1), batch = x->numel() / (m * n);
   const long bytes = kb_newton_schulz_bytes(batch, m, n);
@@ -152,9 +151,9 @@ PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   int* status = g_status[x->device().index()];
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
   const int rc = without_gil([&] {
-    return kb_newton_schulz(px, bf16, batch, m, n, a, b, c, steps, eps, scale, po, pw, status, stream);
+    return kb_newton_schulz(px, bf16, batch, m, n, a, b, c, steps, eps, scale, scale_q, po, pw, status, stream);
   });
-  if (!finish(rc, "orthogonalize", launches)) return nullptr;
+  if (!finish(rc, "orthogonalize", kb_newton_schulz_launches(m, n, steps))) return nullptr;
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }

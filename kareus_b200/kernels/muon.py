@@ -17,21 +17,27 @@ COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
 
 @functools.lru_cache(maxsize=64)
-def fp16_scale(steps: int, coefficients: tuple) -> float:
-    """The power of two (at most 2^14) under which the entries of X, of G = X Xt and of P = b G + c G G fit into fp16 in every step.
-    Entries are at most the largest singular value, which starts at 1 or below; the range that a step can reach is sampled."""
+def fp16_scales(steps: int, coefficients: tuple) -> tuple:
+    """Powers of two under which what the steps hold in fp16 fits: one (at most 2^14) for X, G = X Xt and P = b G + c G G, one for
+    products of up to three consecutive a I + P.  Entries are at most the largest singular value; those of X start at 1 or below, and
+    the range that a step can reach is sampled."""
     a, b, c = coefficients
-    bound, worst = 1.0, 1.0
-    for _ in range(steps):
+    bound, worst, worst_q = 1.0, 1.0, 1.0
+    for k in range(steps):
         s = torch.linspace(0.0, bound * 1.01, 8193, dtype=torch.float64)       # 1 %: what rounding adds
-        t = s * s
-        poly = b * t + c * t * t
-        worst = max(worst, t.max().item(), poly.abs().max().item())
-        bound = (s * (a + poly)).abs().max().item()
-        worst = max(worst, bound)
-        if not worst < 1e3:
+        t, prod = s * s, 1.0
+        for j in range(min(3, steps - k)):
+            q = a + b * t + c * t * t
+            if j == 0:
+                worst = max(worst, t.max().item(), (q - a).abs().max().item())
+                bound = (s * q).abs().max().item()
+                worst = max(worst, bound)
+            prod = prod * q
+            t = t * q * q
+            worst_q = max(worst_q, prod.abs().max().item())
+        if not worst < 1e3 or not worst_q < 3e4:
             raise KernelError(f"Newton-Schulz coefficients {coefficients} let the iterates grow without bound")
-    return 2.0 ** min(14, math.floor(math.log2(65000.0 / worst)))
+    return tuple(2.0 ** min(14, math.floor(math.log2(65000.0 / w))) for w in (worst, worst_q))
 
 
 def _parameters(steps, coefficients, eps):
@@ -48,14 +54,10 @@ def _workspace(batch, m, n, device):
     return torch.empty(size, dtype=torch.uint8, device=device)
 
 
-def _launches(steps: int) -> int:
-    return 2 + 3 * steps
-
-
 def orthogonalize(x, steps, coefficients, eps):
     steps, coefficients, eps = _parameters(steps, coefficients, eps)
     if _entry._OPS is not None and x.is_cuda:
-        r = _entry._OPS.orthogonalize(x, *coefficients, steps, eps, fp16_scale(steps, coefficients), _launches(steps))
+        r = _entry._OPS.orthogonalize(x, *coefficients, steps, eps, *fp16_scales(steps, coefficients))
         if r is not None:
             return r
     if x.dim() < 2 or not x.is_floating_point():
@@ -63,7 +65,8 @@ def orthogonalize(x, steps, coefficients, eps):
     if not (x.is_cuda and x.dtype in (torch.bfloat16, torch.float32)):
         return ref.orthogonalize(x, steps, coefficients, eps)
     require_current_device("orthogonalize", x)
-    scale = fp16_scale(steps, coefficients)
+    scales = fp16_scales(steps, coefficients)
+    status_word(x.device)                     # the native call takes over from the next one on
     out = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
     if not x.numel():
         return out
@@ -73,10 +76,10 @@ def orthogonalize(x, steps, coefficients, eps):
     m, n = x.shape[-2:]
     batch = x.numel() // (m * n)
     work = _workspace(batch, m, n, x.device)
-    _check(lib().kb_newton_schulz(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, batch, m, n, *coefficients, steps, eps, scale,
+    _check(lib().kb_newton_schulz(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, batch, m, n, *coefficients, steps, eps, *scales,
                                   out.data_ptr(), work.data_ptr(), status_word(x.device).data_ptr(), _stream()),
            f"orthogonalize {batch} x {m} x {n}")
-    _count(_launches(steps))
+    _count(lib().kb_newton_schulz_launches(m, n, steps))
     return out
 
 
@@ -106,7 +109,7 @@ def muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, step
     _check(lib().kb_muon_step(g.data_ptr(), m.data_ptr(), master.data_ptr(), p.data_ptr(), o.data_ptr(), rows, cols, float(momentum),
                               1 if nesterov else 0, 1.0 - lr * weight_decay, lr * scale,
                               0 if grad_scale_tensor is None else grad_scale_tensor.data_ptr(), *coefficients, steps, eps,
-                              fp16_scale(steps, coefficients), work.data_ptr(), status_word(g.device).data_ptr(), _stream()),
+                              *fp16_scales(steps, coefficients), work.data_ptr(), status_word(g.device).data_ptr(), _stream()),
            f"muon_step {rows} x {cols}")
-    _count(_launches(steps) + 1)
+    _count(lib().kb_newton_schulz_launches(rows, cols, steps) + 1)
     return o

@@ -8,7 +8,7 @@ import torch
 
 from kareus_b200 import kernels as K
 from kareus_b200.kernels.cuda import KernelError
-from kareus_b200.kernels.muon import COEFFICIENTS, fp16_scale
+from kareus_b200.kernels.muon import COEFFICIENTS, fp16_scales
 
 gpu = pytest.mark.gpu
 
@@ -28,7 +28,7 @@ def iterate(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, rnd=lambda t: t):
 
 
 def check(o, x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
-    scale = fp16_scale(steps, coefficients)
+    scale, _ = fp16_scales(steps, coefficients)
     exact = iterate(x, steps, coefficients, eps)
     rounded = iterate(x, steps, coefficients, eps, lambda t: (t * scale).half().double() / scale)
     assert o.shape == x.shape and o.dtype == torch.bfloat16
@@ -48,7 +48,7 @@ def matrices(batch, m, n, device="cuda", seed=0, std=1e-3):
 
 
 SIZES = [(1, 1, 1), (1, 1, 7), (1, 9, 1), (1, 5, 3), (2, 16, 16), (1, 64, 200), (3, 130, 70), (3, 333, 1000), (1, 1000, 333), (2, 512, 512),
-         (1, 2048, 512), (40, 24, 40), (1, 300, 1504), (1, 1100, 2600), (1, 1500, 900), (1, 257, 256), (1, 256, 321)]
+         (1, 2048, 512), (40, 24, 40), (1, 300, 1504), (1, 1100, 2600), (1, 1500, 900), (1, 257, 256), (1, 256, 321), (2, 1030, 1800), (1, 1700, 1024)]
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
@@ -71,9 +71,10 @@ def test_orthogonalize(size, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("steps, coefficients", [(1, COEFFICIENTS), (2, COEFFICIENTS), (8, (1.5, -0.5, 0.0)), (6, (1.875, -1.25, 0.375))])
+@pytest.mark.parametrize("steps, coefficients", [(1, COEFFICIENTS), (2, COEFFICIENTS), (3, COEFFICIENTS), (4, COEFFICIENTS),
+                                                 (8, (1.5, -0.5, 0.0)), (6, (1.875, -1.25, 0.375))])
 def test_other_coefficients(steps, coefficients):
-    for size in ((1, 200, 456), (2, 321, 130)):
+    for size in ((1, 200, 456), (2, 321, 130), (1, 1600, 1040)):
         x = matrices(*size, seed=3)
         check(K.orthogonalize(x, steps, coefficients), x, steps, coefficients)
 
@@ -219,10 +220,10 @@ def test_refusals(device):
 
 
 def test_scale_of_the_iterates():
-    assert fp16_scale(5, COEFFICIENTS) == 2.0 ** 14
-    assert fp16_scale(1, (6.0, -4.0, 2.0)) == 2.0 ** 13
+    assert fp16_scales(5, COEFFICIENTS) == (2.0 ** 14, 2.0 ** 10)          # three first steps: up to 3.4445^3 = 41
+    assert fp16_scales(1, (6.0, -4.0, 2.0))[0] == 2.0 ** 13
     with pytest.raises(KernelError, match="without bound"):
-        fp16_scale(5, (5.0, 4.0, 3.0))
+        fp16_scales(5, (5.0, 4.0, 3.0))
 
 
 @gpu
