@@ -65,6 +65,20 @@ class ModelConfig:
     max_seq_len: int = 4096
     init_std: float = 0.02
     num_layers_in_first_pipeline_stage: Optional[int] = None
+    # "fp8": the layers' matrix products run on 8-bit operands with block scales (forward, input and weight gradients), the rest
+    # of the model and the weights stay as they are; fp8_grad: format of the gradients, "e4m3" or "e5m2"
+    linear_precision: str = "bf16"
+    fp8_grad: str = "e4m3"
+    embedding_scale: float = 1.0      # factor of the looked-up embeddings (some models: the square root of the hidden size)
+    embedding_grad: str = "any"       # order in which the table's gradient is summed: "any", or "sorted" (the same bits every run)
+
+    def __post_init__(self):
+        if self.linear_precision not in ("bf16", "fp8"):
+            raise ValueError(f"bad linear_precision {self.linear_precision!r}: bf16 (the model's own type) or fp8")
+        if self.fp8_grad not in ("e4m3", "e5m2"):
+            raise ValueError(f"bad fp8_grad {self.fp8_grad!r}: e4m3 or e5m2")
+        if self.embedding_grad not in ("any", "sorted"):
+            raise ValueError(f"bad embedding_grad {self.embedding_grad!r}: any or sorted")
 
     @property
     def hd(self) -> int:
@@ -202,6 +216,15 @@ class TrainConfig:
     max_steps: int = 100000
     seed: int = 42
     dtype: str = "bf16"
+    # "muon": the layers' weight matrices take orthogonalised momentum (train/muon.py), everything else AdamW with the same
+    # learning rate and weight decay
+    optimizer: str = "adamw"
+    muon_momentum: float = 0.95
+    muon_steps: int = 5
+
+    def __post_init__(self):
+        if self.optimizer not in ("adamw", "muon"):
+            raise ValueError(f"bad optimizer {self.optimizer!r}: adamw or muon")
 
     def num_microbatches(self, dp: int) -> int:
         per = self.micro_batch_size * dp

@@ -86,7 +86,10 @@ def load_run_config(path, overrides: Iterable[str] = (), world_size: Optional[in
         hidden_dropout=float(m.get("hidden_dropout", 0.0)), qk_layernorm=bool(m.get("qk_layernorm", False)),
         tie_embeddings=bool(m.get("share_embeddings_and_output_weights", False)),
         max_seq_len=int(m.get("encoder_seq_length", 4096)), init_std=float(m.get("init_method_std", 0.02)),
-        num_layers_in_first_pipeline_stage=m.get("num_layers_in_first_pipeline_stage"))
+        num_layers_in_first_pipeline_stage=m.get("num_layers_in_first_pipeline_stage"),
+        linear_precision="fp8" if m.get("fp8") else "bf16",                     # Megatron's `fp8: e4m3` or `fp8: hybrid`
+        fp8_grad="e5m2" if str(m.get("fp8")).lower() == "hybrid" else "e4m3",
+        embedding_scale=float(m.get("embedding_scale", 1.0)), embedding_grad=str(m.get("embedding_grad", "any")))
     tp = int(m.get("tensor_model_parallel_size", 1))
     pp = int(m.get("pipeline_model_parallel_size", 1))
     cp = int(m.get("context_parallel_size", 1))
@@ -103,7 +106,8 @@ def load_run_config(path, overrides: Iterable[str] = (), world_size: Optional[in
                         min_lr=float(sched.get("min_lr", 2e-5)), weight_decay=float(opt.get("weight_decay", 0.01)),
                         betas=(float(betas[0]), float(betas[1])), grad_clip=float(tr.get("gradient_clip_val", 1.0)),
                         warmup_steps=int(sched.get("warmup_steps", 500)), max_steps=int(tr.get("max_steps", 30)),
-                        seed=int(m.get("seed", 1234)),
+                        seed=int(m.get("seed", 1234)), optimizer="muon" if "muon" in str(opt.get("name", "")).lower() else "adamw",
+                        muon_momentum=float(opt.get("momentum", 0.95)),
                         dtype={"bf16": "bf16", "bf16-mixed": "bf16", 16: "fp16", 32: "fp32"}.get(tr.get("precision", "bf16"), "bf16"))
     sw = RunSwitches(enable_zeus_monitor=bool(m.get("enable_zeus_monitor", False)),
                      enable_power_monitor=bool(m.get("enable_power_monitor", False)),

@@ -55,6 +55,14 @@ def _empty(rows: int, cols: int, fmt: str, device) -> Fp8Matrix:
     return Fp8Matrix(data, torch.empty(-(-rows // 128), -(-(-(-cols // 128)) // 4), 32, 4, 4, dtype=torch.uint8, device=device), fmt)
 
 
+def _statement(x, fmt: str, square: bool) -> Fp8Matrix:
+    data, scales = ref.fp8_quantize(x, fmt, square)
+    m = _empty(*x.shape, fmt, x.device)
+    m.data.copy_(data)
+    m.scales = scales
+    return m
+
+
 def quantize(x, rows: bool = True, cols: bool = False, square: bool = False, fmt: str = "e4m3"):
     if _entry._OPS is not None and fmt in _FORMAT_CODE:
         r = _entry._OPS.fp8_quantize(x, rows, cols, square, _FORMAT_CODE[fmt])
@@ -69,8 +77,7 @@ def quantize(x, rows: bool = True, cols: bool = False, square: bool = False, fmt
     if x.shape[0] >= 1 << 31 or x.shape[1] >= 1 << 31:
         raise KernelError(f"fp8_quantize: {tuple(x.shape)} is too large")
     if not (x.is_cuda and x.dtype == torch.bfloat16):
-        return (Fp8Matrix(*ref.fp8_quantize(x, fmt, square), fmt) if rows else None,
-                Fp8Matrix(*ref.fp8_quantize(x.t(), fmt, square), fmt) if cols else None)
+        return _statement(x, fmt, square) if rows else None, _statement(x.t(), fmt, square) if cols else None
     require_current_device("fp8_quantize", x)
     status_word(x.device)                     # the native call takes over from the next one on
     M, N = x.shape

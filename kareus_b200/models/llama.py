@@ -27,7 +27,7 @@ from ..engine.block import BlockEngine
 from ..kernels import ref
 from ..ops.attention import AttentionOp, QKVPostOp, RotaryOp
 from ..ops.basic import DropoutAddOp, RMSNormOp, ResidualFork, SwiGLUOp, accumulate_grad, ensure_main_grad
-from ..ops.linear import ColumnParallelLinear, RowParallelLinear
+from ..ops.linear import ColumnParallelLinear, Fp8ColumnParallelLinear, Fp8RowParallelLinear, RowParallelLinear
 from ..parallel.collectives import CommFactory, dual_chunk_ids
 
 
@@ -52,25 +52,34 @@ class TransformerLayer(nn.Module):
         n = f"layers.{layer_number}"
         out_std = cfg.init_std / math.sqrt(2.0 * cfg.num_layers)
         kw = dict(dtype=dtype, device=device)
+        column, row = ColumnParallelLinear, RowParallelLinear
+        if cfg.linear_precision == "fp8":
+            if par.tp_comm == "sp_fused" and tp > 1:
+                raise ValueError("8-bit linear layers have no kernels with fused collectives: use tp_comm 'sp' or 'allreduce'")
+            column, row = Fp8ColumnParallelLinear, Fp8RowParallelLinear
         self.layer_number = layer_number
         self.attn_fork = ResidualFork(f"{n}.attn_fork")
         self.input_norm = RMSNormOp(h, cfg.norm_eps, f"{n}.input_layernorm", sequence_parallel=sp, **kw)
-        self.qkv = ColumnParallelLinear(h, (hq + 2 * g) * d, f"{n}.self_attention.linear_qkv", "attn",
-                                        par.tp_comm, comm, init_std=cfg.init_std, seed=seed * 16 + 1, **kw)
+        self.qkv = column(h, (hq + 2 * g) * d, f"{n}.self_attention.linear_qkv", "attn",
+                          par.tp_comm, comm, init_std=cfg.init_std, seed=seed * 16 + 1, **kw)
         self.qkv_post = QKVPostOp(hq, g, d, cfg.qk_layernorm, cfg.norm_eps, f"{n}.qkv_post", **kw)
         self.rope = RotaryOp(f"{n}.rope")
         self.core_attn = AttentionOp(d, f"{n}.core_attention", comm, cp_comm=par.cp_comm)
-        self.proj = RowParallelLinear(hq * d, h, f"{n}.self_attention.linear_proj", "attn",
-                                      par.tp_comm, comm, init_std=out_std, seed=seed * 16 + 2, **kw)
+        self.proj = row(hq * d, h, f"{n}.self_attention.linear_proj", "attn",
+                        par.tp_comm, comm, init_std=out_std, seed=seed * 16 + 2, **kw)
         self.attn_bda = DropoutAddOp(cfg.hidden_dropout, f"{n}.attn_bda", base_seed=seed * 16 + 3)
         self.mlp_fork = ResidualFork(f"{n}.mlp_fork")
         self.pre_mlp_norm = RMSNormOp(h, cfg.norm_eps, f"{n}.pre_mlp_layernorm", sequence_parallel=sp, **kw)
-        self.fc1 = ColumnParallelLinear(h, 2 * f, f"{n}.mlp.linear_fc1", "mlp", par.tp_comm, comm,
-                                        init_std=cfg.init_std, seed=seed * 16 + 4, **kw)
+        self.fc1 = column(h, 2 * f, f"{n}.mlp.linear_fc1", "mlp", par.tp_comm, comm,
+                          init_std=cfg.init_std, seed=seed * 16 + 4, **kw)
         self.act = SwiGLUOp(f"{n}.mlp.swiglu")
-        self.fc2 = RowParallelLinear(f, h, f"{n}.mlp.linear_fc2", "mlp", par.tp_comm, comm,
-                                     init_std=out_std, seed=seed * 16 + 5, **kw)
+        self.fc2 = row(f, h, f"{n}.mlp.linear_fc2", "mlp", par.tp_comm, comm,
+                       init_std=out_std, seed=seed * 16 + 5, **kw)
         self.mlp_bda = DropoutAddOp(cfg.hidden_dropout, f"{n}.mlp_bda", base_seed=seed * 16 + 6)
+        if cfg.linear_precision == "fp8":
+            for lin in (self.qkv, self.proj, self.fc1, self.fc2):
+                lin.fp8_grad = cfg.fp8_grad
+        self.fc1.weight.matrices = 2          # gate and up lie one behind the other; an optimizer of matrices takes them apart
         if par.tp_comm == "sp_fused" and tp > 1 and getattr(comm, "heap", None) is not None \
                 and dtype == torch.bfloat16 and torch.device(device or "cpu").type == "cuda":
             from ..ops.fused import attach_fused
@@ -121,7 +130,7 @@ class TransformerBlock(nn.Module):
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, tokens, weight, vocab_start, tp_op, sp_op, module):
-        out = K.embedding_fwd(tokens, weight, vocab_start)          # [s, b, h]
+        out = K.embedding_fwd(tokens, weight, vocab_start, module.scale)          # [s, b, h]
         ctx.save_for_backward(tokens)
         ctx.module, ctx.vocab_start, ctx.tp_op, ctx.sp_op = module, vocab_start, tp_op, sp_op
         if sp_op is not None:
@@ -136,7 +145,7 @@ class _EmbeddingFn(torch.autograd.Function):
         w = ctx.module.weight
         if ctx.sp_op is not None:
             (dout,) = ctx.module.bwd_gather.run((dout.contiguous(),))
-        K.embedding_bwd(dout, tokens, ensure_main_grad(w), ctx.vocab_start)
+        K.embedding_bwd(dout, tokens, ensure_main_grad(w), ctx.vocab_start, ctx.module.scale, ctx.module.grad_order)
         return None, None, None, None, None, None
 
 
@@ -153,6 +162,7 @@ class VocabParallelEmbedding(nn.Module):
             raise ValueError("vocab size must be divisible by tp")
         self.v_local = cfg.vocab_size // tp
         self.vocab_start = rank * self.v_local
+        self.scale, self.grad_order = float(cfg.embedding_scale), cfg.embedding_grad
         w = torch.empty(cfg.vocab_size, cfg.hidden_size, dtype=torch.float32)
         w.normal_(0.0, cfg.init_std, generator=torch.Generator().manual_seed(seed))
         self.weight = nn.Parameter(w[self.vocab_start:self.vocab_start + self.v_local].to(dtype=dtype, device=device))

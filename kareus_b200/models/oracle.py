@@ -50,7 +50,7 @@ class OracleLlama(nn.Module):
         b, s = tokens.shape
         hq, g, d = cfg.num_attention_heads, cfg.num_query_groups, cfg.hd
         rep = hq // g
-        x = self.emb[tokens]                                   # b s h
+        x = self.emb[tokens] * cfg.embedding_scale             # b s h
         fr = ref.rope_table(s, d, cfg.rope_theta).to(x.dtype)
         cos, sin = fr.cos()[None, :, None, :], fr.sin()[None, :, None, :]
 

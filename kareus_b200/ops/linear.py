@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from .. import kernels as K
+from ..kernels.fp8 import Fp8Matrix
 from ..engine.graph import CommKind, CommSpec, ComputeSpec, GraphOperator, grad_channel
 from ..parallel.collectives import AllGather, AllReduce, CommFactory, ReduceScatter
 from .basic import ensure_main_grad
@@ -197,3 +198,46 @@ class RowParallelLinear(_LinearBase):
                              f"bwd_{self.key}_ag", backward=True)]
         return [CommSpec(self.bwd_allgather, CommKind.ALL_GATHER, ("grad_main",), ("grad_main",),
                          f"bwd_{self.key}_ag", backward=True), compute]
+
+
+class _Fp8Linear:
+    """The products of a linear layer on 8-bit operands (``kernels.fp8_quantize``, ``kernels.fp8_gemm``).
+
+    Activations and gradients have a scale for each 1 x 128 piece along the contraction, so the forward pass leaves two copies of
+    its input: along the features for its own product, along the tokens for the weight gradient, which is what it keeps (half the
+    bytes of a bf16 input).  Weights have a scale for each 128 x 128 block and are quantised in every pass: they change between
+    steps, and that is a few percent of a product over many tokens.  The weight gradient is summed in fp32 into ``main_grad``.
+
+    These layers are in no fusion chain (the activation is quantised as it is) and have no fused collectives."""
+
+    fp8_grad = "e4m3"
+
+    def forward(self, ctx, x):
+        shp = x.shape
+        x2 = x.reshape(-1, shp[-1])
+        out = self._fwd_staging((x2.shape[0], self.out_features), x2.dtype, ctx.nb_index, x2.device)
+        xr, xc = K.fp8_quantize(x2, cols=ctx.requires_grad)
+        wr, _ = K.fp8_quantize(self.weight.detach(), square=True)
+        y = K.fp8_gemm(xr, wr, out_dtype=None if x2.dtype == torch.bfloat16 else x2.dtype, out=out)
+        if ctx.requires_grad:
+            ctx.save_for_backward(xc.data, xc.scales)
+        return (y.reshape(shp[:-1] + (self.out_features,)),)
+
+    def backward(self, ctx, dy):
+        xc = Fp8Matrix(*ctx.saved_tensors)
+        shp = dy.shape
+        dy2 = dy.reshape(-1, shp[-1])
+        out = self._bwd_staging((dy2.shape[0], self.in_features), dy2.dtype, ctx.nb_index, dy2.device)
+        dr, dc = K.fp8_quantize(dy2, cols=True, fmt=self.fp8_grad)
+        _, wc = K.fp8_quantize(self.weight.detach(), rows=False, cols=True, square=True)
+        dx = K.fp8_gemm(dr, wc, out_dtype=None if dy2.dtype == torch.bfloat16 else dy2.dtype, out=out)
+        K.fp8_gemm(dc, xc, accumulate=ensure_main_grad(self.weight))
+        return (dx.reshape(shp[:-1] + (self.in_features,)),)
+
+
+class Fp8ColumnParallelLinear(_Fp8Linear, ColumnParallelLinear):
+    """:class:`ColumnParallelLinear` on 8-bit operands."""
+
+
+class Fp8RowParallelLinear(_Fp8Linear, RowParallelLinear):
+    """:class:`RowParallelLinear` on 8-bit operands."""

@@ -23,6 +23,7 @@ from ..models.llama import GPTModel
 from ..parallel.collectives import CommFactory
 from ..parallel.mesh import Mesh
 from ..parallel.pipeline import P2P, PipelineSchedule, one_f_one_b_order
+from .muon import DistributedMuon
 from .optimizer import DistributedAdamW
 
 FWD_BWD_WINDOW = "training_step_fwd_bwd_step_call"
@@ -63,9 +64,12 @@ class Trainer:
         if comm_scheduler is not None:
             self.model.decoder.set_scheduler(comm_scheduler)
         mp_group = mesh.group("tp_pp") if mesh.size("tp_pp") > 1 else None
-        self.optimizer = DistributedAdamW(self.model.parameters(), train_cfg, dp_group=mesh.group("dp_cp"),
-                                          dp_size=mesh.size("dp_cp"), dp_rank=mesh.axis_rank("dp_cp"),
-                                          mp_group=mp_group, tp_rank=mesh.tp_rank)
+        dp = dict(dp_group=mesh.group("dp_cp"), dp_size=mesh.size("dp_cp"), dp_rank=mesh.axis_rank("dp_cp"))
+        if train_cfg.optimizer == "muon":
+            self.optimizer = DistributedMuon(self.model.parameters(), train_cfg, mp_group=mp_group, tp_size=mesh.tp, **dp,
+                                             matrices=[p for p in self.model.decoder.parameters() if p.dim() == 2])
+        else:
+            self.optimizer = DistributedAdamW(self.model.parameters(), train_cfg, mp_group=mp_group, tp_rank=mesh.tp_rank, **dp)
         self.num_microbatches = train_cfg.num_microbatches(par.dp)
         self.p2p: Optional[P2P] = None
         self.step_index = 0
