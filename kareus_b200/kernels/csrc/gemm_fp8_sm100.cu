@@ -116,13 +116,17 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   cluster_sync_all();                       // the peer's barriers exist before anything arrives on them
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+    prefetch_tmap(&tmSA);
+    prefetch_tmap(&tmSB);
+  }
   pdl_begin();
 
   if (warp == 0) {
     // ------------------------------------------------------------------ producer (each CTA: its own halves)
     if (elect_one()) {
-      prefetch_tmap(&tmA);
-      prefetch_tmap(&tmB);
       const uint32_t full0 = cluster_addr(full, 0);
       int s = 0;
       uint32_t ph = 1;
@@ -242,11 +246,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           }
         }
         const bool shared = shared_cols && c == (buf == 0 ? slabs - 1 : 0), last = j == mine - 1;
-        if (shared || last) {
+        if (shared || last) {                         // hand over what the next tiles wait for (half a microsecond each)
           tc_fence_before();
           __syncwarp();
-          if (lane == 0 && shared) mbar_arrive_cluster(cluster_addr(tshare, 0));
-          if (lane == 0 && last) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+          if (lane == 0 && shared && t + step < tiles) mbar_arrive_cluster(cluster_addr(tshare, 0));
+          if (lane == 0 && last && t + 2 * step < tiles) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
         }
         if (lane == 0) tma_store_wait_read<0>();      // the previous slab has left the staging buffer
         __syncwarp();
@@ -278,10 +282,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       if (mine == 0) {                                // no slab for this warp (narrow tile): release all the same
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+        if (lane == 0 && t + 2 * step < tiles) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
       }
     }
-    if (lane == 0) tma_store_wait<0>();               // nothing in flight out of shared memory at exit
+    if (lane == 0) tma_store_wait_read<0>();          // nothing in flight out of shared memory at exit
   }
 
   tc_fence_before();

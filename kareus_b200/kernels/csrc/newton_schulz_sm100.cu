@@ -239,6 +239,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     const int slabs = bn / 64;
     constexpr bool ADDS = ns_adds(MODE), SYMMETRIC = ns_symmetric(MODE);
     uint4 v[8];                               // the tile that is added: 32 rows x 64 columns, on its way
+    float2 d_next = make_float2(0.f, 0.f);    // NS_UPDATE_T: P's diagonal for two of these columns, lane by lane
     auto fetch = [&](int u, int c) {
       int pair, z, tm, tn;
       w.decode(u, pair, z, tm, tn);
@@ -249,6 +250,11 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const int r = row0 + i * 4 + (lane >> 3);
         v[i] = make_uint4(0u, 0u, 0u, 0u);
         if (r < M && col < ep.e_cols) v[i] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(r) * ep.lde);
+      }
+      if constexpr (MODE == NS_UPDATE_T) {
+        const int dc = tn * bn + c * 64 + 2 * lane;
+        const float* d = ep.diag + static_cast<size_t>(z) * ep.diag_len;
+        d_next = make_float2(dc < N ? d[dc] : 0.f, dc + 1 < N ? d[dc + 1] : 0.f);
       }
     };
     if (ADDS && first < units && h < slabs) fetch(first, h);
@@ -266,12 +272,14 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       if (!mbar_wait_warp(&tfull[buf], (tile_i >> 1) & 1u, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + buf * 256 + (static_cast<uint32_t>(q * 32) << 16);
+      const bool reused = u + 2 * step < units;      // a later tile takes this accumulator; handing it back costs half a microsecond
       const bool mirror = SYMMETRIC && tn * bn / NS_BM > tm;
 #pragma unroll 1
       for (int c = h; c < slabs; c += 2, ++slab_i) {
         // Symmetric outputs use one buffer for the tile and one for its transpose, the others two in turn.
         uint8_t* const stg = SYMMETRIC ? stg0 : stg0 + (slab_i & 1u) * 4096;
         uint8_t* const stg_row = stg + lane * 128;
+        const float2 d_now = d_next;
         if (lane == 0) {
           if constexpr (SYMMETRIC) tma_store_wait_read<0>();
           else tma_store_wait_read<1>();
@@ -291,9 +299,13 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const int col0 = tn * bn + c * 64;
         uint32_t o[32];
         uint32_t o2[MODE == NS_POLY ? 32 : 1];           // a I + P
+        // the diagonal crosses few slabs: the others are spared the search for it
+        const bool on_diagonal = MODE == NS_POLY && col0 < row0 + 32 && row0 < col0 + 64;
+        float diagonal = 0.f;
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           uint32_t a[32];
+          float f[32];
           __syncwarp();                               // TMEM is read by whole warps: what lanes did on their own before ends here
           tmem_ld_32x32(taddr + c * 64 + half * 32, a);
           tmem_ld_wait();
@@ -305,40 +317,51 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             const uint32_t e[4] = {e4.x, e4.y, e4.z, e4.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              float x = __uint_as_float(a[8 * j + 2 * i]) * ep.alpha, y = __uint_as_float(a[8 * j + 2 * i + 1]) * ep.alpha;
+              const int k = 8 * j + 2 * i;
+              float x = __uint_as_float(a[k]) * ep.alpha, y = __uint_as_float(a[k + 1]) * ep.alpha;
               if constexpr (ADDS) {
                 const float2 p = f16_pair(e[i]);
                 float c0 = coef, c1 = coef;
                 if constexpr (MODE == NS_UPDATE_T) {
-                  const int col = col0 + unit * 8 + 2 * i;
-                  const float* d = ep.diag + static_cast<size_t>(z) * ep.diag_len;
-                  if (col < N) c0 += d[col];
-                  if (col + 1 < N) c1 += d[col + 1];
+                  c0 += __shfl_sync(0xffffffffu, d_now.x, half * 16 + k / 2);
+                  c1 += __shfl_sync(0xffffffffu, d_now.y, half * 16 + k / 2);
                 }
                 x = fmaf(c0, p.x, x);
                 y = fmaf(c1, p.y, y);
               }
-              if constexpr (MODE == NS_POLY) {
-                const int d = row - (col0 + unit * 8 + 2 * i);      // the diagonal is held apart
-                if (ep.also != 0.f) {
-                  const float full = ep.coef2;
-                  o2[unit * 4 + i] = pack_f16x2((d == 0 ? x + full : x) * ep.also, (d == 1 ? y + full : y) * ep.also);
-                }
-                if (d == 0 || d == 1) {
-                  if (row < M) ep.diag[static_cast<size_t>(z) * ep.diag_len + row] = (d ? y : x) * ep.unit;
-                  if (d) y = 0.f;
-                  else x = 0.f;
-                }
-              }
-              o[unit * 4 + i] = ep.last ? pack_bf16x2(x * ep.unit, y * ep.unit) : pack_f16x2(x, y);
+              f[k] = x;
+              f[k + 1] = y;
             }
           }
+          if constexpr (MODE == NS_POLY) {
+            if (ep.also != 0.f) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) o2[half * 16 + i] = pack_f16x2(f[2 * i] * ep.also, f[2 * i + 1] * ep.also);
+            }
+            if (on_diagonal) {
+              const int at = row - col0 - half * 32;      // this row's diagonal element, if it is here
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const bool d0 = at == 2 * i, d1 = at == 2 * i + 1;
+                diagonal = d0 ? f[2 * i] : d1 ? f[2 * i + 1] : diagonal;
+                if (ep.also != 0.f)
+                  o2[half * 16 + i] = pack_f16x2((f[2 * i] + (d0 ? ep.coef2 : 0.f)) * ep.also, (f[2 * i + 1] + (d1 ? ep.coef2 : 0.f)) * ep.also);
+                f[2 * i] = d0 ? 0.f : f[2 * i];
+                f[2 * i + 1] = d1 ? 0.f : f[2 * i + 1];
+              }
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            o[half * 16 + i] = ep.last ? pack_bf16x2(f[2 * i] * ep.unit, f[2 * i + 1] * ep.unit) : pack_f16x2(f[2 * i], f[2 * i + 1]);
         }
+        if (on_diagonal && row >= col0 && row < col0 + 64 && row < M)
+          ep.diag[static_cast<size_t>(z) * ep.diag_len + row] = diagonal * ep.unit;
         if (c + 2 >= slabs) {
           // this warp's last read of the accumulator: hand it back before the stores go out
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+          if (lane == 0 && reused) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
         }
         __syncwarp();
         if (!SYMMETRIC && ep.last && (N & 7)) {      // rows of the result start anywhere
@@ -385,10 +408,10 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       if (slabs <= h) {                              // no slab for this warp (narrow tile): release all the same
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+        if (lane == 0 && reused) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
       }
     }
-    if (lane == 0) tma_store_wait<0>();              // nothing in flight out of shared memory at exit
+    if (lane == 0) tma_store_wait_read<0>();         // nothing in flight out of shared memory at exit
   }
 
   tc_fence_before();
