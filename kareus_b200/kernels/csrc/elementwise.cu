@@ -3,11 +3,10 @@
 //   rmsnorm fwd/bwd      (reference path: TransformerEngine rmsnorm_fwd/bwd kernels)
 //   rope (q and k in one launch, in place, strided views)  (reference: Apex fused RoPE)
 //   swiglu fwd/bwd, dropout-add fwd/bwd, add (reference: torch.compile/Triton fused ops)
-//   embedding gather / scatter-add, vocab-parallel cross entropy (reference: TE Triton CE)
+//   embedding scatter-add (the gather: embedding_sorted.cu), vocab-parallel cross entropy (reference: TE Triton CE)
 //   fused AdamW over flat buffers, sum of squares (reference: TE/Apex multi_tensor kernels)
 #include <cuda_bf16.h>
 #include "launch.h"
-#include "native_ops.h"
 #include "pdl.cuh"
 #include "host_utils.h"
 #include <cuda_runtime.h>
@@ -604,18 +603,6 @@ __global__ void add_kernel(const __nv_bfloat16* __restrict__ a, const __nv_bfloa
 }
 
 // ----------------------------------------------------------------------------- embedding
-__global__ void embedding_fwd_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __restrict__ w,
-                                     __nv_bfloat16* __restrict__ out, long ntok, int H, long vocab_start, long vlocal) {
-  pdl_begin();
-  const int hv = H >> 3;
-  for (long t = blockIdx.x; t < ntok; t += gridDim.x) {
-    const long id = tokens[t] - vocab_start;
-    const bool inside = id >= 0 && id < vlocal;
-    const uint4* src = reinterpret_cast<const uint4*>(w + (inside ? id : 0) * H);
-    uint4* dst = reinterpret_cast<uint4*>(out + t * H);
-    for (int c = threadIdx.x; c < hv; c += blockDim.x) dst[c] = inside ? src[c] : make_uint4(0, 0, 0, 0);
-  }
-}
 // Scatter-add of token gradients into the fp32 weight gradient: 16-byte reductions, four elements a thread (H is a
 // multiple of 4 and rows are 16-byte aligned; `wide` false: single elements).
 __global__ void __launch_bounds__(256)
@@ -1076,13 +1063,6 @@ extern "C" int kb_add(const void* a, const void* b, void* y, long n, cudaStream_
   if (n % 8) return 7;
   KB_LAUNCH_PDL(add_kernel, grid_for(n / 8, 256, 148 * 16), 256, 0, st, (const __nv_bfloat16*)a, (const __nv_bfloat16*)b,
                                                               (__nv_bfloat16*)y, n / 8);
-  KB_CHECK_LAUNCH();
-}
-extern "C" int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long vocab_start,
-                                long vlocal, cudaStream_t st) {
-  if (H % 8) return 7;
-  KB_LAUNCH_PDL(embedding_fwd_kernel, grid_for(ntok, 1, 148 * 16), 128, 0, st, tokens, (const __nv_bfloat16*)w,
-                                                                     (__nv_bfloat16*)out, ntok, H, vocab_start, vlocal);
   KB_CHECK_LAUNCH();
 }
 extern "C" int kb_embedding_bwd(const long* tokens, const void* dout, float* gw, long ntok, int H, long vocab_start,

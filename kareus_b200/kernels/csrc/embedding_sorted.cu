@@ -6,9 +6,9 @@
 // and tokens that make up much of a batch (padding, a frequent word) queue up for the same addresses.  Here the tokens are sorted
 // first and each row of the table gets one addition of a sum that was formed in registers:
 //
-//   1. Stable radix sort of (id, t) by one cluster of eight blocks.  Keys and positions stay in the blocks' shared memory; a pass
-//      ranks the items of a warp by __match_any, adds up the counts of warps, blocks and digits, and writes every item to its place
-//      in the shared memory of the block that owns it.  Tokens of other shards get the key `rows` and end up behind the others.
+//   1. Stable radix sort of (id, t) by one cluster of eight blocks.  Items stay in the blocks' shared memory; a pass ranks the items
+//      of a warp by ballots over the digit's bits, adds up the counts of warps, blocks and digits, and writes every item to its
+//      place in the shared memory of the block that owns it.  Tokens of other shards are left out.
 //   2. Blocks take windows of `window` sorted positions and 1024 columns, sum the rows of each token in order and add the sum to the
 //      table.  A token whose positions cross the border of a window leaves partial sums: the part that began before the window and
 //      the part that goes on after it.
@@ -25,29 +25,44 @@
 namespace kb {
 
 // ----------------------------------------------------------------------------- lookup
+// Four tokens a block: their rows are on their way together, since what one row waits for is the latency of its id and of itself.
+constexpr int EL_TOKENS = 4;
+
 template <bool VEC>
 __global__ void __launch_bounds__(128)
-embedding_scaled_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ out, long ntok,
+embedding_fwd_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ out, long ntok,
                         int H, long first, long rows, float scale) {
   pdl_begin();
-  for (long t = blockIdx.x; t < ntok; t += gridDim.x) {
-    const long id = tokens[t] - first;
-    const bool inside = id >= 0 && id < rows;
-    const __nv_bfloat16* src = w + (inside ? id : 0) * H;
-    __nv_bfloat16* dst = out + t * H;
-    if constexpr (VEC) {
-      for (int c = threadIdx.x * 8; c < H; c += 128 * 8) {
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (inside) {
-          v = *reinterpret_cast<const uint4*>(src + c);
-          uint32_t* p = reinterpret_cast<uint32_t*>(&v);
+  const long t0 = static_cast<long>(blockIdx.x) * EL_TOKENS;
+  long id[EL_TOKENS];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) p[j] = pack_bf16x2(__uint_as_float(p[j] << 16) * scale, __uint_as_float(p[j] & 0xffff0000u) * scale);
+  for (int k = 0; k < EL_TOKENS; ++k) {
+    id[k] = t0 + k < ntok ? tokens[t0 + k] - first : -1;
+    if (id[k] >= rows) id[k] = -1;
+  }
+  if constexpr (VEC) {
+    for (int c = threadIdx.x * 8; c < H; c += 128 * 8) {
+      uint4 v[EL_TOKENS];
+#pragma unroll
+      for (int k = 0; k < EL_TOKENS; ++k)
+        v[k] = id[k] >= 0 ? __ldg(reinterpret_cast<const uint4*>(w + id[k] * H + c)) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int k = 0; k < EL_TOKENS; ++k) {
+        if (scale != 1.f) {
+          uint32_t* p = reinterpret_cast<uint32_t*>(&v[k]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            p[j] = id[k] >= 0 ? pack_bf16x2(__uint_as_float(p[j] << 16) * scale, __uint_as_float(p[j] & 0xffff0000u) * scale) : 0u;
         }
-        *reinterpret_cast<uint4*>(dst + c) = v;
+        if (t0 + k < ntok) *reinterpret_cast<uint4*>(out + (t0 + k) * H + c) = v[k];
       }
-    } else {
-      for (int c = threadIdx.x; c < H; c += 128) dst[c] = __float2bfloat16(inside ? __bfloat162float(src[c]) * scale : 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < EL_TOKENS; ++k) {
+      if (t0 + k >= ntok) break;
+      for (int c = threadIdx.x; c < H; c += 128)
+        out[(t0 + k) * H + c] = __float2bfloat16(id[k] >= 0 ? __bfloat162float(w[id[k] * H + c]) * scale : 0.f);
     }
   }
 }
@@ -58,13 +73,14 @@ constexpr int ES_THREADS = 1024;
 constexpr int ES_WARPS = ES_THREADS / 32;
 constexpr int ES_PER_BLOCK = 8192;             // items
 constexpr int ES_MOST = ES_BLOCKS * ES_PER_BLOCK;
-constexpr int ES_BINS = 256;
+constexpr int ES_BITS = 9;                     // of a digit at most: two passes for up to 2^18 rows
+constexpr int ES_BINS = 1 << ES_BITS;
 constexpr int ES_STEPS = ES_PER_BLOCK / ES_THREADS;        // items a thread at most
 
-__device__ __forceinline__ void st_cluster(uint32_t local, uint32_t rank, uint32_t v) {
+__device__ __forceinline__ void st_cluster(uint32_t local, uint32_t rank, uint2 v) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(local), "r"(rank));
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
 }
 __device__ __forceinline__ uint32_t ld_cluster(uint32_t local, uint32_t rank) {
   uint32_t a, v;
@@ -73,57 +89,69 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t local, uint32_t rank) {
   return v;
 }
 
-// ids / order [n]: keys in ascending order and where they stood.  `per`: items of a block (a multiple of 32, at most ES_PER_BLOCK,
-// ES_BLOCKS * per >= n); `passes` digits of `bits` (at most 8) bits hold every key 0 .. rows.
+// ids / order [n]: keys below `rows` in ascending order and where they stood; ids behind them are `rows`.  `per`: items of a block (a
+// multiple of 32, at most ES_PER_BLOCK, ES_BLOCKS * per >= n); `passes` digits of `bits` (at most ES_BITS) bits hold every key.
+// Tokens of other shards leave in the first pass.
 __global__ void __cluster_dims__(ES_BLOCKS, 1, 1) __launch_bounds__(ES_THREADS, 1)
 embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
                       uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
-  extern __shared__ uint32_t sm[];
+  extern __shared__ uint4 sm[];
   __shared__ uint32_t count[ES_BINS], base[ES_BINS], warp_sum[ES_BINS / 32];
-  uint32_t* const hist = sm;                              // [warps][bins]
-  uint32_t *src = sm + ES_WARPS * ES_BINS, *dst = src + 2 * per;       // keys, positions
+  uint32_t* const hist = reinterpret_cast<uint32_t*>(sm);              // [warps][bins] of 16 bits
+  constexpr int HIST_WORDS = ES_BINS / 2;
+  uint2 *src = reinterpret_cast<uint2*>(hist + ES_WARPS * HIST_WORDS), *dst = src + per;      // (key, position)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = blockIdx.x;
-  const int begin = static_cast<int>(rank) * per, here = max(0, min(per, n - begin));
-  // a warp takes consecutive items, 32 at a time, so that its ranks follow their order
-  const int per_warp = ((per + ES_WARPS - 1) / ES_WARPS + 31) / 32 * 32, steps = per_warp / 32;
   const int bins = 1 << bits;
+  const int all = n;
+  int begin = static_cast<int>(rank) * per, here = max(0, min(per, n - begin));
   pdl_begin();
   for (int i = tid; i < here; i += ES_THREADS) {
     const long id = tokens[begin + i] - first;
-    src[i] = static_cast<uint32_t>(id >= 0 && id < rows ? id : rows);
-    src[per + i] = begin + i;
+    src[i] = make_uint2(static_cast<uint32_t>(id >= 0 && id < rows ? id : rows), begin + i);
   }
-  cluster_sync_all();
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    for (int i = tid; i < ES_WARPS * bins; i += ES_THREADS) hist[(i >> bits) * ES_BINS + (i & (bins - 1))] = 0;
+    // a warp takes consecutive items, 32 at a time, so that its ranks follow their order
+    const int per_warp = ((per + ES_WARPS - 1) / ES_WARPS + 31) / 32 * 32, steps = per_warp / 32;
+    const int used = min(ES_WARPS, (here + per_warp - 1) / per_warp);          // warps with items
+    for (int i = tid; i < used * (HIST_WORDS / 4); i += ES_THREADS) sm[i] = make_uint4(0u, 0u, 0u, 0u);
     __syncthreads();
     uint32_t where[ES_STEPS];
+    uint16_t* const mine = reinterpret_cast<uint16_t*>(hist + warp * HIST_WORDS);
 #pragma unroll
     for (int s = 0; s < ES_STEPS; ++s) {
-      if (s < steps) {
-        const int i = warp * per_warp + s * 32 + lane;
-        const bool in = i < here;
-        const uint32_t d = in ? (src[i] >> shift) & (bins - 1) : ES_BINS;
-        const uint32_t peers = __match_any_sync(0xffffffffu, d);
-        uint32_t* h = hist + warp * ES_BINS + (in ? d : 0);
-        const uint32_t before = in ? *h : 0;
+      const int i = warp * per_warp + s * 32 + lane;
+      if (s < steps && warp * per_warp + s * 32 < here) {
+        const uint32_t key = i < here ? src[i].x : static_cast<uint32_t>(rows), d = (key >> shift) & (bins - 1);
+        const bool in = key < rows;
+        uint32_t peers = __ballot_sync(0xffffffffu, in);                       // lanes with the same digit
+#pragma unroll
+        for (int b = 0; b < ES_BITS; ++b) {
+          if (b < bits) {
+            const bool one = d >> b & 1u;
+            const uint32_t v = __ballot_sync(0xffffffffu, one);
+            peers &= one ? v : ~v;
+          }
+        }
+        const uint32_t before = in ? mine[d] : 0u;
         __syncwarp();
-        if (in && lane == __ffs(peers) - 1) *h = before + __popc(peers);
+        if (in && lane == __ffs(peers) - 1) mine[d] = static_cast<uint16_t>(before + __popc(peers));
         __syncwarp();
         where[s] = before + __popc(peers & ((1u << lane) - 1));
       }
     }
     __syncthreads();
-    if (tid < bins) {                                     // counts of the warps before, of the block
+    if (tid < bins / 2 || tid == 0) {                     // counts of the warps before, of the block; two digits a word
       uint32_t sum = 0;
-      for (int w = 0; w < ES_WARPS; ++w) {
-        const uint32_t c = hist[w * ES_BINS + tid];
-        hist[w * ES_BINS + tid] = sum;
+#pragma unroll 4
+      for (int w = 0; w < used; ++w) {
+        const uint32_t c = hist[w * HIST_WORDS + tid];
+        hist[w * HIST_WORDS + tid] = sum;
         sum += c;
       }
-      count[tid] = sum;
+      count[2 * tid] = sum & 0xffffu;
+      count[2 * tid + 1] = sum >> 16;
     }
     cluster_sync_all();
     uint32_t total = 0, before = 0;                       // of this digit in the cluster, in the blocks before
@@ -150,28 +178,38 @@ embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long firs
       for (int w = 0; w < warp; ++w) add += warp_sum[w];
       base[tid] = add + scan - total + before;
     }
+    if (p == 0) {                                         // what is left, spread evenly again
+      n = 0;
+#pragma unroll
+      for (int w = 0; w < ES_BINS / 32; ++w) n += static_cast<int>(warp_sum[w]);
+    }
+    const int next_per = max(32, (n + ES_BLOCKS - 1) / ES_BLOCKS);
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < ES_STEPS; ++s) {
       const int i = warp * per_warp + s * 32 + lane;
       if (s < steps && i < here) {
-        const uint32_t key = src[i], d = (key >> shift) & (bins - 1);
-        const uint32_t at = base[d] + hist[warp * ES_BINS + d] + where[s];
-        const uint32_t block = at / static_cast<uint32_t>(per), slot = at - block * per;
-        const uint32_t to = smem_u32(dst + slot);
-        st_cluster(to, block, key);
-        st_cluster(to + per * 4, block, src[per + i]);
+        const uint2 item = src[i];
+        if (item.x < rows) {
+          const uint32_t d = (item.x >> shift) & (bins - 1);
+          const uint32_t at = base[d] + mine[d] + where[s], block = at / static_cast<uint32_t>(next_per);
+          st_cluster(smem_u32(dst + (at - block * next_per)), block, item);
+        }
       }
     }
     cluster_sync_all();
-    uint32_t* const t = src;
+    per = next_per;
+    begin = static_cast<int>(rank) * per;
+    here = max(0, min(per, n - begin));
+    uint2* const t = src;
     src = dst;
     dst = t;
   }
   for (int i = tid; i < here; i += ES_THREADS) {
-    ids[begin + i] = src[i];
-    order[begin + i] = src[per + i];
+    ids[begin + i] = src[i].x;
+    order[begin + i] = src[i].y;
   }
+  for (int i = n + static_cast<int>(rank) * ES_THREADS + tid; i < all; i += ES_BLOCKS * ES_THREADS) ids[i] = static_cast<uint32_t>(rows);
 }
 
 // ----------------------------------------------------------------------------- sums
@@ -190,20 +228,27 @@ struct EmbeddingSum {
   float scale;
 };
 
+// Eight columns of the table's gradient.
 template <bool VEC>
-__device__ __forceinline__ void flush(float* dst, const float (&acc)[8], int left, bool add) {
+__device__ __forceinline__ void load_sums(const float* src, float (&g)[8], int left) {
   if constexpr (VEC) {
-    if (add) {
-      red_add_f32x4(reinterpret_cast<float4*>(dst), make_float4(acc[0], acc[1], acc[2], acc[3]));
-      red_add_f32x4(reinterpret_cast<float4*>(dst) + 1, make_float4(acc[4], acc[5], acc[6], acc[7]));
-    } else {
-      reinterpret_cast<float4*>(dst)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      reinterpret_cast<float4*>(dst)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-    }
+    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+    g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = j < left ? src[j] : 0.f;
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void store_sums(float* dst, const float (&v)[8], int left) {
+  if constexpr (VEC) {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < left) dst[j] = add ? dst[j] + acc[j] : acc[j];
+      if (j < left) dst[j] = v[j];
   }
 }
 
@@ -225,11 +270,15 @@ __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const Embe
   bool began = id[1] != id[0];                            // the token at hand starts in this window
   for (int b = 0; b < len; b += EW_BATCH) {
     if (id[1 + b] >= p.rows) break;                       // tokens of other shards: nothing but those from here on
+    // the batch's rows, and the table's rows that its sums go to, are on their way together
     uint4 v[EW_BATCH];
+    float old[EW_BATCH][8];
+    bool starts = began;
 #pragma unroll
     for (int j = 0; j < EW_BATCH; ++j) {
       v[j] = make_uint4(0u, 0u, 0u, 0u);
-      if (b + j < len && id[1 + b + j] < p.rows) {
+      const uint32_t me = b + j < len ? id[1 + b + j] : NONE;
+      if (me < p.rows) {
         const __nv_bfloat16* src = p.dout + static_cast<size_t>(pos[b + j]) * p.H + col;
         if constexpr (VEC) {
           v[j] = __ldcs(reinterpret_cast<const uint4*>(src));
@@ -239,24 +288,34 @@ __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const Embe
           for (int k = 0; k < 8; ++k)
             if (k < left) q[k >> 1] |= static_cast<uint32_t>(__bfloat16_as_ushort(src[k])) << (k & 1 ? 16 : 0);
         }
+        const bool ends = id[2 + b + j] != me;
+        if (ends && starts) load_sums<VEC>(p.grad + static_cast<size_t>(me) * p.H + col, old[j], left);
+        if (ends) starts = true;
       }
     }
 #pragma unroll
     for (int j = 0; j < EW_BATCH; ++j) {
-      if (b + j < len && id[1 + b + j] < p.rows) {
+      const uint32_t me = b + j < len ? id[1 + b + j] : NONE;
+      if (me < p.rows) {
         const uint32_t q[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           acc[2 * k] += __uint_as_float(q[k] << 16);
           acc[2 * k + 1] += __uint_as_float(q[k] & 0xffff0000u);
         }
-        const uint32_t me = id[1 + b + j];
         const bool last = b + j == len - 1, ends = id[2 + b + j] != me;
         if (last || ends) {
+          float* dst;
+          if (began && ends) {
+            dst = p.grad + static_cast<size_t>(me) * p.H + col;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] *= p.scale;
-          if (began && ends) flush<VEC>(p.grad + static_cast<size_t>(me) * p.H + col, acc, left, true);
-          else flush<VEC>((began ? p.after : p.before) + static_cast<size_t>(blockIdx.x) * p.H + col, acc, left, false);
+            for (int k = 0; k < 8; ++k) acc[k] = fmaf(acc[k], p.scale, old[j][k]);
+          } else {
+            dst = (began ? p.after : p.before) + static_cast<size_t>(blockIdx.x) * p.H + col;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) acc[k] *= p.scale;
+          }
+          store_sums<VEC>(dst, acc, left);
 #pragma unroll
           for (int k = 0; k < 8; ++k) acc[k] = 0.f;
           began = true;
@@ -266,50 +325,97 @@ __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const Embe
   }
 }
 
-// Tokens that cross windows: block x looks whether one begins in window x and goes on, and adds up its parts.  Eight warps take
-// consecutive runs of the windows behind the first, 128 columns a block.
+// Tokens that cross windows.  A warp looks whether one begins in its window and goes on.  If it ends within the next few windows the
+// warp adds up the parts itself; otherwise the block's eight warps share them, each a run of consecutive windows, eight of them on
+// their way at once.  128 columns a block.
 constexpr int EC_THREADS = 256;
+constexpr int EC_WARPS = EC_THREADS / 32;
 constexpr int EC_COLS = 128;
+constexpr int EC_SHORT = 8;
 
-__global__ void __launch_bounds__(EC_THREADS) embedding_join_kernel(const EmbeddingSum p, int windows) {
-  __shared__ float part[EC_THREADS / 32][EC_COLS];
-  __shared__ int end;
-  pdl_begin();
-  const int w = blockIdx.x, W = p.window, border = (w + 1) * W;         // first position of the next window
-  if (border >= p.n) return;
-  const uint32_t me = p.ids[border];
-  if (me >= p.rows || p.ids[border - 1] != me) return;
-  if (p.ids[border - W] == me && w > 0 && p.ids[border - W - 1] == me) return;   // it began before this window
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) end = windows;
-  __syncthreads();
-  // the first window from w + 1 on that the token does not leave: keys are sorted, so that is where the next border's key differs
-  for (int v = w + 1; v < windows; v += EC_THREADS) {
-    const int mine = v + static_cast<int>(threadIdx.x), next = (mine + 1) * W;
-    const bool stops = mine < windows && (next >= p.n || p.ids[next] != me);
-    if (stops) atomicMin(&end, mine);
-    if (__syncthreads_or(stops)) break;
-  }
-  const int last = min(end, windows - 1), many = last - w;              // windows w + 1 .. last hold `before` parts
-  const int share = (many + EC_THREADS / 32 - 1) / (EC_THREADS / 32);
-  const int col = blockIdx.y * EC_COLS + lane;                          // columns col, + 32, + 64, + 96
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const int from = w + 1 + warp * share, to = min(from + share, last + 1);
-#pragma unroll 4
+// Sum of the parts that windows from .. to - 1 hold of four columns, in order.
+template <bool VEC>
+__device__ __forceinline__ float4 sum_parts(const EmbeddingSum& p, int from, int to, int col, int left) {
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (left <= 0) return acc;
+#pragma unroll 8
   for (int v = from; v < to; ++v) {
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (col + 32 * k < p.H) acc[k] += p.before[static_cast<size_t>(v) * p.H + col + 32 * k];
+    const float* q = p.before + static_cast<size_t>(v) * p.H + col;
+    float4 x;
+    if constexpr (VEC) x = *reinterpret_cast<const float4*>(q);
+    else x = make_float4(q[0], left > 1 ? q[1] : 0.f, left > 2 ? q[2] : 0.f, left > 3 ? q[3] : 0.f);
+    acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
   }
+  return acc;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(EC_THREADS) embedding_join_kernel(const EmbeddingSum p) {
+  __shared__ __align__(16) float part[EC_WARPS][EC_COLS];
+  __shared__ int last_of[EC_WARPS];             // last window of a long token that begins in the warp's window, or 0
+  pdl_begin();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, W = p.window;
+  const int w = blockIdx.x * EC_WARPS + warp, border = (w + 1) * W;     // first position of the next window
+  const int col = blockIdx.y * EC_COLS + lane * 4, left = p.H - col;    // four columns
+  const uint32_t NONE = 0xffffffffu;
+  uint32_t me = NONE;
+  bool begins = false;
+  if (border < p.n) {
+    me = p.ids[border];
+    const uint32_t end_here = p.ids[border - 1], first_here = p.ids[border - W], before = w > 0 ? p.ids[border - W - 1] : NONE;
+    begins = me < p.rows && end_here == me && !(first_here == me && before == me);
+  }
+  int last = 0;                                 // windows w + 1 .. last hold `before` parts of the token
+  if (begins) {
+    // the first window that it does not leave: keys are sorted, so that is where the next border's key differs
+    for (int v = w + 1; !last; v += 128) {
+      bool stop[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) part[warp][lane + 32 * k] = acc[k];
-  __syncthreads();
-  const int c = blockIdx.y * EC_COLS + threadIdx.x;
-  if (threadIdx.x < EC_COLS && c < p.H) {
-    float sum = p.after[static_cast<size_t>(w) * p.H + c];
+      for (int k = 0; k < 4; ++k) {
+        const int next = (v + k * 32 + lane + 1) * W;
+        stop[k] = next >= p.n || p.ids[next] != me;
+      }
 #pragma unroll
-    for (int i = 0; i < EC_THREADS / 32; ++i) sum += part[i][threadIdx.x];
-    p.grad[static_cast<size_t>(me) * p.H + c] += sum;
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t stops = __ballot_sync(0xffffffffu, stop[k]);
+        if (!last && stops) last = v + k * 32 + __ffs(stops) - 1;
+      }
+    }
+    if (last - w <= EC_SHORT) {
+      float4 sum = sum_parts<VEC>(p, w + 1, last + 1, col, left);
+      const float* a = p.after + static_cast<size_t>(w) * p.H + col;
+      float* g = p.grad + static_cast<size_t>(me) * p.H + col;
+      if constexpr (VEC) {
+        if (left > 0) {
+          const float4 x = *reinterpret_cast<const float4*>(a), y = *reinterpret_cast<const float4*>(g);
+          *reinterpret_cast<float4*>(g) = make_float4(y.x + (x.x + sum.x), y.y + (x.y + sum.y), y.z + (x.z + sum.z), y.w + (x.w + sum.w));
+        }
+      } else {
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < left) g[k] += a[k] + v[k];
+      }
+      last = 0;
+    }
+  }
+  if (lane == 0) last_of[warp] = last;
+  if (!__syncthreads_or(last)) return;
+  for (int i = 0; i < EC_WARPS; ++i) {
+    const int end = last_of[i];
+    if (!end) continue;                         // the same for the whole block
+    const int start = blockIdx.x * EC_WARPS + i, share = (end - start + EC_WARPS - 1) / EC_WARPS;
+    const int from = start + 1 + warp * share, to = min(from + share, end + 1);
+    *reinterpret_cast<float4*>(&part[warp][lane * 4]) = sum_parts<VEC>(p, from, to, col, left);
+    __syncthreads();
+    const int c = blockIdx.y * EC_COLS + threadIdx.x;
+    if (threadIdx.x < EC_COLS && c < p.H) {
+      float sum = p.after[static_cast<size_t>(start) * p.H + c];
+#pragma unroll
+      for (int k = 0; k < EC_WARPS; ++k) sum += part[k][threadIdx.x];
+      p.grad[static_cast<size_t>(p.ids[(start + 1) * W]) * p.H + c] += sum;
+    }
+    __syncthreads();
   }
 }
 
@@ -328,12 +434,13 @@ static long chunk_bytes(long n, int H) {
 
 }  // namespace kb
 
-extern "C" int kb_embedding_fwd_scaled(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,
+extern "C" int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,
                                        cudaStream_t stream) {
   if (ntok <= 0 || H <= 0 || rows <= 0) return 7;
   const bool vec = H % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-  const unsigned grid = static_cast<unsigned>(ntok < 148 * 16 ? ntok : 148 * 16);
-  KB_LAUNCH_PDL((vec ? kb::embedding_scaled_kernel<true> : kb::embedding_scaled_kernel<false>), grid, 128, 0, stream, tokens,
+  const long grid = (ntok + kb::EL_TOKENS - 1) / kb::EL_TOKENS;
+  if (grid >= 1L << 31) return 7;
+  KB_LAUNCH_PDL((vec ? kb::embedding_fwd_kernel<true> : kb::embedding_fwd_kernel<false>), static_cast<unsigned>(grid), 128, 0, stream, tokens,
                 static_cast<const __nv_bfloat16*>(w), static_cast<__nv_bfloat16*>(out), ntok, H, first, rows, scale);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
@@ -353,15 +460,15 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
   if (ntok <= 0 || H <= 0 || rows <= 0 || rows >= 1L << 31 || !work || reinterpret_cast<uintptr_t>(work) % 256) return 7;
   const bool vec = H % 8 == 0 && reinterpret_cast<uintptr_t>(dout) % 16 == 0 && reinterpret_cast<uintptr_t>(grad) % 16 == 0;
   int bits_all = 1;
-  while (rows >> bits_all) ++bits_all;                    // keys 0 .. rows
-  const int passes = (bits_all + 7) / 8, bits = (bits_all + passes - 1) / passes;
+  while ((rows - 1) >> bits_all) ++bits_all;              // keys 0 .. rows - 1
+  const int passes = (bits_all + ES_BITS - 1) / ES_BITS, bits = (bits_all + passes - 1) / passes;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 7;
   if (!configured[dev]) {
     const cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (ES_WARPS * ES_BINS + 4 * ES_PER_BLOCK) * 4);
+                                               ES_WARPS * ES_BINS * 2 + 2 * ES_PER_BLOCK * 8);
     if (e != cudaSuccess) return 1000 + static_cast<int>(e);
     configured[dev] = true;
   }
@@ -385,11 +492,12 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
     s.H = H;
     s.rows = static_cast<uint32_t>(rows);
     s.scale = scale;
-    KB_LAUNCH_PDL(embedding_sort_kernel, ES_BLOCKS, ES_THREADS, (ES_WARPS * ES_BINS + 4 * per) * 4, stream, tokens + at, n, per, first, rows,
+    KB_LAUNCH_PDL(embedding_sort_kernel, ES_BLOCKS, ES_THREADS, ES_WARPS * ES_BINS * 2 + 2 * per * 8, stream, tokens + at, n, per, first, rows,
                   passes, bits, ids, order);
     KB_LAUNCH_PDL((vec ? embedding_window_kernel<true> : embedding_window_kernel<false>), dim3(windows, (H + EW_COLS - 1) / EW_COLS),
                   EW_THREADS, 0, stream, s);
-    KB_LAUNCH_PDL(embedding_join_kernel, dim3(windows, (H + EC_COLS - 1) / EC_COLS), EC_THREADS, 0, stream, s, windows);
+    KB_LAUNCH_PDL((vec ? embedding_join_kernel<true> : embedding_join_kernel<false>), dim3((windows + EC_WARPS - 1) / EC_WARPS, (H + EC_COLS - 1) / EC_COLS),
+                  EC_THREADS, 0, stream, s);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);

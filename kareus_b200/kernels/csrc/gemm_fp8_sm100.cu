@@ -24,14 +24,14 @@ namespace kb {
 
 constexpr int G8_BM = 256;                     // rows of a tile (128 per CTA)
 constexpr int G8_BK = 128;                     // one block of the scales; 128 bytes
-constexpr int G8_MAX_STAGES = 8;
+constexpr int G8_MAX_STAGES = 16;
 constexpr int G8_EPI_WARPS = 8;                // 4 TMEM lane quarters x 2 sets of column slabs
 constexpr int G8_THREADS = (2 + G8_EPI_WARPS) * 32;
-constexpr int G8_A_BYTES = 128 * G8_BK;        // 16 KB: this CTA's rows of A
+constexpr int G8_A_BYTES = 128 * G8_BK;        // 16 KB: this CTA's rows of A, where there are that many
 constexpr int G8_SF_BYTES = 2048;              // scales of 512 of K: 512 bytes for A, up to 1024 for B, in the first stage of each 512
 constexpr int G8_RING = 5 * (2 * G8_A_BYTES + G8_SF_BYTES);
 constexpr int G8_STG_BYTES = G8_EPI_WARPS * 4096;
-constexpr int G8_SMEM = G8_RING + G8_STG_BYTES + 256 + 1024;
+constexpr int G8_SMEM = G8_RING + G8_STG_BYTES + 512 + 1024;
 constexpr int G8_ACC1 = 224;                   // column of the second accumulator
 constexpr int G8_SF_COL = 480;                 // scales: two buffers of 16 columns (4 for A, 8 for B)
 static_assert(G8_SMEM <= 227 * 1024, "shared memory per CTA");
@@ -39,6 +39,7 @@ static_assert(G8_SMEM <= 227 * 1024, "shared memory per CTA");
 struct Fp8Work {
   int tiles_m, tiles_n, group_m, nk;
   int groups_k;                                // 512-wide groups of scales along K
+  int a_rows;                                  // rows of A that a CTA loads: 128, or all there are in whole groups of 8
   __device__ __forceinline__ void coords(int t, int& tm, int& tn) const {
     // m-tiles are taken in groups of `group_m`; inside a group the m index runs fastest
     const int per_group = group_m * tiles_n;
@@ -92,7 +93,10 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
   const int tiles = w.tiles_m * w.tiles_n;
   const int half_n = bn >> 1;
-  const int b_bytes = half_n * G8_BK, stage_bytes = G8_A_BYTES + b_bytes;
+  const int a_bytes = w.a_rows * G8_BK, b_bytes = half_n * G8_BK, stage_bytes = a_bytes + b_bytes;
+  // An A of few rows: the MMA reads 128 all the same, of each CTA.  What it finds behind the loaded ones only reaches rows of the
+  // accumulator that nobody stores, and lies in this block's shared memory (the stages are followed by 32 KB of staging).
+  const bool load_a = rank == 0 || M > 128;
   const int stages = min(G8_MAX_STAGES, G8_RING / (stage_bytes + G8_SF_BYTES));
   uint8_t* const sf = smem + stages * stage_bytes;          // a slot per stage
   const bool shared_cols = bn > G8_ACC1;
@@ -128,6 +132,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     // ------------------------------------------------------------------ producer (each CTA: its own halves)
     if (elect_one()) {
       const uint32_t full0 = cluster_addr(full, 0);
+      const uint32_t tx = 2u * b_bytes + (M > 128 ? 2u : 1u) * a_bytes;      // bytes of both CTAs, counted on the leader's barrier
       int s = 0;
       uint32_t ph = 1;
       bool ok = true;
@@ -140,12 +145,12 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         for (int kb_ = 0; kb_ < w.nk; ++kb_) {
           if (!mbar_wait(&empty[s], ph, abort_flag, status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
           uint8_t* a_dst = smem + s * stage_bytes;
-          uint8_t* b_dst = a_dst + G8_A_BYTES;
+          uint8_t* b_dst = a_dst + a_bytes;
           const uint32_t bar = full0 + s * 8;
           const bool scales = (kb_ & 3) == 0;
-          if (rank == 0) mbar_expect_tx(&full[s], 2u * stage_bytes + (scales ? sf_tx : 0u));
+          if (rank == 0) mbar_expect_tx(&full[s], tx + (scales ? sf_tx : 0u));
           const int k0 = kb_ * G8_BK;
-          tma_load_2d_pair(a_dst, &tmA, bar, k0, m0);
+          if (load_a) tma_load_2d_pair(a_dst, &tmA, bar, k0, m0);
           tma_load_2d_pair(b_dst, &tmB, bar, k0, n0 + rank * half_n);
           if (scales) {
             uint8_t* d = sf + s * G8_SF_BYTES;
@@ -167,7 +172,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     // ------------------------------------------------------------------ MMA issuer (leader)
     if (rank == 0 && elect_one()) {
       const uint32_t smem0 = smem_u32(smem), sf0 = smem_u32(sf);
-      const uint64_t ad0 = make_smem_desc(smem0, 16, 1024), bd0 = make_smem_desc(smem0 + G8_A_BYTES, 16, 1024);
+      const uint64_t ad0 = make_smem_desc(smem0, 16, 1024), bd0 = make_smem_desc(smem0 + a_bytes, 16, 1024);
       uint32_t tile_i = 0, group_i = 0;
       int s = 0;
       uint32_t ph = 0;
@@ -345,13 +350,14 @@ extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, c
   w.tiles_m = (M + G8_BM - 1) / G8_BM;
   w.nk = (K + G8_BK - 1) / G8_BK;
   w.groups_k = (w.nk + 3) / 4;
+  w.a_rows = M < 128 ? (M + 7) / 8 * 8 : 128;
   // Width of the tiles: clocks of a step of 128 are the larger of the tensor cores' (2 per column) and of the loads' (64 bytes a
-  // clock reach an SM: 256 for A, one per column for B), times the tiles that a pair works through.
+  // clock reach an SM: two per row of A, one per column for B), times the tiles that a pair works through.
   int bn = 256;
   double best = 0;
   for (int b = 256; b >= 64; b -= 64) {
     const long tiles = (long)w.tiles_m * ((N + b - 1) / b);
-    const double cost = (double)((tiles + pairs - 1) / pairs) * (w.nk * (double)(2 * b > 256 + b ? 2 * b : 256 + b) + 1500.0);
+    const double cost = (double)((tiles + pairs - 1) / pairs) * (w.nk * (double)(b > 2 * w.a_rows ? 2 * b : 2 * w.a_rows + b) + 1500.0);
     if (b == 256 || cost < best * 0.97) {
       best = cost;
       bn = b;
@@ -368,7 +374,7 @@ extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, c
   int rc;
   {
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)M}, str[1] = {(uint64_t)lda};
-    const uint32_t box[2] = {(uint32_t)G8_BK, 128u};
+    const uint32_t box[2] = {(uint32_t)G8_BK, (uint32_t)w.a_rows};
     if ((rc = make_tmap(&tmA, A, 1, 2, dims, str, box, 3))) return rc;
   }
   {

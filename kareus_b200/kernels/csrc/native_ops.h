@@ -13,8 +13,7 @@ long kb_newton_schulz_bytes(long batch, long m, long n);
 int kb_newton_schulz_launches(int m, int n, int steps);
 int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
                      float scale_q, void* out, void* work, int* status, cudaStream_t stream);
-int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long vocab_start, long vlocal, cudaStream_t st);
-int kb_embedding_fwd_scaled(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,
+int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,
                             cudaStream_t stream);
 long kb_embedding_sorted_bytes(long ntok, int H);
 int kb_embedding_bwd_sorted(const long* tokens, const void* dout, float* grad, long ntok, int H, long first, long rows, float scale,

@@ -180,12 +180,8 @@ PyObject* embedding_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const long* pt = reinterpret_cast<const long*>(t->data_ptr());
   const void* pw = w->data_ptr();
   void* po = out.data_ptr();
-  const bool plain_copy = scale == 1.0 && H % 8 == 0 && aligned(*w);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
-  const int rc = without_gil([&] {
-    return plain_copy ? kb_embedding_fwd(pt, pw, po, n, H, first, rows, stream)
-                      : kb_embedding_fwd_scaled(pt, pw, po, n, H, first, rows, scale, stream);
-  });
+  const int rc = without_gil([&] { return kb_embedding_fwd(pt, pw, po, n, H, first, rows, scale, stream); });
   if (!finish(rc, "embedding_fwd", 1)) return nullptr;
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS

@@ -93,7 +93,6 @@ def _declare(L) -> None:
         "kb_dropout_add_fwd": [P, P, P, LNG, F, U, P],
         "kb_dropout_bwd": [P, P, LNG, F, U, P],
         "kb_add": [P, P, P, LNG, P],
-        "kb_embedding_fwd": [P, P, P, LNG, I, LNG, LNG, P],
         "kb_embedding_bwd": [P, P, P, LNG, I, LNG, LNG, P],
         "kb_ce_stats": [P, P, P, P, P, LNG, I, LNG, P],
         "kb_ce_grad": [P, P, P, P, P, LNG, I, LNG, P],
@@ -103,7 +102,7 @@ def _declare(L) -> None:
         "kb_newton_schulz": [P, I, I, I, I, F, F, F, I, F, F, F, P, P, P, P],
         "kb_newton_schulz_launches": [I, I, I],
         "kb_muon_step": [P, P, P, P, P, I, I, F, I, F, F, P, F, F, F, I, F, F, F, P, P, P],
-        "kb_embedding_fwd_scaled": [P, P, P, LNG, I, LNG, LNG, F, P],
+        "kb_embedding_fwd": [P, P, P, LNG, I, LNG, LNG, F, P],
         "kb_embedding_bwd_sorted": [P, P, P, LNG, I, LNG, LNG, F, P, P],
         "kb_sumsq": [P, LNG, I, P, P],
         "kb_clip_scale": [P, F, P, P],
@@ -738,12 +737,8 @@ def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
     out = torch.empty(tuple(tokens.shape) + (H,), dtype=weight.dtype, device=weight.device)
     if not out.numel():
         return out
-    if scale == 1.0 and H % 8 == 0 and weight.data_ptr() % 16 == 0:
-        _check(lib().kb_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
-                                      int(vocab_start), weight.shape[0], _stream()), "embedding_fwd")
-    else:
-        _check(lib().kb_embedding_fwd_scaled(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
-                                             int(vocab_start), weight.shape[0], float(scale), _stream()), "embedding_fwd")
+    _check(lib().kb_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
+                                         int(vocab_start), weight.shape[0], float(scale), _stream()), "embedding_fwd")
     _count()
     return out
 
