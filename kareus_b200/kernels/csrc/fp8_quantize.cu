@@ -11,7 +11,8 @@
 // them at (r % 32) * 16 + (r / 32) * 4; [ceil(rows / 128)][ceil(pieces / 4)] such blocks.  Bytes past the edge are 0.
 //
 // What bounds it: memory.  A block of 256 threads takes a 128 x 128 tile, reads it once (16 lanes a row, 16 bytes each), writes the
-// rows' bytes from registers and the columns' by way of shared memory, 32 tokens (one sector) of a column a thread.
+// rows' bytes from registers and the columns' by way of shared memory, in whole lines of 128 tokens (as 32-byte pieces of a thread
+// each they took a third longer).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -47,22 +48,27 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax) {
 __device__ __forceinline__ float inverse_scale(uint32_t byte) {
   return __uint_as_float(byte == 255u ? 0x7fc00000u : (254u - byte) << 23);
 }
-// Two values as two bytes; `lo` goes to the low one.
+// Four values as four bytes, the first in the lowest.
 template <bool E5M2>
-__device__ __forceinline__ uint32_t quantize2(float lo, float hi) {
-  uint16_t r;
-  if constexpr (E5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-  else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+__device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d) {
+  uint32_t r;
+  if constexpr (E5M2)
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e5m2x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e5m2x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
+  else
+    asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};\n\t}"
+        : "=r"(r) : "f"(a), "f"(b), "f"(c), "f"(d));
   return r;
 }
 // The two bf16 of a word, each times its factor.
 __device__ __forceinline__ float2 scaled(uint32_t v, float2 inv) {
   return __fmul2_rn(make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)), inv);
 }
-// Larger |x| of two pairs of bf16, element by element; a NaN stays one.
+// Larger |x| of two pairs of bf16, element by element; a NaN stays one.  The signs of the result mean nothing.
 __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
-  const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<__nv_bfloat162*>(&a)), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
-  return *reinterpret_cast<const uint32_t*>(&m);
+  uint32_t m;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  return m;
 }
 
 // Where the scale of (row, piece) lies.
@@ -112,7 +118,7 @@ __global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Qu
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max_abs2(m, max_abs2(max_abs2(v[i].x, v[i].y), max_abs2(v[i].z, v[i].w)));
-    m = max(m & 0x7fffu, m >> 16);
+    m = max(m & 0x7fffu, m >> 16 & 0x7fffu);
     m = __reduce_max_sync(0xffffffffu, m);
     if ((tid & 31) == 0) whole[tid >> 5] = m;
     __syncthreads();
@@ -133,7 +139,7 @@ __global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Qu
 #pragma unroll
         for (int s = 8; s > 0; s >>= 1) m = max_abs2(m, __shfl_xor_sync(0xffffffffu, m, s));
         byte[i] = scale_byte<TOP>(m & 0x7fffu);
-        byte[i + 1] = scale_byte<TOP>(m >> 16);
+        byte[i + 1] = scale_byte<TOP>(m >> 16 & 0x7fffu);
       }
     }
     uint8_t* dst = p.q + (r0 + rsub) * p.ldq + col;
@@ -143,8 +149,7 @@ __global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Qu
       const float f = inverse_scale(byte[i]);
       const float2 inv = make_float2(f, f);
       const float2 a = scaled(v[i].x, inv), b = scaled(v[i].y, inv), c = scaled(v[i].z, inv), d = scaled(v[i].w, inv);
-      const uint2 o = make_uint2(quantize2<E5M2>(a.x, a.y) | quantize2<E5M2>(b.x, b.y) << 16,
-                                 quantize2<E5M2>(c.x, c.y) | quantize2<E5M2>(d.x, d.y) << 16);
+      const uint2 o = make_uint2(quantize4<E5M2>(a.x, a.y, b.x, b.y), quantize4<E5M2>(c.x, c.y, d.x, d.y));
       if (r0 + i * 16 + rsub < p.rows && col < p.ldq) *reinterpret_cast<uint2*>(dst) = o;
       dst += 16 * p.ldq;
       if (unit == 0) row_byte[i * 16 + rsub] = static_cast<uint8_t>(byte[i]);
@@ -167,15 +172,16 @@ __global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Qu
       __syncthreads();
       m = max_abs2(max_abs2(part[0][pair], part[1][pair]), max_abs2(part[2][pair], part[3][pair]));
       b0 = scale_byte<TOP>(m & 0x7fffu);
-      b1 = scale_byte<TOP>(m >> 16);
+      b1 = scale_byte<TOP>(m >> 16 & 0x7fffu);
     }
     if (rg == 0) {
       col_byte[2 * pair] = static_cast<uint8_t>(b0);
       col_byte[2 * pair + 1] = static_cast<uint8_t>(b1);
     }
+    if constexpr (SQUARE) __syncthreads();                // (else the one above) everybody has read the tile
+    // The columns' bytes go through its place, so that a column's 128 leave as whole lines: 16-byte units, swizzled by column pair.
     const float2 inv = make_float2(inverse_scale(b0), inverse_scale(b1));
-    const int c = c0 + 2 * pair, r = r0 + rg * 32;
-    uint8_t* dst = p.qt + c * p.ldqt + r;                 // ldqt is a multiple of 16: 16-byte units are whole or outside
+    uint4* const bytes = reinterpret_cast<uint4*>(tile);  // [128 columns][8 units]
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t lo[4], hi[4];                              // 16 rows of either column
@@ -183,12 +189,20 @@ __global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Qu
       for (int j = 0; j < 4; ++j) {
         const uint32_t* x = w + half * 16 + 4 * j;
         const float2 e = scaled(x[0], inv), f = scaled(x[1], inv), g = scaled(x[2], inv), h = scaled(x[3], inv);
-        lo[j] = quantize2<E5M2>(e.x, f.x) | quantize2<E5M2>(g.x, h.x) << 16;
-        hi[j] = quantize2<E5M2>(e.y, f.y) | quantize2<E5M2>(g.y, h.y) << 16;
+        lo[j] = quantize4<E5M2>(e.x, f.x, g.x, h.x);
+        hi[j] = quantize4<E5M2>(e.y, f.y, g.y, h.y);
       }
-      if (r + half * 16 < p.ldqt) {
-        if (c < p.cols) *reinterpret_cast<uint4*>(dst + half * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (c + 1 < p.cols) *reinterpret_cast<uint4*>(dst + p.ldqt + half * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      const int at = (rg * 2 + half) ^ (pair & 7);
+      bytes[2 * pair * 8 + at] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      bytes[(2 * pair + 1) * 8 + at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    }
+    __syncthreads();
+    const int cu = tid & 7;                               // ldqt is a multiple of 16: 16-byte units are whole or outside
+    if (r0 + cu * 16 < p.ldqt) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int c = k * 32 + (tid >> 3);
+        if (c0 + c < p.cols) *reinterpret_cast<uint4*>(p.qt + (c0 + c) * p.ldqt + r0 + cu * 16) = bytes[c * 8 + (cu ^ ((c >> 1) & 7))];
       }
     }
   }
