@@ -10,7 +10,7 @@ int kb_fp8_quantize(const void* x, long rows, long cols, long ld, void* q, long 
 int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, const void* B, const void* SB, int fmt_b, long ldb, void* C,
                 long ldc, int M, int N, int K, int out_f32, int accumulate, int* status, cudaStream_t stream);
 long kb_newton_schulz_bytes(long batch, long m, long n);
-int kb_newton_schulz_launches(int m, int n, int steps);
+int kb_newton_schulz_launches(int batch, int m, int n, int steps);
 int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
                      float scale_q, void* out, void* work, int* status, cudaStream_t stream);
 int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,

@@ -11,7 +11,7 @@
 // P) X.  Norms are summed in fp32 per thread and fp64 beyond, in a fixed order.
 //
 // Long matrices.  X_{k+1} = Q_k X_k with Q_k = a I + P_k, and G_{k+1} = Q_k G_k Q_k, where everything but X is as small as the shorter
-// side.  Where the longer side is at least 1.5 times the shorter one and that is long enough to be bound by arithmetic, G is carried from step to step so (T = Q G, G' = Q T), the Q are
+// side.  Where the longer side is at least 1.5 times the shorter one and it saves time (ns_carries), G is carried from step to step so (T = Q G, G' = Q T), the Q are
 // multiplied up, and X is read twice per segment of two or three steps instead of twice per step: five steps of a matrix with
 // sides m and r m take 6 r + 14 units of m^3 multiplications instead of 15 r + 5.  G of a carried step is off by the roundings
 // before it, and small singular values suffer most from that; with segments of three and two steps (the singular values grow in
@@ -51,16 +51,25 @@ enum NsMode : int {
   NS_UPDATE_T = 3,   // X <- X (a + d) + X P
   NS_CARRY = 4,      // Y <- (a + d) Y + P Y for symmetric Y that P commutes with
   NS_APPLY = 5,      // X <- Q X or X Q
+  NS_GRAM_PARTS = 6, // parts of X Xt along K, as fp32 sums
 };
-__host__ __device__ constexpr bool ns_symmetric(int mode) { return mode == NS_GRAM || mode == NS_POLY || mode == NS_CARRY; }
-__host__ __device__ constexpr bool ns_adds(int mode) { return mode != NS_GRAM && mode != NS_APPLY; }
+__host__ __device__ constexpr bool ns_symmetric(int mode) { return mode != NS_UPDATE && mode != NS_UPDATE_T && mode != NS_APPLY; }
+__host__ __device__ constexpr bool ns_adds(int mode) { return mode != NS_GRAM && mode != NS_GRAM_PARTS && mode != NS_APPLY; }
 
 struct NsWork {
   int batch, pairs, tiles_m, tiles_n, per_matrix, nk;      // pairs: matrices per item of the batch (NS_CARRY takes G and Q at once)
   int ratio;                                   // column tiles per 256 rows, where only the upper tiles are computed; else 0
   int group_m;
-  __device__ __forceinline__ int units() const { return pairs * batch * per_matrix; }
+  int parts;                                   // of the sum over K (NS_GRAM_PARTS): all tiles of part 0, then those of part 1, ...
+  __device__ __forceinline__ int tiles() const { return pairs * batch * per_matrix; }
+  __device__ __forceinline__ int units() const { return parts * tiles(); }
+  __device__ __forceinline__ void steps(int u, int& kb0, int& kb1) const {
+    const int part = u / tiles();
+    kb0 = split_begin(nk, parts, part);
+    kb1 = split_begin(nk, parts, part + 1);
+  }
   __device__ __forceinline__ void decode(int u, int& pair, int& z, int& tm, int& tn) const {
+    if (parts > 1) u %= tiles();
     z = u / per_matrix;
     int t = u - z * per_matrix;
     pair = z / batch;
@@ -169,8 +178,10 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         int pair, z, tm, tn;
         w.decode(u, pair, z, tm, tn);
         const int pa = MODE == NS_CARRY ? 0 : pair;      // P serves both
+        int kb0 = 0, kb1 = w.nk;
+        if constexpr (MODE == NS_GRAM_PARTS) w.steps(u, kb0, kb1);
         const int m0 = tm * NS_BM + rank * 128, n0 = tn * bn + rank * half_n;
-        for (int kb_ = 0; kb_ < w.nk; ++kb_) {
+        for (int kb_ = kb0; kb_ < kb1; ++kb_) {
           if (!mbar_wait(&empty[s], ph, abort_flag, status, ST_TIMEOUT_EMPTY)) { ok = false; break; }
           uint8_t* a_dst = smem + s * stage_bytes;
           uint8_t* b_dst = a_dst + NS_A_BYTES;
@@ -216,16 +227,18 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         if (!mbar_wait(&tempty[buf], ((tile_i >> 1) & 1u) ^ 1u, abort_flag, status, ST_TIMEOUT_TMEM_EMPTY)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * 256;
-        for (int kb_ = 0; kb_ < w.nk; ++kb_) {
+        int kb0 = 0, kb1 = w.nk;
+        if constexpr (MODE == NS_GRAM_PARTS) w.steps(u, kb0, kb1);
+        for (int kb_ = kb0; kb_ < kb1; ++kb_) {
           if (!mbar_wait(&full[s], ph, abort_flag, status, ST_TIMEOUT_FULL)) { ok = false; break; }
           tc_fence_after();
           const uint64_t ad = ad0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
           const uint64_t bd = bd0 + static_cast<uint64_t>(s * (stage_bytes >> 4));
 #pragma unroll
           for (int k = 0; k < NS_BK / 16; ++k)
-            umma_ss_pair(d_tmem, ad + k * ka, bd + k * kb, idesc, (kb_ > 0 || k > 0) ? 1u : 0u);
+            umma_ss_pair(d_tmem, ad + k * ka, bd + k * kb, idesc, (kb_ > kb0 || k > 0) ? 1u : 0u);
           umma_commit_pair(&empty[s]);
-          if (kb_ == w.nk - 1) umma_commit_pair(&tfull[buf]);
+          if (kb_ == kb1 - 1) umma_commit_pair(&tfull[buf]);
           if (++s == stages) { s = 0; ph ^= 1u; }
         }
       }
@@ -297,6 +310,31 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           __syncwarp();
         }
         const int col0 = tn * bn + c * 64;
+        if constexpr (MODE == NS_GRAM_PARTS) {           // the sums themselves, 32 columns at a time, to the workspace
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t a[32];
+            __syncwarp();
+            tmem_ld_32x32(taddr + c * 64 + half * 32, a);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              st_shared_v4(smem_u32(stg_row) + half * 4096 + ((j ^ (lane & 7)) << 4), a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
+          }
+          if (c + 2 >= slabs) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0 && reused) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&tmC2, stg0, c * 64, u * NS_BM + rank * 128 + q * 32);
+            tma_store_2d(&tmC2, stg0 + 4096, c * 64 + 32, u * NS_BM + rank * 128 + q * 32);
+            tma_store_commit();
+          }
+          continue;
+        }
         uint32_t o[32];
         uint32_t o2[MODE == NS_POLY ? 32 : 1];           // a I + P
         // the diagonal crosses few slabs: the others are spared the search for it
@@ -421,6 +459,38 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 512);
   }
+}
+
+// G from the sums of its parts along K, added in order: 32 x 32 elements a block, as they are and transposed.
+__global__ void __launch_bounds__(256)
+ns_sum_parts_kernel(const float* __restrict__ work, __half* __restrict__ G, long ldg, int side, int bn, const NsWork w, float alpha) {
+  __shared__ float t[32][33];
+  pdl_begin();
+  const int per_tile = 8 * (bn / 32), tile = blockIdx.x / per_tile, sub = blockIdx.x - tile * per_tile;
+  int pair, z, tm, tn;
+  w.decode(tile, pair, z, tm, tn);
+  const int r0 = sub % 8 * 32, c0 = sub / 8 * 32;       // inside the tile
+  const int row0 = tm * NS_BM + r0, col0 = tn * bn + c0;
+  if (row0 >= side || col0 >= side) return;
+  const int r = threadIdx.x >> 3, c = (threadIdx.x & 7) * 4;
+  const float* src = work + (static_cast<size_t>(tile) * NS_BM + r0 + r) * bn + c0 + c;
+  const size_t part = static_cast<size_t>(w.tiles()) * NS_BM * bn;
+  float4 s = *reinterpret_cast<const float4*>(src);
+#pragma unroll 4
+  for (int p = 1; p < w.parts; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(src + p * part);
+    s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+  }
+  s.x *= alpha; s.y *= alpha; s.z *= alpha; s.w *= alpha;
+  __half* g = G + static_cast<size_t>(z) * side * ldg;
+  // rows hold whole groups of eight columns; what lies behind the last column is zero
+  if (row0 + r < side && col0 + c < ldg)
+    *reinterpret_cast<uint2*>(g + (row0 + r) * ldg + col0 + c) = make_uint2(pack_f16x2(s.x, s.y), pack_f16x2(s.z, s.w));
+  if (tn * bn / NS_BM == tm) return;
+  t[r][c] = s.x; t[r][c + 1] = s.y; t[r][c + 2] = s.z; t[r][c + 3] = s.w;
+  __syncthreads();
+  if (col0 + r < side && row0 + c < ldg)
+    *reinterpret_cast<uint2*>(g + (col0 + r) * ldg + row0 + c) = make_uint2(pack_f16x2(t[c][r], t[c + 1][r]), pack_f16x2(t[c + 2][r], t[c + 3][r]));
 }
 
 // ----------------------------------------------------------------------------- the passes around the products
@@ -588,10 +658,56 @@ muon_apply_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ p, con
 // ----------------------------------------------------------------------------- host side
 constexpr int NS_G = 0, NS_T = 1, NS_Q = 2, NS_P = 4, NS_SLOTS = 5;      // square matrices of the workspace: G, T, two Q, P
 
+// How a product is cut: tile width, tiles and parts of the sum over K.
+struct NsPlan {
+  int bn, tiles_m, tiles_n, per_matrix, nk, parts;
+  double clocks;             // modelled time, with 7 us for a launch, its first loads and its epilogue, 5 us for adding up parts
+};
+static NsPlan ns_plan(int mode, long matrices, int M, int N, int K) {
+  const bool symmetric = ns_symmetric(mode);
+  const int sms = device_sm_count() / 2;
+  NsPlan p{};
+  p.tiles_m = (M + NS_BM - 1) / NS_BM;
+  p.nk = (K + NS_BK - 1) / NS_BK;
+  p.parts = 1;
+  // Width of the tiles: as for the other products on pairs of SMs, clocks of a step of 64 are the larger of the tensor cores' (2 a
+  // column) and of the loads' (64 bytes a clock reach an SM).
+  double best = 0, step = 0;
+  for (int b = 256; b >= 64; b -= 64) {
+    if (symmetric && 256 % b) continue;        // rows of tiles start on the diagonal
+    const int tn = (N + b - 1) / b;
+    long tiles = 0;
+    if (symmetric) for (int i = 0; i < p.tiles_m; ++i) tiles += tn - i * (256 / b);
+    else tiles = (long)p.tiles_m * tn;
+    const long waves = (tiles * matrices + sms - 1) / sms;
+    const double clocks = 2 * b > 256 + b ? 2 * b : 256 + b, cost = (double)waves * (p.nk * clocks + 1500.0);
+    if (!p.bn || cost < best * 0.97) {
+      best = cost;
+      step = clocks;
+      p.bn = b;
+      p.tiles_n = tn;
+      p.per_matrix = (int)tiles;
+    }
+  }
+  // Few tiles and a long sum: parts of 8 steps and more on the SMs that would idle, where that saves more than the 5 us that adding
+  // them up takes.  32 x 14336: 316 us as one part, 122 so.
+  if (mode == NS_GRAM) {
+    const long units = matrices * p.per_matrix;
+    long parts = units ? sms / units : 1;
+    parts = parts > p.nk / 8 ? p.nk / 8 : parts;
+    if (parts > 1 && (p.nk - (p.nk + parts - 1) / parts) * step > 10000.) {
+      p.parts = (int)parts;
+      best = (p.nk + parts - 1) / parts * step + 1500. + 10000.;
+    }
+  }
+  p.clocks = best + 13000.;
+  return p;
+}
+
 struct NsLayout {
   int rows, cols, side;      // side: the smaller of the two
   long ldx, ldg;             // row strides in elements (multiples of 8)
-  long x, g, diag, part, total;                // bytes; g: one square matrix of every item
+  long x, g, diag, part, sums, total;          // bytes; g: one square matrix of every item; sums: parts of a G
   NsLayout(int batch, int m, int n) : rows(m), cols(n), side(m < n ? m : n) {
     const auto up = [](long b) { return (b + 255) / 256 * 256; };
     ldx = (n + 7L) / 8 * 8;
@@ -600,7 +716,9 @@ struct NsLayout {
     g = up(2L * batch * side * ldg);
     diag = up(4L * batch * side);
     part = up(8L * batch * NS_SUM_BLOCKS);
-    total = 2 * x + NS_SLOTS * g + diag + part;
+    const NsPlan p = ns_plan(NS_GRAM, batch, side, side, m < n ? n : m);
+    sums = p.parts > 1 ? up(4L * p.parts * batch * p.per_matrix * NS_BM * p.bn) : 0;
+    total = 2 * x + NS_SLOTS * g + diag + part + sums;
   }
 };
 
@@ -623,33 +741,19 @@ static int ns_map(CUtensorMap* map, const NsMatrix& m, long inner, long rows, lo
 // C [M, N] of each matrix of the batch from A and B: [rows][ld] matrices whose rows run along K (K-major) or along M / N.
 template <bool A_MN, bool B_MN, int MODE>
 static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, const NsMatrix& C2, int batch, int pairs, int M, int N, int K,
-                      const NsEpilogue& ep, int* status, cudaStream_t stream) {
+                      const NsEpilogue& ep, float* sums, int* status, cudaStream_t stream) {
   constexpr bool SYMMETRIC = ns_symmetric(MODE);
   const int sms = device_sm_count() / 2;
+  const NsPlan plan = ns_plan(MODE, (long)batch * pairs, M, N, K);
+  const int bn = plan.bn;
   NsWork w;
   w.batch = batch;
   w.pairs = pairs;
-  w.tiles_m = (M + NS_BM - 1) / NS_BM;
-  w.nk = (K + NS_BK - 1) / NS_BK;
-  // Width of the tiles: as for the other products on pairs of SMs, clocks of a step of 64 are the larger of the tensor cores' (2 a
-  // column) and of the loads' (64 bytes a clock reach an SM).
-  int bn = 0;
-  double best = 0;
-  for (int b = 256; b >= 64; b -= 64) {
-    if (SYMMETRIC && 256 % b) continue;        // rows of tiles start on the diagonal
-    const int tn = (N + b - 1) / b;
-    long tiles = 0;
-    if (SYMMETRIC) for (int i = 0; i < w.tiles_m; ++i) tiles += tn - i * (256 / b);
-    else tiles = (long)w.tiles_m * tn;
-    const long waves = (tiles * batch * pairs + sms - 1) / sms;
-    const double cost = (double)waves * (w.nk * (double)(2 * b > 256 + b ? 2 * b : 256 + b) + 1500.0);
-    if (!bn || cost < best * 0.97) {
-      best = cost;
-      bn = b;
-      w.tiles_n = tn;
-      w.per_matrix = (int)tiles;
-    }
-  }
+  w.tiles_m = plan.tiles_m;
+  w.tiles_n = plan.tiles_n;
+  w.per_matrix = plan.per_matrix;
+  w.nk = plan.nk;
+  w.parts = plan.parts;
   w.ratio = SYMMETRIC ? 256 / bn : 0;
   long gm = (24L << 20) / ((long)NS_BM * K * 2);
   gm = gm < 8 ? 8 : gm > 16 ? 16 : gm;
@@ -674,34 +778,48 @@ static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, c
   if (MODE == NS_POLY && C2.p && ((rc = ns_map(&tmC2, C2, C2.ld, M, batch, pairs, 64, 32, 3)) ||
                                   (rc = ns_map(&tmM2, C2, C2.ld, M, batch, pairs, 32, 64, 0))))
     return rc;
-  auto kern = newton_schulz_kernel<A_MN, B_MN, MODE>;
-  static bool configured[64] = {};
+  const long units = (long)plan.parts * pairs * batch * w.per_matrix;
+  if (units >= 1L << 22) return 7;
+  if (MODE == NS_GRAM && plan.parts > 1) {
+    const uint64_t dims[2] = {(uint64_t)bn, (uint64_t)units * NS_BM}, str[1] = {(uint64_t)bn * 4};
+    const uint32_t box[2] = {32u, 32u};
+    if ((rc = make_tmap(&tmC2, sums, 4, 2, dims, str, box, 3))) return rc;
+  }
+  constexpr int PARTS = MODE == NS_GRAM ? NS_GRAM_PARTS : MODE;
+  auto kern = plan.parts > 1 ? newton_schulz_kernel<A_MN, B_MN, PARTS> : newton_schulz_kernel<A_MN, B_MN, MODE>;
+  static bool configured[2][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 7;
-  if (!configured[dev]) {
+  if (!configured[plan.parts > 1][dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM);
     if (e != cudaSuccess) return 1000 + static_cast<int>(e);
-    configured[dev] = true;
+    configured[plan.parts > 1][dev] = true;
   }
-  const long units = (long)pairs * batch * w.per_matrix;
-  if (units >= 1L << 30) return 7;
   const int grid = 2 * (int)(units < sms ? units : sms);
   KB_LAUNCH_PDL(kern, grid, NS_THREADS, NS_SMEM, stream, tmA, tmB, tmC, tmM, tmC2, tmM2, w, M, N, bn, ep, status);
+  if (MODE == NS_GRAM && plan.parts > 1)
+    KB_LAUNCH_PDL(ns_sum_parts_kernel, (unsigned)(batch * w.per_matrix * 8 * (bn / 32)), 256, 0, stream, (const float*)sums,
+                  static_cast<__half*>(C.p), C.ld, M, bn, w, ep.alpha);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }
 
-// Whether G is carried from step to step (see the head of this file).  One B200, us step by step / carried: 14336 x 4096 3650 / 2560,
-// 6144 x 4096 1842 / 1675.  Below a side of 1024 a product is over before its launch and its epilogue are, and there are no fewer of
-// them: 2048 x 512 139 / 143, three of 333 x 1000 126 / 138.
-static bool ns_carries(int m, int n, int steps) {
-  const long side = m < n ? m : n, other = m < n ? n : m;
-  return steps > 1 && side >= 1024 && 2 * other >= 3 * side;
+// Whether G is carried from step to step (see the head of this file): where the longer side is at least 1.5 times the other and the
+// modelled time is 5 % less.  One B200, us step by step / carried: 14336 x 4096 3650 / 2560, 6144 x 4096 1842 / 1675; where products
+// are over before their launches and epilogues are there is nothing to gain: 2048 x 512 139 / 143, three of 333 x 1000 126 / 138.
+static bool ns_carries(int batch, int m, int n, int steps) {
+  const int side = m < n ? m : n, other = m < n ? n : m;
+  if (steps < 2 || 2L * other < 3L * side) return false;
+  const bool tall = m > n;
+  const double gram = ns_plan(NS_GRAM, batch, side, side, other).clocks, square = ns_plan(NS_CARRY, batch, side, side, side).clocks;
+  const double x = ns_plan(NS_APPLY, batch, tall ? other : side, tall ? side : other, side).clocks;
+  const int segments = steps / 2, products = 3 * steps - segments + steps % 2;    // of G's size: P, T, G' and products of Q
+  return segments * (gram + x) + products * square < 0.95 * steps * (gram + square + x);
 }
 // Steps of the segment that begins with `left` steps to go: three and then two, or only two.
-static int ns_segment(int m, int n, int steps, int left) {
-  if (!ns_carries(m, n, steps)) return 1;
+static int ns_segment(bool carries, int left) {
+  if (!carries) return 1;
   return left % 2 == 1 && left > 1 ? 3 : left < 2 ? left : 2;
 }
 
@@ -712,6 +830,7 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
   uint8_t* const square = work + 2 * lay.x;
   float* const diag = reinterpret_cast<float*>(square + NS_SLOTS * lay.g);
   double* const part = reinterpret_cast<double*>(square + NS_SLOTS * lay.g + lay.diag);
+  float* const sums = reinterpret_cast<float*>(square + NS_SLOTS * lay.g + lay.diag + lay.part);
   const long count = (long)m * n;
   const auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
   const long per_block = 8L * NS_SUM_THREADS;
@@ -735,15 +854,16 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
   const float unit = 1.f / scale, unit_q = 1.f / scale_q;      // powers of two
   const auto slot = [&](int i) { return NsMatrix{square + i * lay.g, ldg, 0}; };
   const NsMatrix none{nullptr, 0, 0};
+  const bool carries = ns_carries(batch, m, n, steps);
   int cur = 0, rc = 0;
   for (int done = 0; done < steps;) {
-    const int len = ns_segment(m, n, steps, steps - done);
+    const int len = ns_segment(carries, steps - done);
     const bool last = done + len == steps;
     const NsMatrix xi{x[cur], lay.ldx, 0}, xo{last ? out : x[cur ^ 1], last ? (long)n : lay.ldx, 0};
     NsEpilogue eg{};
     eg.alpha = eg.unit = unit;
-    rc = tall ? ns_product<true, true, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, m, eg, status, stream)
-              : ns_product<false, false, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, n, eg, status, stream);
+    rc = tall ? ns_product<true, true, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, m, eg, sums, status, stream)
+              : ns_product<false, false, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, n, eg, sums, status, stream);
     if (rc) return rc;
     // P of the G at hand; with `q` also a I + P
     const auto poly = [&](bool q) {
@@ -758,8 +878,8 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
       e.unit = unit;
       e.coef2 = a * scale;
       e.also = q ? scale_q * unit : 0.f;
-      return ns_product<false, false, NS_POLY>(slot(NS_G), slot(NS_G), slot(NS_P), q ? slot(NS_Q) : none, batch, 1, side, side, side, e, status,
-                                               stream);
+      return ns_product<false, false, NS_POLY>(slot(NS_G), slot(NS_G), slot(NS_P), q ? slot(NS_Q) : none, batch, 1, side, side, side, e, sums,
+                                               status, stream);
     };
     // slot `to` = (a I + P) slot `from`, with a second pair of slots where `from2` says so
     const auto carry = [&](int from, int to, int from2, int to2) {
@@ -777,7 +897,7 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
       e.diag = diag;
       e.diag_len = side;
       e.unit = unit;
-      return ns_product<false, false, NS_CARRY>(slot(NS_P), y, z, none, batch, pairs, side, side, side, e, status, stream);
+      return ns_product<false, false, NS_CARRY>(slot(NS_P), y, z, none, batch, pairs, side, side, side, e, sums, status, stream);
     };
     NsEpilogue eu{};
     eu.diag = diag;
@@ -791,8 +911,8 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
       eu.lde = eu.e_cols = (int)lay.ldx;
       eu.alpha = eu.unit = unit;
       eu.coef = a;
-      rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, slot(NS_P), xo, none, batch, 1, m, n, side, eu, status, stream)
-                : ns_product<false, true, NS_UPDATE>(slot(NS_P), xi, xo, none, batch, 1, m, n, side, eu, status, stream);
+      rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, slot(NS_P), xo, none, batch, 1, m, n, side, eu, sums, status, stream)
+                : ns_product<false, true, NS_UPDATE>(slot(NS_P), xi, xo, none, batch, 1, m, n, side, eu, sums, status, stream);
     } else {
       int q = NS_Q, spare = NS_Q + 1;
       if ((rc = poly(true)) || (rc = carry(NS_G, NS_T, 0, 0)) || (rc = carry(NS_T, NS_G, 0, 0))) return rc;
@@ -806,8 +926,8 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
       }
       eu.alpha = unit_q;
       eu.unit = unit;
-      rc = tall ? ns_product<false, false, NS_APPLY>(xi, slot(q), xo, none, batch, 1, m, n, side, eu, status, stream)
-                : ns_product<false, true, NS_APPLY>(slot(q), xi, xo, none, batch, 1, m, n, side, eu, status, stream);
+      rc = tall ? ns_product<false, false, NS_APPLY>(xi, slot(q), xo, none, batch, 1, m, n, side, eu, sums, status, stream)
+                : ns_product<false, true, NS_APPLY>(slot(q), xi, xo, none, batch, 1, m, n, side, eu, sums, status, stream);
     }
     if (rc) return rc;
     done += len;
@@ -827,11 +947,14 @@ extern "C" long kb_newton_schulz_bytes(long batch, long m, long n) {
   return kb::ns_sizes_ok(batch, m, n) ? kb::NsLayout((int)batch, (int)m, (int)n).total : -1;
 }
 // Kernels that a call of the functions below launches for a batch (the optimizer step: one more).
-extern "C" int kb_newton_schulz_launches(int m, int n, int steps) {
+extern "C" int kb_newton_schulz_launches(int batch, int m, int n, int steps) {
+  const int side = m < n ? m : n;
+  const int gram = kb::ns_plan(kb::NS_GRAM, batch, side, side, m < n ? n : m).parts > 1 ? 2 : 1;
+  const bool carries = kb::ns_carries(batch, m, n, steps);
   int launches = 2;
   for (int done = 0; done < steps;) {
-    const int len = kb::ns_segment(m, n, steps, steps - done);
-    launches += len == 1 ? 3 : 1 + 3 + 3 * (len - 1) - 1 + 1;
+    const int len = kb::ns_segment(carries, steps - done);
+    launches += gram + (len == 1 ? 2 : 3 * len);
     done += len;
   }
   return launches;

@@ -153,7 +153,7 @@ PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int rc = without_gil([&] {
     return kb_newton_schulz(px, bf16, batch, m, n, a, b, c, steps, eps, scale, scale_q, po, pw, status, stream);
   });
-  if (!finish(rc, "orthogonalize", kb_newton_schulz_launches(m, n, steps))) return nullptr;
+  if (!finish(rc, "orthogonalize", kb_newton_schulz_launches(batch, m, n, steps))) return nullptr;
   return THPVariable_Wrap(std::move(out));
   END_HANDLE_TH_ERRORS
 }

@@ -79,7 +79,7 @@ def orthogonalize(x, steps, coefficients, eps):
     _check(lib().kb_newton_schulz(x.data_ptr(), 1 if x.dtype == torch.bfloat16 else 0, batch, m, n, *coefficients, steps, eps, *scales,
                                   out.data_ptr(), work.data_ptr(), status_word(x.device).data_ptr(), _stream()),
            f"orthogonalize {batch} x {m} x {n}")
-    _count(lib().kb_newton_schulz_launches(m, n, steps))
+    _count(lib().kb_newton_schulz_launches(batch, m, n, steps))
     return out
 
 
@@ -111,5 +111,5 @@ def muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, step
                               0 if grad_scale_tensor is None else grad_scale_tensor.data_ptr(), *coefficients, steps, eps,
                               *fp16_scales(steps, coefficients), work.data_ptr(), status_word(g.device).data_ptr(), _stream()),
            f"muon_step {rows} x {cols}")
-    _count(lib().kb_newton_schulz_launches(rows, cols, steps) + 1)
+    _count(lib().kb_newton_schulz_launches(1, rows, cols, steps) + 1)
     return o

@@ -48,7 +48,8 @@ def matrices(batch, m, n, device="cuda", seed=0, std=1e-3):
 
 
 SIZES = [(1, 1, 1), (1, 1, 7), (1, 9, 1), (1, 5, 3), (2, 16, 16), (1, 64, 200), (3, 130, 70), (3, 333, 1000), (1, 1000, 333), (2, 512, 512),
-         (1, 2048, 512), (40, 24, 40), (1, 300, 1504), (1, 1100, 2600), (1, 1500, 900), (1, 257, 256), (1, 256, 321), (2, 1030, 1800), (1, 1700, 1024)]
+         (1, 2048, 512), (40, 24, 40), (1, 300, 1504), (1, 1100, 2600), (1, 1500, 900), (1, 257, 256), (1, 256, 321), (2, 1030, 1800), (1, 1700, 1024),
+         (1, 24, 9000), (1, 7001, 40), (2, 300, 6000), (1, 5003, 130)]
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
