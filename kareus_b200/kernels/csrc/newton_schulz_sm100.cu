@@ -661,7 +661,7 @@ constexpr int NS_G = 0, NS_T = 1, NS_Q = 2, NS_P = 4, NS_SLOTS = 5;      // squa
 // How a product is cut: tile width, tiles and parts of the sum over K.
 struct NsPlan {
   int bn, tiles_m, tiles_n, per_matrix, nk, parts;
-  double clocks;             // modelled time, with 7 us for a launch, its first loads and its epilogue, 5 us for adding up parts
+  double clocks;             // modelled time, with 6 to 7 us for a launch, its first loads and its epilogue, 5 us for adding up parts
 };
 static NsPlan ns_plan(int mode, long matrices, int M, int N, int K) {
   const bool symmetric = ns_symmetric(mode);
@@ -700,7 +700,7 @@ static NsPlan ns_plan(int mode, long matrices, int M, int N, int K) {
       best = (p.nk + parts - 1) / parts * step + 1500. + 10000.;
     }
   }
-  p.clocks = best + 13000.;
+  p.clocks = best + (mode == NS_CARRY ? 11000. : 13000.);
   return p;
 }
 
@@ -806,8 +806,9 @@ static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, c
 }
 
 // Whether G is carried from step to step (see the head of this file): where the longer side is at least 1.5 times the other and the
-// modelled time is 5 % less.  One B200, us step by step / carried: 14336 x 4096 3650 / 2560, 6144 x 4096 1842 / 1675; where products
-// are over before their launches and epilogues are there is nothing to gain: 2048 x 512 139 / 143, three of 333 x 1000 126 / 138.
+// modelled time is less.  One B200, us step by step / carried: 14336 x 4096 3650 / 2560, 6144 x 4096 1842 / 1675, 1024 x 4096 195 / 177,
+// 20 x 14336 134 / 109; where all products are over before their launches and epilogues are there is nothing to gain: 2048 x 512 139 /
+// 143, three of 333 x 1000 126 / 138.
 static bool ns_carries(int batch, int m, int n, int steps) {
   const int side = m < n ? m : n, other = m < n ? n : m;
   if (steps < 2 || 2L * other < 3L * side) return false;
@@ -815,7 +816,7 @@ static bool ns_carries(int batch, int m, int n, int steps) {
   const double gram = ns_plan(NS_GRAM, batch, side, side, other).clocks, square = ns_plan(NS_CARRY, batch, side, side, side).clocks;
   const double x = ns_plan(NS_APPLY, batch, tall ? other : side, tall ? side : other, side).clocks;
   const int segments = steps / 2, products = 3 * steps - segments + steps % 2;    // of G's size: P, T, G' and products of Q
-  return segments * (gram + x) + products * square < 0.95 * steps * (gram + square + x);
+  return segments * (gram + x) + products * square < steps * (gram + square + x);
 }
 // Steps of the segment that begins with `left` steps to go: three and then two, or only two.
 static int ns_segment(bool carries, int left) {
