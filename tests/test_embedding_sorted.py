@@ -99,6 +99,15 @@ def test_one_token_many_times(n, share):
 
 
 @gpu
+@pytest.mark.parametrize("H", [7, 24, 136, 520])
+def test_long_runs_beside_short_ones(H):
+    """Several tokens that fill many windows, one after the other, with tokens of a few rows between them."""
+    runs = torch.tensor([3, 900, 1, 70, 2000, 5, 130, 64, 64, 1, 700, 12, 20, 300, 63, 65])
+    t = torch.repeat_interleave(torch.arange(16), runs).cuda()
+    check(t[torch.randperm(t.numel(), generator=torch.Generator().manual_seed(1)).cuda()], table(16, H), 0, 1.0)
+
+
+@gpu
 def test_runs_of_every_length():
     """Sorted tokens whose runs start and end at every place of a window."""
     runs = torch.arange(1, 200)

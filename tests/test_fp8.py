@@ -102,10 +102,38 @@ def test_quantize_edges(device, fmt):
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_square_blocks_that_are_not_finite(device):
+    x = sample(300, 300, device)
+    x[5, 7], x[200, 290], x[299, 0] = float("inf"), float("nan"), -float("inf")
+    for kw in ({"cols": True}, {}, {"rows": False, "cols": True}):
+        r, c = K.fp8_quantize(x, square=True, **kw)
+        if r is not None:
+            check_quantized(r, x, "e4m3", True)
+            assert torch.isnan(r.dequantize()[:128, :128]).all() and not torch.isnan(r.dequantize()[:128, 128:]).any()
+        if c is not None:
+            check_quantized(c, x.t(), "e4m3", True)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """Rows more than 2^30 elements apart, in and out."""
+    step = 1_200_000_000
+    buf = torch.zeros(2 * step + 512, dtype=torch.bfloat16, device="cuda")
+    x = buf.as_strided((3, 512), (step, 1))
+    x.copy_(sample(3, 512, "cuda", 20))
+    r, c = K.fp8_quantize(x, cols=True)
+    check_quantized(r, x, "e4m3")
+    check_quantized(c, x.t(), "e4m3")
+    out = buf.as_strided((3, 200), (step, 1), 256)
+    b, _ = K.fp8_quantize(sample(200, 512, "cuda", 21))
+    check_product(K.fp8_gemm(r, b, out=out), r, b)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
 def test_quantize_views(device):
     """Rows of a wider buffer, an odd offset, a transposed matrix, every second row."""
     base = sample(200, 400, device)
-    for x in (base[:, 16:216], base[3:, 1:258], base.t(), base[::2], base[:1, 5:90], base[:, 7:8]):
+    for x in (base[:, 16:216], base[3:, 1:258], base.t(), base[::2], base[:1, 5:90], base[:, 7:8], base[4].expand(9, 400)):
         r, c = K.fp8_quantize(x, cols=True)
         check_quantized(r, x, "e4m3")
         check_quantized(c, x.t(), "e4m3")
@@ -158,6 +186,17 @@ def test_gemm_tile_widths(width):
         b, _ = K.fp8_quantize(sample(N, Kd, "cuda", 4))
         check_product(K.fp8_gemm(a, b), a, b)
         check_product(K.fp8_gemm(a, b, out_dtype=torch.float32), a, b)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 7, 8, 9, 64, 100, 120, 121, 127, 128, 129, 255, 257])
+def test_gemm_few_rows(M):
+    """Rows of A that are loaded: all there are, in groups of 8, below 128."""
+    a, _ = K.fp8_quantize(sample(M, 700, "cuda", 3))
+    for N in (40, 300, 9000):
+        b, _ = K.fp8_quantize(sample(N, 700, "cuda", 4))
+        check_product(K.fp8_gemm(a, b), a, b)
+        check_product(K.fp8_gemm(b, a, out_dtype=torch.float32), b, a)
 
 
 @gpu
