@@ -71,7 +71,8 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t saddr) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
 }
 
-template <bool OUT_F32, bool ACCUM>
+// NARROW: a bf16 output in tiles of 64 columns, whose epilogue takes slabs of 32 so that both sets of warps have one.
+template <bool OUT_F32, bool ACCUM, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1)
 gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmSA, const __grid_constant__ CUtensorMap tmSB,
@@ -217,9 +218,11 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int q = warp & 3;                   // TMEM lane quarter
     const int h = (warp - 2) >> 2;            // this warp takes the column slabs h, h + 2, ...
     uint8_t* stg = smem + G8_RING + (warp - 2) * 4096;
-    constexpr int SLAB = OUT_F32 ? 32 : 64;   // output columns of one 128-byte wide slab
+    constexpr int SLAB = OUT_F32 || NARROW ? 32 : 64;          // output columns of a slab, 64 bytes wide if NARROW, else 128
+    constexpr int UNITS = NARROW ? 4 : 8, PER_UNIT = OUT_F32 ? 4 : 8;
+    const int swizzle = NARROW ? (lane >> 1) & 3 : lane & 7;   // of the 16-byte units of this thread's row, as TMA expects
     const int slabs = bn / SLAB, mine = (slabs - h + 1) >> 1;
-    const uint32_t stg_row = smem_u32(stg) + lane * 128;
+    const uint32_t stg_row = smem_u32(stg) + lane * (UNITS * 16);
     uint32_t tile_i = 0;
     for (int t = first; t < tiles; t += step, ++tile_i) {
       int tm, tn;
@@ -234,9 +237,15 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // the slab with the columns that the other accumulator shares comes first: the last one of the first accumulator, the
         // first one of the second
         const int c = h + 2 * (buf == 0 ? mine - 1 - j : j);
-        uint32_t o[32];
+        uint32_t o[4 * UNITS];
         __syncwarp();
-        if constexpr (OUT_F32) {
+        if constexpr (NARROW) {
+          uint32_t v[32];
+          tmem_ld_32x32(taddr + c * 32, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = pack_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        } else if constexpr (OUT_F32) {
           tmem_ld_32x32(taddr + c * 32, o);
           tmem_ld_wait();
         } else {
@@ -260,8 +269,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (lane == 0) tma_store_wait_read<0>();      // the previous slab has left the staging buffer
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          st_shared_v4(stg_row + ((i ^ (lane & 7)) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        for (int i = 0; i < UNITS; ++i)
+          st_shared_v4(stg_row + ((i ^ swizzle) << 4), o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         fence_proxy_async_smem();
         __syncwarp();
         const int col = tn * bn + c * SLAB;
@@ -269,8 +278,8 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // elsewhere, are stored one by one
         if (col + SLAB > whole && row0 + lane < M) {
           for (int x = max(whole, col); x < min(N, col + SLAB); ++x) {
-            const int i = x - col, unit = i / (OUT_F32 ? 4 : 8), sub = i % (OUT_F32 ? 4 : 8);
-            const uint8_t* src = stg + lane * 128 + ((unit ^ (lane & 7)) << 4);
+            const int i = x - col, unit = i / PER_UNIT, sub = i % PER_UNIT;
+            const uint8_t* src = stg + lane * (UNITS * 16) + ((unit ^ swizzle) << 4);
             const size_t at = static_cast<size_t>(row0 + lane) * ldc + x;
             if constexpr (!OUT_F32) static_cast<__nv_bfloat16*>(C)[at] = reinterpret_cast<const __nv_bfloat16*>(src)[sub];
             else if constexpr (ACCUM) static_cast<float*>(C)[at] += reinterpret_cast<const float*>(src)[sub];
@@ -302,7 +311,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   }
 }
 
-template <bool OUT_F32, bool ACCUM>
+template <bool OUT_F32, bool ACCUM, bool NARROW>
 static int launch_fp8(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmSA, const CUtensorMap& tmSB, void* C,
                       int M, int N, long ldc, const Fp8Work& w, int bn, uint32_t idesc, int pairs, int* status, cudaStream_t stream) {
   CUtensorMap tmC = tmA;                       // without columns that TMA can store there is no map and none is needed
@@ -311,11 +320,11 @@ static int launch_fp8(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUte
   if (whole) {
     const uint64_t dims[2] = {(uint64_t)whole, (uint64_t)M};
     const uint64_t str[1] = {(uint64_t)ldc * (OUT_F32 ? 4 : 2)};
-    const uint32_t box[2] = {OUT_F32 ? 32u : 64u, 32u};
-    const int rc = make_tmap(&tmC, C, OUT_F32 ? 4 : 2, 2, dims, str, box, 3);
+    const uint32_t box[2] = {OUT_F32 || NARROW ? 32u : 64u, 32u};
+    const int rc = make_tmap(&tmC, C, OUT_F32 ? 4 : 2, 2, dims, str, box, NARROW ? 2 : 3);
     if (rc) return rc;
   }
-  auto kern = gemm_fp8_kernel<OUT_F32, ACCUM>;
+  auto kern = gemm_fp8_kernel<OUT_F32, ACCUM, NARROW>;
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -388,7 +397,9 @@ extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, c
   if ((rc = make_tmap(&tmSA, SA, 4, 2, da, str, box, 0))) return rc;
   if ((rc = make_tmap(&tmSB, SB, 4, 2, db, str, box, 0))) return rc;
   const uint32_t idesc = make_idesc_mxf8(G8_BM, bn, fmt_a, fmt_b);
-  if (!out_f32) return launch_fp8<false, false>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
-  if (accumulate) return launch_fp8<true, true>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
-  return launch_fp8<true, false>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
+  if (!out_f32 && bn == 64)
+    return launch_fp8<false, false, true>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
+  if (!out_f32) return launch_fp8<false, false, false>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
+  if (accumulate) return launch_fp8<true, true, false>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
+  return launch_fp8<true, false, false>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
 }

@@ -118,7 +118,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 __device__ __forceinline__ float2 f16_pair(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
-template <bool A_MN, bool B_MN, int MODE>
+// NARROW: tiles of 64 columns, whose epilogue takes slabs of 32 so that both sets of warps have one.
+template <bool A_MN, bool B_MN, int MODE, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NS_THREADS, 1)
 newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmM,
@@ -247,25 +248,29 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
   } else {
     // ------------------------------------------------------------------ epilogue
     const int q = warp & 3;                   // TMEM lane quarter
-    const int h = (warp - 2) >> 2;            // this warp takes the 64-column slabs h, h + 2, ...
+    const int h = (warp - 2) >> 2;            // this warp takes the column slabs h, h + 2, ...
+    constexpr int HALVES = NARROW ? 1 : 2;    // of 32 columns in a slab
+    constexpr int SLAB = 32 * HALVES, UNITS = SLAB / 8, ROW = UNITS * 16;      // columns, 16-byte units and bytes of a slab's row
+    // units are swizzled by row, as TMA expects rows of 64 or 128 bytes
+    const auto swizzle = [](int r) { return NARROW ? (r >> 1) & 3 : r & 7; };
     uint8_t* const stg0 = smem + NS_RING + (warp - 2) * 8192;
-    const int slabs = bn / 64;
+    const int slabs = bn / SLAB;
     constexpr bool ADDS = ns_adds(MODE), SYMMETRIC = ns_symmetric(MODE);
-    uint4 v[8];                               // the tile that is added: 32 rows x 64 columns, on its way
+    uint4 v[UNITS];                           // the slab that is added, on its way
     float2 d_next = make_float2(0.f, 0.f);    // NS_UPDATE_T: P's diagonal for two of these columns, lane by lane
     auto fetch = [&](int u, int c) {
       int pair, z, tm, tn;
       w.decode(u, pair, z, tm, tn);
-      const int row0 = tm * NS_BM + rank * 128 + q * 32, col = tn * bn + c * 64 + (lane & 7) * 8;
+      const int row0 = tm * NS_BM + rank * 128 + q * 32, col = tn * bn + c * SLAB + lane % UNITS * 8;
       const __half* src = ep.e + pair * ep.e_pair + z * ep.e_batch + col;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = row0 + i * 4 + (lane >> 3);
+      for (int i = 0; i < UNITS; ++i) {
+        const int r = row0 + i * (32 / UNITS) + lane / UNITS;
         v[i] = make_uint4(0u, 0u, 0u, 0u);
         if (r < M && col < ep.e_cols) v[i] = *reinterpret_cast<const uint4*>(src + static_cast<size_t>(r) * ep.lde);
       }
       if constexpr (MODE == NS_UPDATE_T) {
-        const int dc = tn * bn + c * 64 + 2 * lane;
+        const int dc = tn * bn + c * SLAB + 2 * lane;
         const float* d = ep.diag + static_cast<size_t>(z) * ep.diag_len;
         d_next = make_float2(dc < N ? d[dc] : 0.f, dc + 1 < N ? d[dc + 1] : 0.f);
       }
@@ -291,7 +296,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       for (int c = h; c < slabs; c += 2, ++slab_i) {
         // Symmetric outputs use one buffer for the tile and one for its transpose, the others two in turn.
         uint8_t* const stg = SYMMETRIC ? stg0 : stg0 + (slab_i & 1u) * 4096;
-        uint8_t* const stg_row = stg + lane * 128;
+        uint8_t* const stg_row = stg + lane * ROW;
         const float2 d_now = d_next;
         if (lane == 0) {
           if constexpr (SYMMETRIC) tma_store_wait_read<0>();
@@ -300,26 +305,26 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         __syncwarp();
         if constexpr (ADDS) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3);
-            *reinterpret_cast<uint4*>(stg + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = v[i];
+          for (int i = 0; i < UNITS; ++i) {
+            const int r = i * (32 / UNITS) + lane / UNITS;
+            *reinterpret_cast<uint4*>(stg + r * ROW + ((lane % UNITS ^ swizzle(r)) << 4)) = v[i];
           }
           __syncwarp();
           if (c + 2 < slabs) fetch(u, c + 2);
           else if (u + step < units) fetch(u + step, h);
           __syncwarp();
         }
-        const int col0 = tn * bn + c * 64;
+        const int col0 = tn * bn + c * SLAB;
         if constexpr (MODE == NS_GRAM_PARTS) {           // the sums themselves, 32 columns at a time, to the workspace
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < HALVES; ++half) {
             uint32_t a[32];
             __syncwarp();
-            tmem_ld_32x32(taddr + c * 64 + half * 32, a);
+            tmem_ld_32x32(taddr + c * SLAB + half * 32, a);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              st_shared_v4(smem_u32(stg_row) + half * 4096 + ((j ^ (lane & 7)) << 4), a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
+              st_shared_v4(smem_u32(stg0) + lane * 128 + half * 4096 + ((j ^ (lane & 7)) << 4), a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
           }
           if (c + 2 >= slabs) {
             tc_fence_before();
@@ -329,29 +334,29 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmC2, stg0, c * 64, u * NS_BM + rank * 128 + q * 32);
-            tma_store_2d(&tmC2, stg0 + 4096, c * 64 + 32, u * NS_BM + rank * 128 + q * 32);
+            for (int half = 0; half < HALVES; ++half)
+              tma_store_2d(&tmC2, stg0 + half * 4096, c * SLAB + half * 32, u * NS_BM + rank * 128 + q * 32);
             tma_store_commit();
           }
           continue;
         }
-        uint32_t o[32];
-        uint32_t o2[MODE == NS_POLY ? 32 : 1];           // a I + P
+        uint32_t o[16 * HALVES];
+        uint32_t o2[MODE == NS_POLY ? 16 * HALVES : 1];  // a I + P
         // the diagonal crosses few slabs: the others are spared the search for it
-        const bool on_diagonal = MODE == NS_POLY && col0 < row0 + 32 && row0 < col0 + 64;
+        const bool on_diagonal = MODE == NS_POLY && col0 < row0 + 32 && row0 < col0 + SLAB;
         float diagonal = 0.f;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < HALVES; ++half) {
           uint32_t a[32];
           float f[32];
           __syncwarp();                               // TMEM is read by whole warps: what lanes did on their own before ends here
-          tmem_ld_32x32(taddr + c * 64 + half * 32, a);
+          tmem_ld_32x32(taddr + c * SLAB + half * 32, a);
           tmem_ld_wait();
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int unit = half * 4 + j;
             uint4 e4 = make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (ADDS) e4 = *reinterpret_cast<const uint4*>(stg_row + ((unit ^ (lane & 7)) << 4));
+            if constexpr (ADDS) e4 = *reinterpret_cast<const uint4*>(stg_row + ((unit ^ swizzle(lane)) << 4));
             const uint32_t e[4] = {e4.x, e4.y, e4.z, e4.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -393,7 +398,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           for (int i = 0; i < 16; ++i)
             o[half * 16 + i] = ep.last ? pack_bf16x2(f[2 * i] * ep.unit, f[2 * i + 1] * ep.unit) : pack_f16x2(f[2 * i], f[2 * i + 1]);
         }
-        if (on_diagonal && row >= col0 && row < col0 + 64 && row < M)
+        if (on_diagonal && row >= col0 && row < col0 + SLAB && row < M)
           ep.diag[static_cast<size_t>(z) * ep.diag_len + row] = diagonal * ep.unit;
         if (c + 2 >= slabs) {
           // this warp's last read of the accumulator: hand it back before the stores go out
@@ -406,7 +411,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           __nv_bfloat16* dst = ep.out + (static_cast<size_t>(z) * M + row) * N + col0;
           if (row < M) {
 #pragma unroll
-            for (int j = 0; j < 64; ++j)
+            for (int j = 0; j < SLAB; ++j)
               if (col0 + j < N) dst[j] = __ushort_as_bfloat16(static_cast<unsigned short>(o[j >> 1] >> (j & 1 ? 16 : 0)));
           }
           continue;
@@ -414,12 +419,12 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const bool here = row0 < M && col0 < N;      // the tensor maps clip what crosses the edge
         auto put = [&](const uint32_t* v, const CUtensorMap* direct, const CUtensorMap* transposed) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            st_shared_v4(smem_u32(stg_row) + ((j ^ (lane & 7)) << 4), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          if (mirror) {                              // [64 columns][32 rows]
+          for (int j = 0; j < UNITS; ++j)
+            st_shared_v4(smem_u32(stg_row) + ((j ^ swizzle(lane)) << 4), v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          if (mirror) {                              // [columns][32 rows]
             uint16_t* t = reinterpret_cast<uint16_t*>(stg0 + 4096) + lane;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
+            for (int j = 0; j < 16 * HALVES; ++j) {
               t[(2 * j) * 32] = static_cast<uint16_t>(v[j]);
               t[(2 * j + 1) * 32] = static_cast<uint16_t>(v[j] >> 16);
             }
@@ -770,13 +775,16 @@ static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, c
   if (rc) return rc;
   // the output's rows in whole 16-byte units (the padding of the workspace takes zeros); a result with other rows is not stored by TMA
   tmC = tmA;
-  if (C.ld % 8 == 0 && (rc = ns_map(&tmC, C, C.ld, M, batch, pairs, 64, 32, 3))) return rc;
+  const bool narrow = bn == 64;
+  const uint32_t slab = narrow ? 32 : 64;
+  const int swizzle = narrow ? 2 : 3;
+  if (C.ld % 8 == 0 && (rc = ns_map(&tmC, C, C.ld, M, batch, pairs, slab, 32, swizzle))) return rc;
   tmM = tmC;
-  if (SYMMETRIC && (rc = ns_map(&tmM, C, C.ld, M, batch, pairs, 32, 64, 0))) return rc;
+  if (SYMMETRIC && (rc = ns_map(&tmM, C, C.ld, M, batch, pairs, 32, slab, 0))) return rc;
   tmC2 = tmC;
   tmM2 = tmM;
-  if (MODE == NS_POLY && C2.p && ((rc = ns_map(&tmC2, C2, C2.ld, M, batch, pairs, 64, 32, 3)) ||
-                                  (rc = ns_map(&tmM2, C2, C2.ld, M, batch, pairs, 32, 64, 0))))
+  if (MODE == NS_POLY && C2.p && ((rc = ns_map(&tmC2, C2, C2.ld, M, batch, pairs, slab, 32, swizzle)) ||
+                                  (rc = ns_map(&tmM2, C2, C2.ld, M, batch, pairs, 32, slab, 0))))
     return rc;
   const long units = (long)plan.parts * pairs * batch * w.per_matrix;
   if (units >= 1L << 22) return 7;
@@ -786,15 +794,17 @@ static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, c
     if ((rc = make_tmap(&tmC2, sums, 4, 2, dims, str, box, 3))) return rc;
   }
   constexpr int PARTS = MODE == NS_GRAM ? NS_GRAM_PARTS : MODE;
-  auto kern = plan.parts > 1 ? newton_schulz_kernel<A_MN, B_MN, PARTS> : newton_schulz_kernel<A_MN, B_MN, MODE>;
-  static bool configured[2][64] = {};
+  auto kern = plan.parts > 1 ? (narrow ? newton_schulz_kernel<A_MN, B_MN, PARTS, true> : newton_schulz_kernel<A_MN, B_MN, PARTS, false>)
+                             : (narrow ? newton_schulz_kernel<A_MN, B_MN, MODE, true> : newton_schulz_kernel<A_MN, B_MN, MODE, false>);
+  const int variant = (plan.parts > 1 ? 2 : 0) + (narrow ? 1 : 0);
+  static bool configured[4][64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 7;
-  if (!configured[plan.parts > 1][dev]) {
+  if (!configured[variant][dev]) {
     const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM);
     if (e != cudaSuccess) return 1000 + static_cast<int>(e);
-    configured[plan.parts > 1][dev] = true;
+    configured[variant][dev] = true;
   }
   const int grid = 2 * (int)(units < sms ? units : sms);
   KB_LAUNCH_PDL(kern, grid, NS_THREADS, NS_SMEM, stream, tmA, tmB, tmC, tmM, tmC2, tmM2, w, M, N, bn, ep, status);
