@@ -99,7 +99,14 @@ struct NsEpilogue {
   float also;                // NS_POLY: a I + P times this goes to a second matrix; 0: not wanted
   __nv_bfloat16* out;        // last update: the result, [batch][M][N]
   bool last;
+  // last update of an optimizer step: master <- keep * master - step * result, p = bf16(master), of rows of N elements; or null
+  float* master;
+  __nv_bfloat16* p;
+  float keep, step;
 };
+
+// One element of that.
+__device__ __forceinline__ float muon_weight(float master, float o, float keep, float step) { return fmaf(-step, o, master * keep); }
 
 // D[tmem] (+)= A * B in fp16: the instruction descriptor's formats are 0.
 __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn, bool b_mn) {
@@ -440,6 +447,31 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           }
         };
         put(o, &tmC, &tmM);
+        if constexpr (!SYMMETRIC) {
+          if (ep.master) {                           // eight columns a lane, from the slab that is being stored
+#pragma unroll 4
+            for (int i = 0; i < UNITS; ++i) {
+              const int r = i * (32 / UNITS) + lane / UNITS, u8 = lane % UNITS;
+              if (row0 + r >= M || col0 + u8 * 8 >= N) continue;
+              const uint4 x = *reinterpret_cast<const uint4*>(stg + r * ROW + ((u8 ^ swizzle(r)) << 4));
+              const size_t at = static_cast<size_t>(row0 + r) * N + col0 + u8 * 8;
+              float4* m = reinterpret_cast<float4*>(ep.master + at);
+              float4 a = m[0], b = m[1];
+              a.x = muon_weight(a.x, __uint_as_float(x.x << 16), ep.keep, ep.step);
+              a.y = muon_weight(a.y, __uint_as_float(x.x & 0xffff0000u), ep.keep, ep.step);
+              a.z = muon_weight(a.z, __uint_as_float(x.y << 16), ep.keep, ep.step);
+              a.w = muon_weight(a.w, __uint_as_float(x.y & 0xffff0000u), ep.keep, ep.step);
+              b.x = muon_weight(b.x, __uint_as_float(x.z << 16), ep.keep, ep.step);
+              b.y = muon_weight(b.y, __uint_as_float(x.z & 0xffff0000u), ep.keep, ep.step);
+              b.z = muon_weight(b.z, __uint_as_float(x.w << 16), ep.keep, ep.step);
+              b.w = muon_weight(b.w, __uint_as_float(x.w & 0xffff0000u), ep.keep, ep.step);
+              m[0] = a;
+              m[1] = b;
+              *reinterpret_cast<uint4*>(ep.p + at) = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+            }
+            __syncwarp();
+          }
+        }
         if constexpr (MODE == NS_POLY) {
           if (ep.also != 0.f) {
             if (lane == 0) tma_store_wait_read<0>();
@@ -632,29 +664,13 @@ ns_normalize_kernel(const NsSource src, int rows, int cols, int ldx, bool aligne
   }
 }
 
-// master <- master * keep - step * o;  p = bf16(master)
+// The same where rows of the result start anywhere, so that the product's epilogue cannot take it along.
 __global__ void __launch_bounds__(256)
-muon_apply_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ p, const __nv_bfloat16* __restrict__ o, long n, bool aligned,
-                  float keep, float step) {
+muon_apply_kernel(float* __restrict__ master, __nv_bfloat16* __restrict__ p, const __nv_bfloat16* __restrict__ o, long n, float keep,
+                  float step) {
   pdl_begin();
-  const long vecs = aligned ? n / 8 : 0;
-  for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < vecs; i += static_cast<long>(gridDim.x) * 256) {
-    const uint4 r = reinterpret_cast<const uint4*>(o)[i];
-    float4 a = reinterpret_cast<float4*>(master)[2 * i], b = reinterpret_cast<float4*>(master)[2 * i + 1];
-    a.x = fmaf(-step, __uint_as_float(r.x << 16), a.x * keep);
-    a.y = fmaf(-step, __uint_as_float(r.x & 0xffff0000u), a.y * keep);
-    a.z = fmaf(-step, __uint_as_float(r.y << 16), a.z * keep);
-    a.w = fmaf(-step, __uint_as_float(r.y & 0xffff0000u), a.w * keep);
-    b.x = fmaf(-step, __uint_as_float(r.z << 16), b.x * keep);
-    b.y = fmaf(-step, __uint_as_float(r.z & 0xffff0000u), b.y * keep);
-    b.z = fmaf(-step, __uint_as_float(r.w << 16), b.z * keep);
-    b.w = fmaf(-step, __uint_as_float(r.w & 0xffff0000u), b.w * keep);
-    reinterpret_cast<float4*>(master)[2 * i] = a;
-    reinterpret_cast<float4*>(master)[2 * i + 1] = b;
-    reinterpret_cast<uint4*>(p)[i] = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
-  }
-  for (long i = vecs * 8 + static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long>(gridDim.x) * 256) {
-    const float a = fmaf(-step, __bfloat162float(o[i]), master[i] * keep);
+  for (long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<long>(gridDim.x) * 256) {
+    const float a = muon_weight(master[i], __bfloat162float(o[i]), keep, step);
     master[i] = a;
     p[i] = __float2bfloat16(a);
   }
@@ -834,7 +850,14 @@ static int ns_segment(bool carries, int left) {
   return left % 2 == 1 && left > 1 ? 3 : left < 2 ? left : 2;
 }
 
-static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
+// What the last product of an optimizer step does beside its result.
+struct MuonApply {
+  float* master;
+  __nv_bfloat16* p;
+  float keep, step;
+};
+
+static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
                          float scale_q, void* out, uint8_t* work, int* status, cudaStream_t stream) {
   const NsLayout lay(batch, m, n);
   uint8_t* const x[2] = {work, work + lay.x};
@@ -915,6 +938,12 @@ static int newton_schulz(const NsSource& src, int batch, int m, int n, float a, 
     eu.diag_len = side;
     eu.out = static_cast<__nv_bfloat16*>(out);
     eu.last = last;
+    if (last) {
+      eu.master = apply.master;
+      eu.p = apply.p;
+      eu.keep = apply.keep;
+      eu.step = apply.step;
+    }
     if (len == 1) {
       if ((rc = poly(false))) return rc;
       eu.e = static_cast<const __half*>(xi.p);
@@ -957,7 +986,7 @@ static bool ns_sizes_ok(long batch, long m, long n) {
 extern "C" long kb_newton_schulz_bytes(long batch, long m, long n) {
   return kb::ns_sizes_ok(batch, m, n) ? kb::NsLayout((int)batch, (int)m, (int)n).total : -1;
 }
-// Kernels that a call of the functions below launches for a batch (the optimizer step: one more).
+// Kernels that a call of the functions below launches for a batch (the optimizer step: one more unless kb_muon_fuses).
 extern "C" int kb_newton_schulz_launches(int batch, int m, int n, int steps) {
   const int side = m < n ? m : n;
   const int gram = kb::ns_plan(kb::NS_GRAM, batch, side, side, m < n ? n : m).parts > 1 ? 2 : 1;
@@ -978,7 +1007,11 @@ extern "C" int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n
       reinterpret_cast<uintptr_t>(work) % 256)
     return 7;
   const kb::NsSource src{x, nullptr, nullptr, 0.f, bf16 != 0, false};
-  return kb::newton_schulz(src, batch, m, n, a, b, c, steps, eps, scale, scale_q, out, static_cast<uint8_t*>(work), status, stream);
+  return kb::newton_schulz(src, kb::MuonApply{}, batch, m, n, a, b, c, steps, eps, scale, scale_q, out, static_cast<uint8_t*>(work), status, stream);
+}
+// Whether the last product of the optimizer step also updates the weights (no kernel of their own): rows of whole 16-byte units.
+extern "C" int kb_muon_fuses(const void* master, const void* p, int n) {
+  return n % 8 == 0 && reinterpret_cast<uintptr_t>(master) % 16 == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
 }
 // One optimizer step of a [m, n] matrix: mom <- beta mom + gs g;  o = Newton-Schulz of (nesterov: gs g + beta mom) or mom;
 // master <- keep * master - step * o;  p = bf16(master).  gs: *grad_scale, 1 where that is null.
@@ -989,14 +1022,16 @@ extern "C" int kb_muon_step(const float* g, float* mom, float* master, void* p, 
       reinterpret_cast<uintptr_t>(work) % 256)
     return 7;
   const kb::NsSource src{g, mom, grad_scale, beta, false, nesterov != 0};
-  const int rc = kb::newton_schulz(src, 1, m, n, a, b, c, steps, eps, scale, scale_q, o, static_cast<uint8_t*>(work), status, stream);
-  if (rc) return rc;
+  const bool fused = kb_muon_fuses(master, p, n);
+  kb::MuonApply apply{};
+  if (fused) apply = kb::MuonApply{master, static_cast<__nv_bfloat16*>(p), keep, step};
+  const int rc = kb::newton_schulz(src, apply, 1, m, n, a, b, c, steps, eps, scale, scale_q, o, static_cast<uint8_t*>(work), status, stream);
+  if (rc || fused) return rc;
   const long count = (long)m * n;
-  const auto al = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % 16 == 0; };
-  long blocks = (count / 8 + 255) / 256;
-  blocks = blocks < 1 ? 1 : blocks > 148 * 8 ? 148 * 8 : blocks;
+  long blocks = (count + 1023) / 1024;
+  blocks = blocks > 148 * 8 ? 148 * 8 : blocks;
   KB_LAUNCH_PDL(kb::muon_apply_kernel, (unsigned)blocks, 256, 0, stream, master, static_cast<__nv_bfloat16*>(p),
-                static_cast<const __nv_bfloat16*>(o), count, al(master) && al(p), keep, step);
+                static_cast<const __nv_bfloat16*>(o), count, keep, step);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }

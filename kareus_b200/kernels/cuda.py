@@ -101,6 +101,7 @@ def _declare(L) -> None:
         "kb_gemm_fp8": [P, P, I, LNG, P, P, I, LNG, P, LNG, I, I, I, I, I, P, P],
         "kb_newton_schulz": [P, I, I, I, I, F, F, F, I, F, F, F, P, P, P, P],
         "kb_newton_schulz_launches": [I, I, I, I],
+        "kb_muon_fuses": [P, P, I],
         "kb_muon_step": [P, P, P, P, P, I, I, F, I, F, F, P, F, F, F, I, F, F, F, P, P, P],
         "kb_embedding_fwd": [P, P, P, LNG, I, LNG, LNG, F, P],
         "kb_embedding_bwd_sorted": [P, P, P, LNG, I, LNG, LNG, F, P, P],

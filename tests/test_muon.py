@@ -143,7 +143,7 @@ def muon_exact(p, g, m, master, lr, momentum, wd, scale, nesterov, gs):
 
 
 @pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
-@pytest.mark.parametrize("size", [(1, 3), (40, 56), (130, 67), (67, 131), (512, 384)])
+@pytest.mark.parametrize("size", [(1, 3), (40, 56), (130, 67), (67, 131), (512, 384), (300, 1000), (600, 136)])
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("clip", [None, 0.37])
 def test_muon_step(device, size, nesterov, clip):
@@ -163,6 +163,27 @@ def test_muon_step(device, size, nesterov, clip):
     want = kept - lr * scale * o.double()
     assert bool(((master.double() - want).abs() <= 6 * step * (kept.abs() + (lr * scale * o.double()).abs() + 1e-12)).all())
     assert torch.equal(p, master.bfloat16())
+
+
+@gpu
+@pytest.mark.parametrize("size", [(1300, 2600), (2600, 1304), (130, 9000)])
+def test_large_muon_step(size):
+    """Updates in the last product's epilogue, over several tiles and both forms of the iteration; weights that are views."""
+    g, m = matrices(2, *size, seed=12).unbind(0)
+    g, m = g.clone(), m.clone()
+    for offset in (0, 4, 3):                                       # 3: no 16-byte boundary, a kernel of its own
+        flat = torch.full((size[0] * size[1] + 8,), 5.0, device="cuda")
+        master = flat[offset:offset + size[0] * size[1]].view(size)
+        master.copy_(matrices(1, *size, seed=13, std=0.02)[0])
+        before = master.double()
+        p = torch.zeros(size, dtype=torch.bfloat16, device="cuda")
+        mm = m.clone()
+        o = K.muon_step(p, g, mm, master, 1e-2, 0.9, 0.1, 1.5)
+        check(o, g.double() + 0.9 * (0.9 * m.double() + g.double()))
+        want = before * (1 - 1e-3) - 1.5e-2 * o.double()
+        assert bool(((master.double() - want).abs() <= 6 * 2.0 ** -24 * (before.abs() + (1.5e-2 * o.double()).abs() + 1e-12)).all())
+        assert torch.equal(p, master.bfloat16())
+        assert bool((flat[:offset] == 5).all()) and bool((flat[offset + size[0] * size[1]:] == 5).all())
 
 
 @gpu
