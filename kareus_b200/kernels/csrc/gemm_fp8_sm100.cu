@@ -71,6 +71,13 @@ __device__ __forceinline__ void scales_to_tmem(uint32_t tmem, uint32_t saddr) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(tmem), "l"(d) : "memory");
 }
 
+// Tells the leader's MMA thread that this warp has read tensor memory.  Nothing else is handed over, and the order of accesses to
+// tensor memory is kept by the tcgen05 fences around the barrier: a release of the cluster's memory, which takes half a microsecond,
+// is not needed.
+__device__ __forceinline__ void mbar_arrive_tmem(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
 // NARROW: a bf16 output in tiles of 64 columns, whose epilogue takes slabs of 32 so that both sets of warps have one.
 template <bool OUT_F32, bool ACCUM, bool NARROW>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(G8_THREADS, 1)
@@ -223,6 +230,13 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     const int swizzle = NARROW ? (lane >> 1) & 3 : lane & 7;   // of the 16-byte units of this thread's row, as TMA expects
     const int slabs = bn / SLAB, mine = (slabs - h + 1) >> 1;
     const uint32_t stg_row = smem_u32(stg) + lane * (UNITS * 16);
+    // columns that this warp has read may be overwritten, if a tile comes that does
+    const auto hand_over = [&](uint64_t* bar, bool awaited) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0 && awaited) mbar_arrive_tmem(cluster_addr(bar, 0));
+      __syncwarp();                                   // TMEM is read by whole warps
+    };
     uint32_t tile_i = 0;
     for (int t = first; t < tiles; t += step, ++tile_i) {
       int tm, tn;
@@ -237,6 +251,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         // the slab with the columns that the other accumulator shares comes first: the last one of the first accumulator, the
         // first one of the second
         const int c = h + 2 * (buf == 0 ? mine - 1 - j : j);
+        const bool shared = shared_cols && c == (buf == 0 ? slabs - 1 : 0);
         uint32_t o[4 * UNITS];
         __syncwarp();
         if constexpr (NARROW) {
@@ -248,10 +263,18 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         } else if constexpr (OUT_F32) {
           tmem_ld_32x32(taddr + c * 32, o);
           tmem_ld_wait();
+          if (shared) hand_over(tshare, t + step < tiles);
         } else {
           uint32_t v0[32], v1[32];
-          tmem_ld_32x32(taddr + c * 64, v0);
-          tmem_ld_32x32(taddr + c * 64 + 32, v1);
+          // the 32 columns that both accumulators share come first
+          if (shared && buf == 0) tmem_ld_32x32(taddr + c * 64 + 32, v1);
+          else tmem_ld_32x32(taddr + c * 64, v0);
+          if (shared) {
+            tmem_ld_wait();
+            hand_over(tshare, t + step < tiles);
+          }
+          if (shared && buf == 0) tmem_ld_32x32(taddr + c * 64, v0);
+          else tmem_ld_32x32(taddr + c * 64 + 32, v1);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
@@ -259,13 +282,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
             o[16 + i] = pack_bf16x2(__uint_as_float(v1[2 * i]), __uint_as_float(v1[2 * i + 1]));
           }
         }
-        const bool shared = shared_cols && c == (buf == 0 ? slabs - 1 : 0), last = j == mine - 1;
-        if (shared || last) {                         // hand over what the next tiles wait for (half a microsecond each)
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0 && shared && t + step < tiles) mbar_arrive_cluster(cluster_addr(tshare, 0));
-          if (lane == 0 && last && t + 2 * step < tiles) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
-        }
+        if (j == mine - 1) hand_over(&tempty[buf], t + 2 * step < tiles);
         if (lane == 0) tma_store_wait_read<0>();      // the previous slab has left the staging buffer
         __syncwarp();
 #pragma unroll
@@ -293,11 +310,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           tma_store_commit();
         }
       }
-      if (mine == 0) {                                // no slab for this warp (narrow tile): release all the same
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0 && t + 2 * step < tiles) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
-      }
+      if (mine == 0) hand_over(&tempty[buf], t + 2 * step < tiles);     // no slab for this warp (narrow tile)
     }
     if (lane == 0) tma_store_wait_read<0>();          // nothing in flight out of shared memory at exit
   }
