@@ -6,9 +6,10 @@
 //
 // Types.  The products run on the tensor cores in fp16 with fp32 sums: their operands are bounded by the singular values, so fp16
 // with a common power of two (`scale`, chosen by the host so that the largest possible entry fits) has 11 bits for everything that
-// counts where bf16 has 8; five steps are then 1e-3 off in the 2-norm instead of 1e-2.  The largest single rounding error would be
-// that of P's diagonal (about -2.6 beside entries near 0), so the diagonal stays in fp32, outside P: X <- (a + diag P) X + (P - diag
-// P) X.  Norms are summed in fp32 per thread and fp64 beyond, in a fixed order.
+// counts where bf16 has 8; five steps are then 1e-3 off in the 2-norm instead of 1e-2.  The largest rounding errors would be those of
+// the square matrices' diagonals (about 1 and -2.6 beside entries near 0, and much the same in every row), so diagonals are also kept
+// in fp32: P's apart from P (X <- (a + diag P) X + (P - diag P) X), the others beside the matrix, where they put right what its
+// rounded diagonal does to the result's.  Norms are summed in fp32 per thread and fp64 beyond, in a fixed order.
 //
 // Long matrices.  X_{k+1} = Q_k X_k with Q_k = a I + P_k, and G_{k+1} = Q_k G_k Q_k, where everything but X is as small as the shorter
 // side.  Where the longer side is at least 1.5 times the shorter one and it saves time (ns_carries), G is carried from step to step so (T = Q G, G' = Q T), the Q are
@@ -47,14 +48,13 @@ static_assert(NS_SMEM <= 227 * 1024, "shared memory per CTA");
 enum NsMode : int {
   NS_GRAM = 0,       // G = X Xt
   NS_POLY = 1,       // P = b G + c G G; diagonal d apart
-  NS_UPDATE = 2,     // X <- (a + d) X + P X
-  NS_UPDATE_T = 3,   // X <- X (a + d) + X P
+  NS_UPDATE = 2,     // X <- (a + d) X + P X, or Q X
+  NS_UPDATE_T = 3,   // X <- X (a + d) + X P, or X Q
   NS_CARRY = 4,      // Y <- (a + d) Y + P Y for symmetric Y that P commutes with
-  NS_APPLY = 5,      // X <- Q X or X Q
-  NS_GRAM_PARTS = 6, // parts of X Xt along K, as fp32 sums
+  NS_GRAM_PARTS = 5, // parts of X Xt along K, as fp32 sums
 };
-__host__ __device__ constexpr bool ns_symmetric(int mode) { return mode != NS_UPDATE && mode != NS_UPDATE_T && mode != NS_APPLY; }
-__host__ __device__ constexpr bool ns_adds(int mode) { return mode != NS_GRAM && mode != NS_GRAM_PARTS && mode != NS_APPLY; }
+__host__ __device__ constexpr bool ns_symmetric(int mode) { return mode != NS_UPDATE && mode != NS_UPDATE_T; }
+__host__ __device__ constexpr bool ns_adds(int mode) { return mode != NS_GRAM && mode != NS_GRAM_PARTS; }
 
 struct NsWork {
   int batch, pairs, tiles_m, tiles_n, per_matrix, nk;      // pairs: matrices per item of the batch (NS_CARRY takes G and Q at once)
@@ -92,11 +92,20 @@ struct NsEpilogue {
   long e_batch, e_pair;
   int lde, e_cols;           // e_cols: columns to read, a multiple of 8
   float alpha, coef;         // accumulator's factor, e's factor
-  float* diag;               // [batch][diag_len]: diagonal of P, written by NS_POLY, read by the updates
-  int diag_len;
-  float unit;                // 1 / scale
-  float coef2;               // a * scale
-  float also;                // NS_POLY: a I + P times this goes to a second matrix; 0: not wanted
+  // Diagonals, [batch][len] each.  `diag`: P's, written by NS_POLY, added to the factor of the row (column) by the updates and
+  // NS_CARRY.  e_diag: of the matrix that is added, c_diag: of the result (NS_GRAM, NS_CARRY); from one of a pair to the other diag_pair
+  // elements.
+  float* diag;
+  const float* e_diag;
+  float* c_diag;
+  long e_diag_pair, c_diag_pair;
+  int len;
+  float scale[2];            // of the matrix that is added and of the result, for the first and the second of a pair
+  float rounded;             // updates by Q: its scale; the factor is what rounding took from the diagonal.  0: updates by P
+  float b, c;                // NS_POLY
+  float unit;                // 1 / scale of the result
+  float also;                // NS_POLY: (a I + P) times this goes to a second matrix, its diagonal to c_diag; 0: not wanted
+  float a;
   __nv_bfloat16* out;        // last update: the result, [batch][M][N]
   bool last;
   // last update of an optimizer step: master <- keep * master - step * result, p = bf16(master), of rows of N elements; or null
@@ -107,6 +116,9 @@ struct NsEpilogue {
 
 // One element of that.
 __device__ __forceinline__ float muon_weight(float master, float o, float keep, float step) { return fmaf(-step, o, master * keep); }
+
+// What fp16 leaves of v at this scale (a power of two).
+__device__ __forceinline__ float rounded16(float v, float scale) { return __half2float(__float2half_rn(v * scale)) / scale; }
 
 // D[tmem] (+)= A * B in fp16: the instruction descriptor's formats are 0.
 __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, bool a_mn, bool b_mn) {
@@ -278,8 +290,9 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       }
       if constexpr (MODE == NS_UPDATE_T) {
         const int dc = tn * bn + c * SLAB + 2 * lane;
-        const float* d = ep.diag + static_cast<size_t>(z) * ep.diag_len;
+        const float* d = ep.diag + static_cast<size_t>(z) * ep.len;
         d_next = make_float2(dc < N ? d[dc] : 0.f, dc + 1 < N ? d[dc + 1] : 0.f);
+        if (ep.rounded != 0.f) d_next = make_float2(d_next.x - rounded16(d_next.x, ep.rounded), d_next.y - rounded16(d_next.y, ep.rounded));
       }
     };
     if (ADDS && first < units && h < slabs) fetch(first, h);
@@ -290,8 +303,21 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
       const uint32_t buf = tile_i & 1u;
       const int row0 = tm * NS_BM + rank * 128 + q * 32, row = row0 + lane;
       float coef = ep.coef;
-      if constexpr (MODE == NS_UPDATE || MODE == NS_CARRY) {
-        if (row < M) coef += ep.diag[static_cast<size_t>(z) * ep.diag_len + row];
+      float correction = 0.f;                 // of this row's diagonal element, for what rounding took from those that it is made of
+      {
+        const size_t at = static_cast<size_t>(z) * ep.len + row;
+        if constexpr (MODE == NS_UPDATE || MODE == NS_CARRY) {
+          if (row < M) {
+            const float d = ep.diag[at];
+            coef += MODE == NS_UPDATE && ep.rounded != 0.f ? d - rounded16(d, ep.rounded) : d;
+          }
+        }
+        if constexpr (MODE == NS_CARRY || MODE == NS_POLY) {
+          if (row < M) {
+            const float scale = ep.scale[pair], v = ep.e_diag[pair * ep.e_diag_pair + at], lost = v - rounded16(v, scale);
+            correction = MODE == NS_CARRY ? coef * lost * scale : (ep.b * lost + ep.c * lost * (2.f * v - lost)) * scale;
+          }
+        }
       }
       __syncwarp();
       if (!mbar_wait_warp(&tfull[buf], (tile_i >> 1) & 1u, abort_flag, status, ST_TIMEOUT_TMEM_FULL)) break;
@@ -350,7 +376,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         uint32_t o[16 * HALVES];
         uint32_t o2[MODE == NS_POLY ? 16 * HALVES : 1];  // a I + P
         // the diagonal crosses few slabs: the others are spared the search for it
-        const bool on_diagonal = MODE == NS_POLY && col0 < row0 + 32 && row0 < col0 + SLAB;
+        const bool on_diagonal = SYMMETRIC && col0 < row0 + 32 && row0 < col0 + SLAB;
         float diagonal = 0.f;
 #pragma unroll
         for (int half = 0; half < HALVES; ++half) {
@@ -388,16 +414,23 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 #pragma unroll
               for (int i = 0; i < 16; ++i) o2[half * 16 + i] = pack_f16x2(f[2 * i] * ep.also, f[2 * i + 1] * ep.also);
             }
-            if (on_diagonal) {
-              const int at = row - col0 - half * 32;      // this row's diagonal element, if it is here
+          }
+          if (on_diagonal) {
+            const int at = row - col0 - half * 32;        // this row's diagonal element, if it is here
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const bool d0 = at == 2 * i, d1 = at == 2 * i + 1;
-                diagonal = d0 ? f[2 * i] : d1 ? f[2 * i + 1] : diagonal;
-                if (ep.also != 0.f)
-                  o2[half * 16 + i] = pack_f16x2((f[2 * i] + (d0 ? ep.coef2 : 0.f)) * ep.also, (f[2 * i + 1] + (d1 ? ep.coef2 : 0.f)) * ep.also);
+            for (int i = 0; i < 16; ++i) {
+              const bool d0 = at == 2 * i, d1 = at == 2 * i + 1;
+              diagonal = d0 ? f[2 * i] + correction : d1 ? f[2 * i + 1] + correction : diagonal;
+              if constexpr (MODE == NS_POLY) {
+                if (ep.also != 0.f && (d0 || d1)) {
+                  const float whole = (diagonal * ep.unit + ep.a) * (ep.also / ep.unit);
+                  o2[half * 16 + i] = d0 ? pack_f16x2(whole, f[2 * i + 1] * ep.also) : pack_f16x2(f[2 * i] * ep.also, whole);
+                }
                 f[2 * i] = d0 ? 0.f : f[2 * i];
                 f[2 * i + 1] = d1 ? 0.f : f[2 * i + 1];
+              } else {
+                f[2 * i] = d0 ? diagonal : f[2 * i];
+                f[2 * i + 1] = d1 ? diagonal : f[2 * i + 1];
               }
             }
           }
@@ -405,8 +438,15 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
           for (int i = 0; i < 16; ++i)
             o[half * 16 + i] = ep.last ? pack_bf16x2(f[2 * i] * ep.unit, f[2 * i + 1] * ep.unit) : pack_f16x2(f[2 * i], f[2 * i + 1]);
         }
-        if (on_diagonal && row >= col0 && row < col0 + SLAB && row < M)
-          ep.diag[static_cast<size_t>(z) * ep.diag_len + row] = diagonal * ep.unit;
+        if (on_diagonal && row >= col0 && row < col0 + SLAB && row < M) {
+          const size_t at = static_cast<size_t>(z) * ep.len + row;
+          if constexpr (MODE == NS_POLY) {
+            ep.diag[at] = diagonal * ep.unit;
+            if (ep.also != 0.f) ep.c_diag[at] = diagonal * ep.unit + ep.a;
+          } else {
+            ep.c_diag[pair * ep.c_diag_pair + at] = diagonal / ep.scale[pair];
+          }
+        }
         if (c + 2 >= slabs) {
           // this warp's last read of the accumulator: hand it back before the stores go out
           tc_fence_before();
@@ -500,7 +540,8 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
 
 // G from the sums of its parts along K, added in order: 32 x 32 elements a block, as they are and transposed.
 __global__ void __launch_bounds__(256)
-ns_sum_parts_kernel(const float* __restrict__ work, __half* __restrict__ G, long ldg, int side, int bn, const NsWork w, float alpha) {
+ns_sum_parts_kernel(const float* __restrict__ work, __half* __restrict__ G, long ldg, int side, int bn, const NsWork w, float alpha,
+                    float* __restrict__ diag) {
   __shared__ float t[32][33];
   pdl_begin();
   const int per_tile = 8 * (bn / 32), tile = blockIdx.x / per_tile, sub = blockIdx.x - tile * per_tile;
@@ -519,6 +560,9 @@ ns_sum_parts_kernel(const float* __restrict__ work, __half* __restrict__ G, long
     s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
   }
   s.x *= alpha; s.y *= alpha; s.z *= alpha; s.w *= alpha;
+  const int on = row0 + r - col0 - c;                   // which of the four columns the row's diagonal element is in
+  if (on >= 0 && on < 4 && row0 + r < side)
+    diag[static_cast<size_t>(z) * side + row0 + r] = (on == 0 ? s.x : on == 1 ? s.y : on == 2 ? s.z : s.w) * alpha;
   __half* g = G + static_cast<size_t>(z) * side * ldg;
   // rows hold whole groups of eight columns; what lies behind the last column is zero
   if (row0 + r < side && col0 + c < ldg)
@@ -735,7 +779,7 @@ struct NsLayout {
     ldg = (side + 7L) / 8 * 8;
     x = up(2L * batch * m * ldx);
     g = up(2L * batch * side * ldg);
-    diag = up(4L * batch * side);
+    diag = up(4L * NS_SLOTS * batch * side);
     part = up(8L * batch * NS_SUM_BLOCKS);
     const NsPlan p = ns_plan(NS_GRAM, batch, side, side, m < n ? n : m);
     sums = p.parts > 1 ? up(4L * p.parts * batch * p.per_matrix * NS_BM * p.bn) : 0;
@@ -826,7 +870,7 @@ static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, c
   KB_LAUNCH_PDL(kern, grid, NS_THREADS, NS_SMEM, stream, tmA, tmB, tmC, tmM, tmC2, tmM2, w, M, N, bn, ep, status);
   if (MODE == NS_GRAM && plan.parts > 1)
     KB_LAUNCH_PDL(ns_sum_parts_kernel, (unsigned)(batch * w.per_matrix * 8 * (bn / 32)), 256, 0, stream, (const float*)sums,
-                  static_cast<__half*>(C.p), C.ld, M, bn, w, ep.alpha);
+                  static_cast<__half*>(C.p), C.ld, M, bn, w, ep.alpha, ep.c_diag);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }
@@ -840,7 +884,7 @@ static bool ns_carries(int batch, int m, int n, int steps) {
   if (steps < 2 || 2L * other < 3L * side) return false;
   const bool tall = m > n;
   const double gram = ns_plan(NS_GRAM, batch, side, side, other).clocks, square = ns_plan(NS_CARRY, batch, side, side, side).clocks;
-  const double x = ns_plan(NS_APPLY, batch, tall ? other : side, tall ? side : other, side).clocks;
+  const double x = ns_plan(NS_UPDATE, batch, tall ? other : side, tall ? side : other, side).clocks;
   const int segments = steps / 2, products = 3 * steps - segments + steps % 2;    // of G's size: P, T, G' and products of Q
   return segments * (gram + x) + products * square < steps * (gram + square + x);
 }
@@ -894,8 +938,12 @@ static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch,
     const int len = ns_segment(carries, steps - done);
     const bool last = done + len == steps;
     const NsMatrix xi{x[cur], lay.ldx, 0}, xo{last ? out : x[cur ^ 1], last ? (long)n : lay.ldx, 0};
+    const auto diagonal = [&](int slot_i) { return diag + static_cast<long>(slot_i) * batch * side; };
     NsEpilogue eg{};
     eg.alpha = eg.unit = unit;
+    eg.c_diag = diagonal(NS_G);
+    eg.len = side;
+    eg.scale[0] = scale;
     rc = tall ? ns_product<true, true, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, m, eg, sums, status, stream)
               : ns_product<false, false, NS_GRAM>(xi, xi, slot(NS_G), none, batch, 1, side, side, n, eg, sums, status, stream);
     if (rc) return rc;
@@ -907,15 +955,20 @@ static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch,
       e.lde = e.e_cols = (int)ldg;
       e.alpha = c * unit;
       e.coef = b;
-      e.diag = diag;
-      e.diag_len = side;
+      e.diag = diagonal(NS_P);
+      e.e_diag = diagonal(NS_G);
+      e.c_diag = diagonal(NS_Q);
+      e.len = side;
+      e.scale[0] = scale;
+      e.a = a;
+      e.b = b;
+      e.c = c;
       e.unit = unit;
-      e.coef2 = a * scale;
       e.also = q ? scale_q * unit : 0.f;
       return ns_product<false, false, NS_POLY>(slot(NS_G), slot(NS_G), slot(NS_P), q ? slot(NS_Q) : none, batch, 1, side, side, side, e, sums,
                                                status, stream);
     };
-    // slot `to` = (a I + P) slot `from`, with a second pair of slots where `from2` says so
+    // slot `to` = (a I + P) slot `from`, with a second pair of slots (products of Q) where `from2` says so
     const auto carry = [&](int from, int to, int from2, int to2) {
       NsEpilogue e{};
       const int pairs = from2 ? 2 : 1;
@@ -928,14 +981,23 @@ static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch,
       e.lde = e.e_cols = (int)ldg;
       e.alpha = unit;
       e.coef = a;
-      e.diag = diag;
-      e.diag_len = side;
+      e.diag = diagonal(NS_P);
+      e.e_diag = diagonal(from);
+      e.c_diag = diagonal(to);
+      e.e_diag_pair = static_cast<long>(from2 - from) * batch * side;
+      e.c_diag_pair = static_cast<long>(to2 - to) * batch * side;
+      e.len = side;
+      e.scale[0] = from >= NS_Q ? scale_q : scale;
+      e.scale[1] = scale_q;
       e.unit = unit;
       return ns_product<false, false, NS_CARRY>(slot(NS_P), y, z, none, batch, pairs, side, side, side, e, sums, status, stream);
     };
     NsEpilogue eu{};
-    eu.diag = diag;
-    eu.diag_len = side;
+    eu.len = side;
+    eu.e = static_cast<const __half*>(xi.p);
+    eu.e_batch = m * lay.ldx;
+    eu.lde = eu.e_cols = (int)lay.ldx;
+    eu.unit = unit;
     eu.out = static_cast<__nv_bfloat16*>(out);
     eu.last = last;
     if (last) {
@@ -944,17 +1006,14 @@ static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch,
       eu.keep = apply.keep;
       eu.step = apply.step;
     }
+    int q = NS_P;                              // the matrix that X is multiplied by
     if (len == 1) {
       if ((rc = poly(false))) return rc;
-      eu.e = static_cast<const __half*>(xi.p);
-      eu.e_batch = m * lay.ldx;
-      eu.lde = eu.e_cols = (int)lay.ldx;
-      eu.alpha = eu.unit = unit;
+      eu.alpha = unit;
       eu.coef = a;
-      rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, slot(NS_P), xo, none, batch, 1, m, n, side, eu, sums, status, stream)
-                : ns_product<false, true, NS_UPDATE>(slot(NS_P), xi, xo, none, batch, 1, m, n, side, eu, sums, status, stream);
     } else {
-      int q = NS_Q, spare = NS_Q + 1;
+      q = NS_Q;
+      int spare = NS_Q + 1;
       if ((rc = poly(true)) || (rc = carry(NS_G, NS_T, 0, 0)) || (rc = carry(NS_T, NS_G, 0, 0))) return rc;
       for (int k = 1; k < len; ++k) {
         if ((rc = poly(false))) return rc;
@@ -965,10 +1024,12 @@ static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch,
         spare = t;
       }
       eu.alpha = unit_q;
-      eu.unit = unit;
-      rc = tall ? ns_product<false, false, NS_APPLY>(xi, slot(q), xo, none, batch, 1, m, n, side, eu, sums, status, stream)
-                : ns_product<false, true, NS_APPLY>(slot(q), xi, xo, none, batch, 1, m, n, side, eu, sums, status, stream);
+      eu.coef = 0.f;
+      eu.rounded = scale_q;
     }
+    eu.diag = diagonal(q);
+    rc = tall ? ns_product<false, false, NS_UPDATE_T>(xi, slot(q), xo, none, batch, 1, m, n, side, eu, sums, status, stream)
+              : ns_product<false, true, NS_UPDATE>(slot(q), xi, xo, none, batch, 1, m, n, side, eu, sums, status, stream);
     if (rc) return rc;
     done += len;
     cur ^= 1;
