@@ -6,7 +6,7 @@
 // and tokens that make up much of a batch (padding, a frequent word) queue up for the same addresses.  Here the tokens are sorted
 // first and each row of the table gets one addition of a sum that was formed in registers:
 //
-//   1. Stable radix sort of (id, t) by one cluster of eight blocks.  Items stay in the blocks' shared memory; a pass ranks the items
+//   1. Stable radix sort of (id, t) by one cluster of eight blocks, small batches by one block.  Items stay in the blocks' shared memory; a pass ranks the items
 //      of a warp by ballots over the digit's bits, adds up the counts of warps, blocks and digits, and writes every item to its
 //      place in the shared memory of the block that owns it.  Tokens of other shards are left out.
 //   2. Blocks take windows of `window` sorted positions and 1024 columns, sum the rows of each token in order and add the sum to the
@@ -69,6 +69,7 @@ embedding_fwd_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __res
 
 // ----------------------------------------------------------------------------- sort
 constexpr int ES_BLOCKS = 8;                   // of a cluster
+constexpr int ES_ALONE = 2048;                 // batches that one block sorts: 512 tokens in 7.4 us, in 8.5 by a cluster
 constexpr int ES_THREADS = 1024;
 constexpr int ES_WARPS = ES_THREADS / 32;
 constexpr int ES_PER_BLOCK = 8192;             // items
@@ -89,21 +90,25 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t local, uint32_t rank) {
   return v;
 }
 
-// ids / order [n]: keys below `rows` in ascending order and where they stood; ids behind them are `rows`.  `per`: items of a block (a
-// multiple of 32, at most ES_PER_BLOCK, ES_BLOCKS * per >= n); `passes` digits of `bits` (at most ES_BITS) bits hold every key.
-// Tokens of other shards leave in the first pass.
-__global__ void __cluster_dims__(ES_BLOCKS, 1, 1) __launch_bounds__(ES_THREADS, 1)
-embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
-                      uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
+// ids / order [n]: keys below `rows` in ascending order and where they stood; ids behind them are `rows`.  `per`: items of each of
+// BLOCKS blocks (a multiple of 32, at most ES_PER_BLOCK, BLOCKS * per >= n); `passes` digits of `bits` (at most ES_BITS) bits hold
+// every key.  Tokens of other shards leave in the first pass.
+template <int BLOCKS>
+__device__ __forceinline__ void sort_tokens(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
+                                            uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
   extern __shared__ uint4 sm[];
   __shared__ uint32_t count[ES_BINS], base[ES_BINS], warp_sum[ES_BINS / 32];
   uint32_t* const hist = reinterpret_cast<uint32_t*>(sm);              // [warps][bins] of 16 bits
   constexpr int HIST_WORDS = ES_BINS / 2;
   uint2 *src = reinterpret_cast<uint2*>(hist + ES_WARPS * HIST_WORDS), *dst = src + per;      // (key, position)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = blockIdx.x;
+  const uint32_t rank = BLOCKS > 1 ? blockIdx.x : 0;
   const int bins = 1 << bits;
   const int all = n;
+  const auto sync = [] {
+    if (BLOCKS > 1) cluster_sync_all();
+    else __syncthreads();
+  };
   int begin = static_cast<int>(rank) * per, here = max(0, min(per, n - begin));
   pdl_begin();
   for (int i = tid; i < here; i += ES_THREADS) {
@@ -153,12 +158,12 @@ embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long firs
       count[2 * tid] = sum & 0xffffu;
       count[2 * tid + 1] = sum >> 16;
     }
-    cluster_sync_all();
+    sync();
     uint32_t total = 0, before = 0;                       // of this digit in the cluster, in the blocks before
     if (tid < bins) {
 #pragma unroll
-      for (int b = 0; b < ES_BLOCKS; ++b) {
-        const uint32_t c = ld_cluster(smem_u32(&count[tid]), b);
+      for (int b = 0; b < BLOCKS; ++b) {
+        const uint32_t c = BLOCKS > 1 ? ld_cluster(smem_u32(&count[tid]), b) : count[tid];
         if (b < static_cast<int>(rank)) before += c;
         total += c;
       }
@@ -183,7 +188,7 @@ embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long firs
 #pragma unroll
       for (int w = 0; w < ES_BINS / 32; ++w) n += static_cast<int>(warp_sum[w]);
     }
-    const int next_per = max(32, (n + ES_BLOCKS - 1) / ES_BLOCKS);
+    const int next_per = max(32, (n + BLOCKS - 1) / BLOCKS);
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < ES_STEPS; ++s) {
@@ -193,11 +198,12 @@ embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long firs
         if (item.x < rows) {
           const uint32_t d = (item.x >> shift) & (bins - 1);
           const uint32_t at = base[d] + mine[d] + where[s], block = at / static_cast<uint32_t>(next_per);
-          st_cluster(smem_u32(dst + (at - block * next_per)), block, item);
+          if (BLOCKS > 1) st_cluster(smem_u32(dst + (at - block * next_per)), block, item);
+          else dst[at] = item;
         }
       }
     }
-    cluster_sync_all();
+    sync();
     per = next_per;
     begin = static_cast<int>(rank) * per;
     here = max(0, min(per, n - begin));
@@ -209,8 +215,19 @@ embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long firs
     ids[begin + i] = src[i].x;
     order[begin + i] = src[i].y;
   }
-  for (int i = n + static_cast<int>(rank) * ES_THREADS + tid; i < all; i += ES_BLOCKS * ES_THREADS) ids[i] = static_cast<uint32_t>(rows);
+  for (int i = n + static_cast<int>(rank) * ES_THREADS + tid; i < all; i += BLOCKS * ES_THREADS) ids[i] = static_cast<uint32_t>(rows);
 }
+__global__ void __cluster_dims__(ES_BLOCKS, 1, 1) __launch_bounds__(ES_THREADS, 1)
+embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
+                      uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
+  sort_tokens<ES_BLOCKS>(tokens, n, per, first, rows, passes, bits, ids, order);
+}
+__global__ void __launch_bounds__(ES_THREADS, 1)
+embedding_sort_small_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
+                            uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
+  sort_tokens<1>(tokens, n, per, first, rows, passes, bits, ids, order);
+}
+
 
 // ----------------------------------------------------------------------------- sums
 constexpr int EW_THREADS = 128;
@@ -467,14 +484,18 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 7;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               ES_WARPS * ES_BINS * 2 + 2 * ES_PER_BLOCK * 8);
+    cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         ES_WARPS * ES_BINS * 2 + 2 * ES_PER_BLOCK * 8);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(embedding_sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               ES_WARPS * ES_BINS * 2 + 2 * ES_ALONE * 8);
     if (e != cudaSuccess) return 1000 + static_cast<int>(e);
     configured[dev] = true;
   }
   for (long at = 0; at < ntok; at += ES_MOST) {
     const int n = static_cast<int>(ntok - at < ES_MOST ? ntok - at : ES_MOST);
-    const int per = ((n + ES_BLOCKS - 1) / ES_BLOCKS + 31) / 32 * 32;
+    const bool alone = n <= ES_ALONE;
+    const int blocks = alone ? 1 : ES_BLOCKS, per = ((n + blocks - 1) / blocks + 31) / 32 * 32;
     const long list = (4L * n + 255) / 256 * 256;
     EmbeddingSum s;
     uint8_t* base = static_cast<uint8_t*>(work);
@@ -492,7 +513,8 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
     s.H = H;
     s.rows = static_cast<uint32_t>(rows);
     s.scale = scale;
-    KB_LAUNCH_PDL(embedding_sort_kernel, ES_BLOCKS, ES_THREADS, ES_WARPS * ES_BINS * 2 + 2 * per * 8, stream, tokens + at, n, per, first, rows,
+    const auto sort = alone ? embedding_sort_small_kernel : embedding_sort_kernel;
+    KB_LAUNCH_PDL(sort, blocks, ES_THREADS, ES_WARPS * ES_BINS * 2 + 2 * per * 8, stream, tokens + at, n, per, first, rows,
                   passes, bits, ids, order);
     KB_LAUNCH_PDL((vec ? embedding_window_kernel<true> : embedding_window_kernel<false>), dim3(windows, (H + EW_COLS - 1) / EW_COLS),
                   EW_THREADS, 0, stream, s);
