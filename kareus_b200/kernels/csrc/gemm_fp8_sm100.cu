@@ -14,6 +14,11 @@
 // Tensor memory: two accumulators of 256 columns and the scales do not fit into 512.  The second accumulator starts at column
 // 224, so that at BN = 256 the two share 32 columns: the epilogue reads those first, and the main loop of the next tile starts as
 // soon as they are read.
+//
+// What bounds it: at 256 columns the tensor pipe (93 to 96 % of its cycles in long sums) and with it the power limit, 1.35 GHz; 32 KB
+// reach an SM per 512 clocks, the 64 bytes a clock that it can take, so narrower tiles wait for loads.  Short sums lose a tenth at
+// tile borders, between the last product of a tile and the first of the next.  One B200: 8192 x 28672 x 4096 632 us (3.04 PFLOP/s),
+// 8192 x 4096 x 28672 623, fp32 += 28672 x 4096 x 8192 674; 17 x 6144 x 4096 11; 328 x 776 x 1032 7, launch and first loads.
 #include "sm100.cuh"
 #include "launch.h"
 #include "native_ops.h"

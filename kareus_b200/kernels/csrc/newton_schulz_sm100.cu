@@ -25,6 +25,11 @@
 //   warp 0      TMA producer of this CTA's halves
 //   warp 1      MMA issuer (leader CTA only); allocates TMEM in both CTAs
 //   warps 2..9  epilogue: accumulator and the tile of G or X that is added to it, which is fetched while the main loop runs
+//
+// What bounds it: for large matrices the tensor pipe and the power limit (326 us for X = Q X at 4096 x 14336, 1.48 PFLOP/s; products of
+// 4096 x 4096 60 us, 1.8 waves of tiles on 74 pairs of SMs), for small ones the chain of launches: 7 us each, of which 1.4 are the
+// first load, 1.2 the epilogue and 2.7 the end of one kernel and the start of the next.  One B200, five steps: 2048 x 512 123 us;
+// optimizer step 6144 x 4096 1.65 ms, 4096 x 14336 2.48.
 #include <cuda_fp16.h>
 #include "sm100.cuh"
 #include "launch.h"
