@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(FQ_THREADS, 4) fp8_quantize_kernel(const Fp8Qu
 // ldq and ldqt are multiples of 16, at least cols / rows; what lies between the two is nobody's.  fmt: 0 e4m3, 1 e5m2.
 extern "C" int kb_fp8_quantize(const void* x, long rows, long cols, long ld, void* q, long ldq, void* s, void* qt, long ldqt,
                                void* st, int square, int fmt, cudaStream_t stream) {
-  if (rows <= 0 || cols <= 0 || rows >= 1L << 31 || cols >= 1L << 31 || ld < cols || (!q && !qt) || (fmt & ~1)) return 7;
+  constexpr long MOST = (1L << 31) - 512;       // row and column numbers are ints, those of tiles across the edge too
+  if (rows <= 0 || cols <= 0 || rows > MOST || cols > MOST || ld < cols || (!q && !qt) || (fmt & ~1)) return 7;
   if (q && (!s || ldq < cols || ldq % 16 || reinterpret_cast<uintptr_t>(q) % 16)) return 7;
   if (qt && (!st || ldqt < rows || ldqt % 16 || reinterpret_cast<uintptr_t>(qt) % 16)) return 7;
   kb::Fp8Quantize p;

@@ -368,7 +368,8 @@ extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, c
                            void* C, long ldc, int M, int N, int K, int out_f32, int accumulate, int* status, cudaStream_t stream) {
   using namespace kb;
   const auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; };
-  if (M <= 0 || N <= 0 || K <= 0 || lda < K || ldb < K || lda % 16 || ldb % 16 || ldc < N ||
+  constexpr int MOST = 0x7fffffff - 511;       // row and column numbers are ints, those of tiles across the edge too
+  if (M <= 0 || N <= 0 || K <= 0 || M > MOST || N > MOST || K > MOST || lda < K || ldb < K || lda % 16 || ldb % 16 || ldc < N ||
       !aligned(A) || !aligned(B) || !aligned(SA) || !aligned(SB) || (fmt_a & ~1) || (fmt_b & ~1) ||
       (accumulate && !out_f32))
     return 7;

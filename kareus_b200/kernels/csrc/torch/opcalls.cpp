@@ -7,6 +7,7 @@
 namespace {
 
 const at::ScalarType FP8[2] = {at::kFloat8_e4m3fn, at::kFloat8_e5m2};
+constexpr int64_t FP8_MOST = (int64_t(1) << 31) - 512;     // rows and columns that kb_fp8_quantize and kb_gemm_fp8 take
 
 bool current(const at::Tensor& t) { return t.device().index() == c10::cuda::getCurrentCUDAStream().device_index(); }
 bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
@@ -31,7 +32,7 @@ PyObject* fp8_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const long fmt = PyLong_AsLong(args[4]);
   if (rows < 0 || cols < 0 || square < 0 || PyErr_Occurred()) return nullptr;
   const int64_t M = x->size(0), N = x->size(1);
-  if (!(rows || cols) || fmt < 0 || fmt > 1 || M < 1 || N < 1 || M > INT_MAX || N > INT_MAX) Py_RETURN_NONE;
+  if (!(rows || cols) || fmt < 0 || fmt > 1 || M < 1 || N < 1 || M > FP8_MOST || N > FP8_MOST) Py_RETURN_NONE;
   const int64_t ld = M > 1 ? x->stride(0) : N;
   if ((x->stride(1) != 1 && N > 1) || ld < N) Py_RETURN_NONE;
   const auto o = x->options().requires_grad(false);
@@ -83,7 +84,7 @@ Operand operand(PyObject* data, PyObject* scales) {
   for (int i = 0; i < 5; ++i)
     if (m.s->size(i) != want[i]) return m;
   const int64_t ld = m.rows > 1 ? m.d->stride(0) : (m.k + 15) / 16 * 16;
-  if (m.rows < 1 || m.k < 1 || m.rows > INT_MAX || m.k > INT_MAX || m.d->stride(1) != 1 || ld % 16 || ld < m.k || !aligned(*m.d) ||
+  if (m.rows < 1 || m.k < 1 || m.rows > FP8_MOST || m.k > FP8_MOST || m.d->stride(1) != 1 || ld % 16 || ld < m.k || !aligned(*m.d) ||
       !aligned(*m.s))
     return m;
   m.ld = ld;

@@ -12,6 +12,7 @@ from . import ref
 from .cuda import KernelError, _check, _count, _rows_readable, _stream, lib, require_current_device, status_word
 
 _FORMAT_CODE = {"e4m3": 0, "e5m2": 1}
+_MOST = (1 << 31) - 512          # rows and columns, whose numbers are ints in the kernels
 _DTYPE = {fmt: ref.FP8_FORMATS[fmt][0] for fmt in _FORMAT_CODE}
 
 
@@ -74,7 +75,7 @@ def quantize(x, rows: bool = True, cols: bool = False, square: bool = False, fmt
         raise KernelError(f"fp8_quantize takes a matrix of floating-point numbers, got {x.dtype} of shape {tuple(x.shape)}")
     if not (rows or cols):
         raise KernelError("fp8_quantize: neither rows nor columns are wanted")
-    if x.shape[0] >= 1 << 31 or x.shape[1] >= 1 << 31:
+    if max(x.shape) > _MOST:
         raise KernelError(f"fp8_quantize: {tuple(x.shape)} is too large")
     if not (x.is_cuda and x.dtype == torch.bfloat16):
         return _statement(x, fmt, square) if rows else None, _statement(x.t(), fmt, square) if cols else None
@@ -114,6 +115,8 @@ def gemm(a: Fp8Matrix, b: Fp8Matrix, out_dtype=None, accumulate=None, out=None):
     (M, K), (N, Kb) = a.shape, b.shape
     if K != Kb:
         raise ValueError(f"fp8_gemm shape mismatch: K={K} vs {Kb}")
+    if max(M, N, K) > _MOST:
+        raise KernelError(f"fp8_gemm: {M} x {N} x {K} is too large")
     if accumulate is not None and (out is not None or out_dtype is not None):
         raise KernelError("fp8_gemm: accumulate names the result, out and out_dtype cannot be given with it")
     if out is not None and out_dtype is not None and out.dtype != out_dtype:

@@ -8,7 +8,7 @@ import torch
 
 from kareus_b200 import kernels as K
 from kareus_b200.kernels import ref
-from kareus_b200.kernels.cuda import KernelError
+from kareus_b200.kernels.cuda import KernelError, lib
 from kareus_b200.kernels.fp8 import Fp8Matrix
 
 gpu = pytest.mark.gpu
@@ -338,3 +338,16 @@ def test_gpu_refusals():
         K.fp8_gemm(Fp8Matrix(a.data[:, 1:], a.scales), Fp8Matrix(a.data[:, 1:], a.scales))
     with pytest.raises(KernelError, match="contiguous"):
         K.fp8_gemm(a, a, out=torch.zeros(32, 32, device="cuda").t()[:, :32].t().t())
+
+
+def test_largest_sizes():
+    """Row and column numbers are ints in the kernels, those of tiles that cross the edge too: sizes near 2^31 are refused."""
+    one = torch.zeros(1, 1, dtype=torch.bfloat16)
+    for shape in ((2 ** 31 - 511, 1), (1, 2 ** 31 - 1), (2 ** 31, 1)):
+        with pytest.raises(KernelError, match="too large"):
+            K.fp8_quantize(one.expand(shape))
+    L = lib()
+    for rows, cols in ((2 ** 31 - 511, 8), (8, 2 ** 31 - 1)):      # refused by the entry itself, before anything is launched
+        assert L.kb_fp8_quantize(16, rows, cols, cols, 16, 2 ** 31, 16, 16, 2 ** 31, 16, 0, 0, 0) == 7
+    for m, n, k in ((2 ** 31 - 511, 8, 16), (8, 2 ** 31 - 1, 16), (8, 8, 2 ** 31 - 511)):
+        assert L.kb_gemm_fp8(16, 16, 0, 2 ** 31, 16, 16, 0, 2 ** 31, 16, 2 ** 31, m, n, k, 0, 0, 0, 0) == 7
