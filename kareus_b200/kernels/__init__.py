@@ -328,8 +328,9 @@ def adamw_step(p, g, m, v, master, lr, beta1, beta2, eps, wd, step, grad_scale=1
 def orthogonalize(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     """The last two dimensions of ``x`` after ``steps`` Newton-Schulz products, as bf16: ``X = x / (|x|_F + eps)``, then ``G = X Xt;
     X = a X + (b G + c G G) X``.  Singular vectors stay, singular values go to about 1 (0.7 to 1.2 with these coefficients and five
-    steps); ones below about 1e-3 of the largest stay small.  The products run in fp16 with fp32 sums.  A matrix with an infinity or
-    a NaN becomes NaN, one of zeros stays zero.  ``coefficients`` that let the iterates leave the range of fp16 are refused."""
+    steps); ones below about 1e-3 of the largest stay small.  The products run in fp16 with fp32 sums.  A matrix with an infinity, a
+    NaN or a sum of squares beyond fp32 becomes NaN, one of zeros stays zero.  ``eps`` is at least 1e-12; ``coefficients`` that let
+    the iterates leave the range of fp16 are refused."""
     from .muon import orthogonalize as f
     return f(x, steps, coefficients, eps)
 

@@ -42,8 +42,10 @@ def fp16_scales(steps: int, coefficients: tuple) -> tuple:
 
 def _parameters(steps, coefficients, eps):
     steps, coefficients, eps = int(steps), tuple(float(v) for v in coefficients), float(eps)
-    if steps < 1 or len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients) or not eps >= 0:
-        raise KernelError(f"Newton-Schulz: at least one step, three finite coefficients and eps >= 0, got {steps}, {coefficients}, {eps}")
+    # squares are summed in fp32: of entries below 1e-19, whose squares it does not hold, the norm counts for nothing beside such an eps
+    if steps < 1 or len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients) or not 1e-12 <= eps < math.inf:
+        raise KernelError(f"Newton-Schulz: at least one step, three finite coefficients and a finite eps >= 1e-12, got {steps}, "
+                          f"{coefficients}, {eps}")
     return steps, coefficients, eps
 
 

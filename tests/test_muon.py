@@ -272,3 +272,19 @@ def test_gpu_refusals():
         K.muon_step(g.bfloat16(), g, g.clone(), g.clone(), lr=1e-3, grad_scale_tensor=torch.ones(2, device="cuda"))
     with pytest.raises(KernelError, match="devices"):
         K.muon_step(g.bfloat16(), g, g.cpu(), g.clone(), lr=1e-3)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_smallest_eps(device):
+    """Squares of entries below 1e-19 are no fp32 numbers, so the norm of a matrix of them reads 0: it must not count beside eps."""
+    x = matrices(1, 24, 40, device, seed=15)
+    for eps in (0.0, 1e-30, float("inf"), float("nan")):
+        with pytest.raises(KernelError, match="eps"):
+            K.orthogonalize(x, eps=eps)
+    # Entries of 1e-21 leave X at 1e-9 and, times 2^14, among fp16's subnormal numbers: off by 2^-25 of 5e-5 for the largest, a third
+    # of that again in each step that takes X to 3.4 times itself, 1e-3 in all; 2^-8 is the result's rounding.  Together below 2^-7.
+    for f in (1e-18, 1e-9):
+        y = (x * f).float()
+        o = K.orthogonalize(y, eps=1e-12)
+        exact = iterate(y, eps=1e-12)
+        assert torch.isfinite(o).all() and bool((o.double() - exact).abs().max() <= 2.0 ** -7 * exact.abs().max())
