@@ -94,12 +94,12 @@ def muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, step
         raise KernelError(f"muon_step: tensors on several devices: {[str(t.device) for t in (p, g, m, master)]}")
     if scale is None:
         scale = 0.2 * math.sqrt(max(g.shape))
-    if not (g.is_cuda and g.dtype == torch.float32 and p.dtype == torch.bfloat16):
+    if not (g.is_cuda and p.dtype == torch.bfloat16):
         gs = 1.0 if grad_scale_tensor is None else grad_scale_tensor.to(g.dtype)
         return ref.muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, steps, coefficients, eps, gs)
     require_current_device("muon_step", g)
-    if m.dtype != torch.float32 or master.dtype != torch.float32 or not all(t.is_contiguous() for t in (p, g, m, master)):
-        raise KernelError("muon_step: momentum and master have to be fp32, all tensors contiguous")
+    if any(t.dtype != torch.float32 for t in (g, m, master)) or not all(t.is_contiguous() for t in (p, g, m, master)):
+        raise KernelError("muon_step: gradient, momentum and master have to be fp32, all tensors contiguous")
     if grad_scale_tensor is not None and (grad_scale_tensor.dtype != torch.float32 or grad_scale_tensor.numel() != 1
                                           or grad_scale_tensor.device != g.device):
         raise KernelError("muon_step: the gradient's factor is one fp32 value on the gradient's device")

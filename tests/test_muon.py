@@ -288,3 +288,12 @@ def test_smallest_eps(device):
         o = K.orthogonalize(y, eps=1e-12)
         exact = iterate(y, eps=1e-12)
         assert torch.isfinite(o).all() and bool((o.double() - exact).abs().max() <= 2.0 ** -7 * exact.abs().max())
+
+
+@gpu
+def test_gradient_type():
+    """A bf16 weight on the GPU has an fp32 gradient; no other one is taken through plain PyTorch instead."""
+    g = matrices(1, 8, 12)[0].clone()
+    for t in (torch.bfloat16, torch.float64):
+        with pytest.raises(KernelError, match="fp32"):
+            K.muon_step(g.bfloat16(), g.to(t), g.clone(), g.clone(), lr=1e-3)
