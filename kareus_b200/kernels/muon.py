@@ -24,7 +24,7 @@ def fp16_scales(steps: int, coefficients: tuple) -> tuple:
     a, b, c = coefficients
     bound, worst, worst_q = 1.0, 1.0, 1.0
     for k in range(steps):
-        s = torch.linspace(0.0, bound * 1.01, 8193, dtype=torch.float64)       # 1 %: what rounding adds
+        s = torch.linspace(0.0, bound * 1.01, 8193, dtype=torch.float64, device="cpu")       # 1 %: what rounding adds
         t, prod = s * s, 1.0
         for j in range(min(3, steps - k)):
             q = a + b * t + c * t * t

@@ -297,3 +297,10 @@ def test_gradient_type():
     for t in (torch.bfloat16, torch.float64):
         with pytest.raises(KernelError, match="fp32"):
             K.muon_step(g.bfloat16(), g.to(t), g.clone(), g.clone(), lr=1e-3)
+
+
+def test_scales_under_another_default_device():
+    want = fp16_scales(5, COEFFICIENTS)
+    fp16_scales.cache_clear()
+    with torch.device("meta"):
+        assert fp16_scales(5, COEFFICIENTS) == want
