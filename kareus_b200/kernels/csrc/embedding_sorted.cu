@@ -6,9 +6,9 @@
 // and tokens that make up much of a batch (padding, a frequent word) queue up for the same addresses.  Here the tokens are sorted
 // first and each row of the table gets one addition of a sum that was formed in registers:
 //
-//   1. Stable radix sort of (id, t) by one cluster of eight blocks, small batches by one block.  Items stay in the blocks' shared memory; a pass ranks the items
-//      of a warp by ballots over the digit's bits, adds up the counts of warps, blocks and digits, and writes every item to its
-//      place in the shared memory of the block that owns it.  Tokens of other shards are left out.
+//   1. Stable radix sort of (id, t) by one cluster of eight blocks, small batches by one block.  Items stay in the blocks' shared
+//      memory; a pass ranks the items of a warp by ballots over the digit's bits, adds up the counts of warps, blocks and digits, and
+//      writes every item to its place in the shared memory of the block that owns it.  Tokens of other shards are left out.
 //   2. Blocks take windows of `window` sorted positions and 1024 columns, sum the rows of each token in order and add the sum to the
 //      table.  A token whose positions cross the border of a window leaves partial sums: the part that began before the window and
 //      the part that goes on after it.
@@ -16,8 +16,8 @@
 //
 // The order of additions depends on the tokens alone, so the same inputs give the same bits.  Sums are fp32.
 //
-// What bounds it: memory for the lookup and the sums, latency for the sort and the join.  One B200, us: 8192 x 4096 into 128256 rows lookup
-// 18, sort 12, sums 50, join 7; 32768 x 2048, a third of it one token, 22, 14, 25, 13 (the atomic form queues for that token's row).
+// What bounds it: memory for the lookup and the sums, latency for the sort and the join.  One B200, us: 8192 x 4096 into 128256 rows
+// lookup 18, sort 12, sums 50, join 7; 32768 x 2048, a third of it one token, 22, 14, 25, 13 (the atomic form queues for that row).
 #include <cuda_bf16.h>
 #include "sm100.cuh"
 #include "launch.h"
@@ -34,7 +34,7 @@ constexpr int EL_TOKENS = 4;
 template <bool VEC>
 __global__ void __launch_bounds__(128)
 embedding_fwd_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __restrict__ w, __nv_bfloat16* __restrict__ out, long ntok,
-                        int H, long first, long rows, float scale) {
+                     int H, long first, long rows, float scale) {
   pdl_begin();
   const long t0 = static_cast<long>(blockIdx.x) * EL_TOKENS;
   long id[EL_TOKENS];
@@ -455,13 +455,13 @@ static long chunk_bytes(long n, int H) {
 }  // namespace kb
 
 extern "C" int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,
-                                       cudaStream_t stream) {
+                                cudaStream_t stream) {
   if (ntok <= 0 || H <= 0 || rows <= 0) return 7;
   const bool vec = H % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
   const long grid = (ntok + kb::EL_TOKENS - 1) / kb::EL_TOKENS;
   if (grid >= 1L << 31) return 7;
-  KB_LAUNCH_PDL((vec ? kb::embedding_fwd_kernel<true> : kb::embedding_fwd_kernel<false>), static_cast<unsigned>(grid), 128, 0, stream, tokens,
-                static_cast<const __nv_bfloat16*>(w), static_cast<__nv_bfloat16*>(out), ntok, H, first, rows, scale);
+  KB_LAUNCH_PDL((vec ? kb::embedding_fwd_kernel<true> : kb::embedding_fwd_kernel<false>), static_cast<unsigned>(grid), 128, 0, stream,
+                tokens, static_cast<const __nv_bfloat16*>(w), static_cast<__nv_bfloat16*>(out), ntok, H, first, rows, scale);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }
@@ -477,7 +477,8 @@ extern "C" long kb_embedding_sorted_bytes(long ntok, int H) {
 extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, float* grad, long ntok, int H, long first, long rows,
                                        float scale, void* work, cudaStream_t stream) {
   using namespace kb;
-  if (ntok <= 0 || H <= 0 || rows <= 0 || rows >= 1L << 31 || !work || reinterpret_cast<uintptr_t>(work) % 256) return 7;
+  constexpr int MOST = 65535 * EC_COLS;         // columns, one row of blocks for each EC_COLS of them
+  if (ntok <= 0 || H <= 0 || H > MOST || rows <= 0 || rows >= 1L << 31 || !work || reinterpret_cast<uintptr_t>(work) % 256) return 7;
   const bool vec = H % 8 == 0 && reinterpret_cast<uintptr_t>(dout) % 16 == 0 && reinterpret_cast<uintptr_t>(grad) % 16 == 0;
   int bits_all = 1;
   while ((rows - 1) >> bits_all) ++bits_all;              // keys 0 .. rows - 1
@@ -521,8 +522,8 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
                   passes, bits, ids, order);
     KB_LAUNCH_PDL((vec ? embedding_window_kernel<true> : embedding_window_kernel<false>), dim3(windows, (H + EW_COLS - 1) / EW_COLS),
                   EW_THREADS, 0, stream, s);
-    KB_LAUNCH_PDL((vec ? embedding_join_kernel<true> : embedding_join_kernel<false>), dim3((windows + EC_WARPS - 1) / EC_WARPS, (H + EC_COLS - 1) / EC_COLS),
-                  EC_THREADS, 0, stream, s);
+    KB_LAUNCH_PDL((vec ? embedding_join_kernel<true> : embedding_join_kernel<false>),
+                  dim3((windows + EC_WARPS - 1) / EC_WARPS, (H + EC_COLS - 1) / EC_COLS), EC_THREADS, 0, stream, s);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);

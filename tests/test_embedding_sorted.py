@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from kareus_b200 import kernels as K
-from kareus_b200.kernels.cuda import KernelError
+from kareus_b200.kernels.cuda import KernelError, lib
 
 gpu = pytest.mark.gpu
 
@@ -220,3 +220,8 @@ def test_gpu_refusals():
         K.embedding_bwd(w[:3].contiguous(), t, torch.zeros(16, 10, device="cuda").t(), 0, order="sorted")
     with pytest.raises(KernelError, match="current device"):
         K.embedding_fwd(t.cpu(), w, 0, scale=2.0)
+
+
+def test_widest_table():
+    """A table whose columns the last kernel's grid does not reach is refused before the first one has added to it."""
+    assert lib().kb_embedding_bwd_sorted(16, 16, 16, 4, 65535 * 128 + 1, 0, 4, 1.0, 256, 0) == 7
