@@ -12,11 +12,11 @@
 // rounded diagonal does to the result's.  Norms are summed in fp32 per thread and fp64 beyond, in a fixed order.
 //
 // Long matrices.  X_{k+1} = Q_k X_k with Q_k = a I + P_k, and G_{k+1} = Q_k G_k Q_k, where everything but X is as small as the shorter
-// side.  Where the longer side is at least 1.5 times the shorter one and it saves time (ns_carries), G is carried from step to step so (T = Q G, G' = Q T), the Q are
-// multiplied up, and X is read twice per segment of two or three steps instead of twice per step: five steps of a matrix with
-// sides m and r m take 6 r + 14 units of m^3 multiplications instead of 15 r + 5.  G of a carried step is off by the roundings
-// before it, and small singular values suffer most from that; with segments of three and two steps (the singular values grow in
-// the first, settle in the second) the result is as exact as step by step, with one of five it would not be.
+// side.  Where the longer side is at least 1.5 times the shorter one and it saves time (ns_carries), G is carried from step to step
+// so (T = Q G, G' = Q T), the Q are multiplied up, and X is read twice per segment of two or three steps instead of twice per step:
+// five steps of a matrix with sides m and r m take 6 r + 14 units of m^3 multiplications instead of 15 r + 5.  G of a carried step
+// is off by the roundings before it, and small singular values suffer most from that; with segments of three and two steps (the
+// singular values grow in the first, settle in the second) the result is as exact as step by step, with one of five it would not be.
 //
 // G, P, T and the products of the Q are symmetric: only the tiles on and above the diagonal are computed, the others are written as
 // their transposes.
@@ -297,7 +297,10 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         const int dc = tn * bn + c * SLAB + 2 * lane;
         const float* d = ep.diag + static_cast<size_t>(z) * ep.len;
         d_next = make_float2(dc < N ? d[dc] : 0.f, dc + 1 < N ? d[dc + 1] : 0.f);
-        if (ep.rounded != 0.f) d_next = make_float2(d_next.x - rounded16(d_next.x, ep.rounded), d_next.y - rounded16(d_next.y, ep.rounded));
+        if (ep.rounded != 0.f) {
+          d_next.x -= rounded16(d_next.x, ep.rounded);
+          d_next.y -= rounded16(d_next.y, ep.rounded);
+        }
       }
     };
     if (ADDS && first < units && h < slabs) fetch(first, h);
@@ -362,7 +365,8 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              st_shared_v4(smem_u32(stg0) + lane * 128 + half * 4096 + ((j ^ (lane & 7)) << 4), a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]);
+              st_shared_v4(smem_u32(stg0) + lane * 128 + half * 4096 + ((j ^ (lane & 7)) << 4), a[4 * j], a[4 * j + 1], a[4 * j + 2],
+                           a[4 * j + 3]);
           }
           if (c + 2 >= slabs) {
             tc_fence_before();
@@ -512,7 +516,8 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
               b.w = muon_weight(b.w, __uint_as_float(x.w & 0xffff0000u), ep.keep, ep.step);
               m[0] = a;
               m[1] = b;
-              *reinterpret_cast<uint4*>(ep.p + at) = make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
+              *reinterpret_cast<uint4*>(ep.p + at) =
+                  make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(a.z, a.w), pack_bf16x2(b.x, b.y), pack_bf16x2(b.z, b.w));
             }
             __syncwarp();
           }
@@ -576,7 +581,8 @@ ns_sum_parts_kernel(const float* __restrict__ work, __half* __restrict__ G, long
   t[r][c] = s.x; t[r][c + 1] = s.y; t[r][c + 2] = s.z; t[r][c + 3] = s.w;
   __syncthreads();
   if (col0 + r < side && row0 + c < ldg)
-    *reinterpret_cast<uint2*>(g + (col0 + r) * ldg + row0 + c) = make_uint2(pack_f16x2(t[c][r], t[c + 1][r]), pack_f16x2(t[c + 2][r], t[c + 3][r]));
+    *reinterpret_cast<uint2*>(g + (col0 + r) * ldg + row0 + c) =
+        make_uint2(pack_f16x2(t[c][r], t[c + 1][r]), pack_f16x2(t[c + 2][r], t[c + 3][r]));
 }
 
 // ----------------------------------------------------------------------------- the passes around the products
@@ -760,7 +766,7 @@ static NsPlan ns_plan(int mode, long matrices, int M, int N, int K) {
     }
   }
   // Few tiles and a long sum: parts of 8 steps and more on the SMs that would idle, where that saves more than the 5 us that adding
-  // them up takes.  32 x 14336: 316 us as one part, 122 so.
+  // them up takes.  20 x 14336, step by step: 316 us as one part, 134 so.
   if (mode == NS_GRAM) {
     const long units = matrices * p.per_matrix;
     long parts = units ? sms / units : 1;
@@ -906,8 +912,8 @@ struct MuonApply {
   float keep, step;
 };
 
-static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch, int m, int n, float a, float b, float c, int steps, float eps, float scale,
-                         float scale_q, void* out, uint8_t* work, int* status, cudaStream_t stream) {
+static int newton_schulz(const NsSource& src, const MuonApply& apply, int batch, int m, int n, float a, float b, float c, int steps,
+                         float eps, float scale, float scale_q, void* out, uint8_t* work, int* status, cudaStream_t stream) {
   const NsLayout lay(batch, m, n);
   uint8_t* const x[2] = {work, work + lay.x};
   uint8_t* const square = work + 2 * lay.x;
@@ -1073,7 +1079,8 @@ extern "C" int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n
       reinterpret_cast<uintptr_t>(work) % 256)
     return 7;
   const kb::NsSource src{x, nullptr, nullptr, 0.f, bf16 != 0, false};
-  return kb::newton_schulz(src, kb::MuonApply{}, batch, m, n, a, b, c, steps, eps, scale, scale_q, out, static_cast<uint8_t*>(work), status, stream);
+  return kb::newton_schulz(src, kb::MuonApply{}, batch, m, n, a, b, c, steps, eps, scale, scale_q, out, static_cast<uint8_t*>(work),
+                           status, stream);
 }
 // Whether the last product of the optimizer step also updates the weights (no kernel of their own): rows of whole 16-byte units.
 extern "C" int kb_muon_fuses(const void* master, const void* p, int n) {
@@ -1091,7 +1098,8 @@ extern "C" int kb_muon_step(const float* g, float* mom, float* master, void* p, 
   const bool fused = kb_muon_fuses(master, p, n);
   kb::MuonApply apply{};
   if (fused) apply = kb::MuonApply{master, static_cast<__nv_bfloat16*>(p), keep, step};
-  const int rc = kb::newton_schulz(src, apply, 1, m, n, a, b, c, steps, eps, scale, scale_q, o, static_cast<uint8_t*>(work), status, stream);
+  const int rc = kb::newton_schulz(src, apply, 1, m, n, a, b, c, steps, eps, scale, scale_q, o, static_cast<uint8_t*>(work), status,
+                                   stream);
   if (rc || fused) return rc;
   const long count = (long)m * n;
   long blocks = (count + 1023) / 1024;

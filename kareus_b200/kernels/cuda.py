@@ -739,7 +739,7 @@ def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
     if not out.numel():
         return out
     _check(lib().kb_embedding_fwd(tokens.data_ptr(), weight.data_ptr(), out.data_ptr(), tokens.numel(), H,
-                                         int(vocab_start), weight.shape[0], float(scale), _stream()), "embedding_fwd")
+                                  int(vocab_start), weight.shape[0], float(scale), _stream()), "embedding_fwd")
     _count()
     return out
 

@@ -113,5 +113,6 @@ def muon_step(p, g, m, master, lr, momentum, weight_decay, scale, nesterov, step
                               0 if grad_scale_tensor is None else grad_scale_tensor.data_ptr(), *coefficients, steps, eps,
                               *fp16_scales(steps, coefficients), work.data_ptr(), status_word(g.device).data_ptr(), _stream()),
            f"muon_step {rows} x {cols}")
-    _count(lib().kb_newton_schulz_launches(1, rows, cols, steps) + (0 if lib().kb_muon_fuses(master.data_ptr(), p.data_ptr(), cols) else 1))
+    fused = lib().kb_muon_fuses(master.data_ptr(), p.data_ptr(), cols)
+    _count(lib().kb_newton_schulz_launches(1, rows, cols, steps) + (0 if fused else 1))
     return o
