@@ -17,7 +17,7 @@
 // The order of additions depends on the tokens alone, so the same inputs give the same bits.  Sums are fp32.
 //
 // What bounds it: memory for the lookup and the sums, latency for the sort and the join.  One B200, us: 8192 x 4096 into 128256 rows
-// lookup 18, sort 12, sums 50, join 7; 32768 x 2048, a third of it one token, 22, 14, 25, 13 (the atomic form queues for that row).
+// lookup 18, sort 12, sums 39, join 8; 32768 x 2048, a third of it one token, 21, 14, 24, 12 (the atomic form queues for that row).
 #include <cuda_bf16.h>
 #include "sm100.cuh"
 #include "launch.h"
@@ -346,9 +346,9 @@ __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const Embe
 }
 
 // Tokens that cross windows.  A warp looks whether one begins in its window and goes on.  If it ends within the next few windows the
-// warp adds up the parts itself; otherwise the block's eight warps share them, each a run of consecutive windows, eight of them on
-// their way at once.  128 columns a block.
-constexpr int EC_THREADS = 256;
+// warp adds up the parts itself; otherwise the block's sixteen warps share them, each a run of consecutive windows, sixteen of them on
+// their way at once (eight and eight took 37 us instead of 33 for 8192 x 2048, nine tenths of it one token).  128 columns a block.
+constexpr int EC_THREADS = 512;
 constexpr int EC_WARPS = EC_THREADS / 32;
 constexpr int EC_COLS = 128;
 constexpr int EC_SHORT = 8;
@@ -358,7 +358,7 @@ template <bool VEC>
 __device__ __forceinline__ float4 sum_parts(const EmbeddingSum& p, int from, int to, int col, int left) {
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   if (left <= 0) return acc;
-#pragma unroll 8
+#pragma unroll 16
   for (int v = from; v < to; ++v) {
     const float* q = p.before + static_cast<size_t>(v) * p.H + col;
     float4 x;
@@ -440,15 +440,17 @@ __global__ void __launch_bounds__(EC_THREADS) embedding_join_kernel(const Embedd
 }
 
 // ----------------------------------------------------------------------------- host side
-// Sorted positions per block of the sums: 64 where that fills the chip twice over, fewer for small batches.
-static int sum_window(long n, int H) {
-  const long cols = (H + EW_COLS - 1) / EW_COLS;
+// Sorted positions per block of the sums: 64, fewer where that would be less than 512 windows, whose blocks wait for memory side by
+// side.  More windows leave a frequent token in more parts to be joined.  One B200, us, 8192 x 5120: 64 positions 97, 32 86, 16 83,
+// 8 85; nine tenths of it one token: 52, 49, 50, 58.  Over 2048 to 65536 tokens, 512 to 5120 columns and none, a third or nine tenths
+// of one token, 512 windows take 3 % less than only as many as fill the chip twice (geometric mean), 1024 are as slow as those.
+static int sum_window(long n) {
   int w = EW_MOST;
-  while (w > EW_BATCH && (n + w - 1) / w * cols < 2L * device_sm_count()) w /= 2;
+  while (w > EW_BATCH && (n + w - 1) / w < 512) w /= 2;
   return w;
 }
 static long chunk_bytes(long n, int H) {
-  const long windows = (n + sum_window(n, H) - 1) / sum_window(n, H);
+  const long windows = (n + sum_window(n) - 1) / sum_window(n);
   return (4L * n + 255) / 256 * 256 * 2 + 2L * windows * H * 4;
 }
 
@@ -505,7 +507,7 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
     uint8_t* base = static_cast<uint8_t*>(work);
     uint32_t* ids = reinterpret_cast<uint32_t*>(base);
     uint32_t* order = reinterpret_cast<uint32_t*>(base + list);
-    s.window = sum_window(n, H);
+    s.window = sum_window(n);
     const int windows = (n + s.window - 1) / s.window;
     s.dout = static_cast<const __nv_bfloat16*>(dout) + at * H;
     s.ids = ids;
