@@ -6,9 +6,9 @@
 // and tokens that make up much of a batch (padding, a frequent word) queue up for the same addresses.  Here the tokens are sorted
 // first and each row of the table gets one addition of a sum that was formed in registers:
 //
-//   1. Stable radix sort of (id, t) by one cluster of eight blocks, small batches by one block.  Items stay in the blocks' shared
-//      memory; a pass ranks the items of a warp by ballots over the digit's bits, adds up the counts of warps, blocks and digits, and
-//      writes every item to its place in the shared memory of the block that owns it.  Tokens of other shards are left out.
+//   1. Stable radix sort of (id, t) by one cluster of eight blocks.  Items stay in the blocks' shared memory; a pass ranks the items
+//      of a warp by ballots over the digit's bits, adds up the counts of warps, blocks and digits, and writes every item to its
+//      place in the shared memory of the block that owns it.  Tokens of other shards are left out.  Small batches: by counting.
 //   2. Blocks take windows of `window` sorted positions and 1024 columns, sum the rows of each token in order and add the sum to the
 //      table.  A token whose positions cross the border of a window leaves partial sums: the part that began before the window and
 //      the part that goes on after it.
@@ -72,7 +72,6 @@ embedding_fwd_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __res
 
 // ----------------------------------------------------------------------------- sort
 constexpr int ES_BLOCKS = 8;                   // of a cluster
-constexpr int ES_ALONE = 2048;                 // batches that one block sorts: 512 tokens in 7.4 us, in 8.5 by a cluster
 constexpr int ES_THREADS = 1024;
 constexpr int ES_WARPS = ES_THREADS / 32;
 constexpr int ES_PER_BLOCK = 8192;             // items
@@ -93,25 +92,21 @@ __device__ __forceinline__ uint32_t ld_cluster(uint32_t local, uint32_t rank) {
   return v;
 }
 
-// ids / order [n]: keys below `rows` in ascending order and where they stood; ids behind them are `rows`.  `per`: items of each of
-// BLOCKS blocks (a multiple of 32, at most ES_PER_BLOCK, BLOCKS * per >= n); `passes` digits of `bits` (at most ES_BITS) bits hold
-// every key.  Tokens of other shards leave in the first pass.
-template <int BLOCKS>
-__device__ __forceinline__ void sort_tokens(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
-                                            uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
+// ids / order [n]: keys below `rows` in ascending order and where they stood; ids behind them are `rows`.  `per`: items of each block
+// (a multiple of 32, at most ES_PER_BLOCK, ES_BLOCKS * per >= n); `passes` digits of `bits` (at most ES_BITS) bits hold every key.
+// Tokens of other shards leave in the first pass.
+__global__ void __cluster_dims__(ES_BLOCKS, 1, 1) __launch_bounds__(ES_THREADS, 1)
+embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
+                      uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
   extern __shared__ uint4 sm[];
   __shared__ uint32_t count[ES_BINS], base[ES_BINS], warp_sum[ES_BINS / 32];
   uint32_t* const hist = reinterpret_cast<uint32_t*>(sm);              // [warps][bins] of 16 bits
   constexpr int HIST_WORDS = ES_BINS / 2;
   uint2 *src = reinterpret_cast<uint2*>(hist + ES_WARPS * HIST_WORDS), *dst = src + per;      // (key, position)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = BLOCKS > 1 ? blockIdx.x : 0;
+  const uint32_t rank = blockIdx.x;
   const int bins = 1 << bits;
   const int all = n;
-  const auto sync = [] {
-    if (BLOCKS > 1) cluster_sync_all();
-    else __syncthreads();
-  };
   int begin = static_cast<int>(rank) * per, here = max(0, min(per, n - begin));
   pdl_begin();
   for (int i = tid; i < here; i += ES_THREADS) {
@@ -161,12 +156,12 @@ __device__ __forceinline__ void sort_tokens(const long* __restrict__ tokens, int
       count[2 * tid] = sum & 0xffffu;
       count[2 * tid + 1] = sum >> 16;
     }
-    sync();
+    cluster_sync_all();
     uint32_t total = 0, before = 0;                       // of this digit in the cluster, in the blocks before
     if (tid < bins) {
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        const uint32_t c = BLOCKS > 1 ? ld_cluster(smem_u32(&count[tid]), b) : count[tid];
+      for (int b = 0; b < ES_BLOCKS; ++b) {
+        const uint32_t c = ld_cluster(smem_u32(&count[tid]), b);
         if (b < static_cast<int>(rank)) before += c;
         total += c;
       }
@@ -191,7 +186,7 @@ __device__ __forceinline__ void sort_tokens(const long* __restrict__ tokens, int
 #pragma unroll
       for (int w = 0; w < ES_BINS / 32; ++w) n += static_cast<int>(warp_sum[w]);
     }
-    const int next_per = max(32, (n + BLOCKS - 1) / BLOCKS);
+    const int next_per = max(32, (n + ES_BLOCKS - 1) / ES_BLOCKS);
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < ES_STEPS; ++s) {
@@ -201,12 +196,11 @@ __device__ __forceinline__ void sort_tokens(const long* __restrict__ tokens, int
         if (item.x < rows) {
           const uint32_t d = (item.x >> shift) & (bins - 1);
           const uint32_t at = base[d] + mine[d] + where[s], block = at / static_cast<uint32_t>(next_per);
-          if (BLOCKS > 1) st_cluster(smem_u32(dst + (at - block * next_per)), block, item);
-          else dst[at] = item;
+          st_cluster(smem_u32(dst + (at - block * next_per)), block, item);
         }
       }
     }
-    sync();
+    cluster_sync_all();
     per = next_per;
     begin = static_cast<int>(rank) * per;
     here = max(0, min(per, n - begin));
@@ -218,19 +212,68 @@ __device__ __forceinline__ void sort_tokens(const long* __restrict__ tokens, int
     ids[begin + i] = src[i].x;
     order[begin + i] = src[i].y;
   }
-  for (int i = n + static_cast<int>(rank) * ES_THREADS + tid; i < all; i += BLOCKS * ES_THREADS) ids[i] = static_cast<uint32_t>(rows);
-}
-__global__ void __cluster_dims__(ES_BLOCKS, 1, 1) __launch_bounds__(ES_THREADS, 1)
-embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
-                      uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
-  sort_tokens<ES_BLOCKS>(tokens, n, per, first, rows, passes, bits, ids, order);
-}
-__global__ void __launch_bounds__(ES_THREADS, 1)
-embedding_sort_small_kernel(const long* __restrict__ tokens, int n, int per, long first, long rows, int passes, int bits,
-                            uint32_t* __restrict__ ids, uint32_t* __restrict__ order) {
-  sort_tokens<1>(tokens, n, per, first, rows, passes, bits, ids, order);
+  for (int i = n + static_cast<int>(rank) * ES_THREADS + tid; i < all; i += ES_BLOCKS * ES_THREADS) ids[i] = static_cast<uint32_t>(rows);
 }
 
+// The same for small batches, by counting: the place of a token is the number of smaller ones and of equal ones before it.  A block
+// holds all keys, a warp counts for ITEMS consecutive tokens, 128 keys at a time.  What a radix pass takes are its many steps; here is
+// one, of n^2 comparisons, over as many blocks as there are.
+// One B200, us of the gradient of n x 2048, by a cluster / by counting: 64 11.4 / 5.4, 512 12.6 / 7.8, 2048 18.6 / 14.6, 3000 22.0 / 19.0,
+// 4096 24.9 / 23.9; with one token a warp and with two: 512 9.8 / 7.8, 1000 11.5 / 11.5, 1500 14.0 / 15.0, 3000 19.0 / 21.3.
+constexpr int ER_MOST = 4096;                  // tokens
+constexpr int ER_TWO = 1024;                   // up to here a warp counts for two
+constexpr int ER_THREADS = 256;
+
+template <int ITEMS>
+__global__ void __launch_bounds__(ER_THREADS)
+embedding_rank_kernel(const long* __restrict__ tokens, int n, long first, long rows, uint32_t* __restrict__ ids,
+                      uint32_t* __restrict__ order) {
+  extern __shared__ uint4 sm[];                // [n rounded up to 128] keys, the largest number behind the last
+  uint32_t* const keys = reinterpret_cast<uint32_t*>(sm);
+  const int chunks = (n + 127) / 128, lane = threadIdx.x & 31;
+  pdl_begin();
+#pragma unroll 8
+  for (int i = threadIdx.x; i < chunks * 128; i += ER_THREADS) {
+    const long id = i < n ? tokens[i] - first : 0;
+    keys[i] = i < n ? static_cast<uint32_t>(id >= 0 && id < rows ? id : rows) : 0xffffffffu;
+  }
+  __syncthreads();
+  const int i0 = (blockIdx.x * (ER_THREADS / 32) + (threadIdx.x >> 5)) * ITEMS;
+  if (i0 >= n) return;
+  uint32_t me[ITEMS];
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) me[k] = keys[i0 + k];
+  uint32_t count[ITEMS] = {};
+  const auto add = [&](int c, uint32_t equal) {          // equal: 1 where equal keys count too
+    const uint4 v = sm[c * 32 + lane];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+      const uint32_t below = me[k] + equal;
+      count[k] += (v.x < below) + (v.y < below) + (v.z < below) + (v.w < below);
+    }
+  };
+  const int own = i0 / 128;
+#pragma unroll 4
+  for (int c = 0; c < own; ++c) add(c, 1u);
+#pragma unroll 4
+  for (int c = own + 1; c < chunks; ++c) add(c, 0u);
+  {
+    const uint4 v = sm[own * 32 + lane];
+    const uint32_t key[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) count[k] += key[j] < me[k] + (own * 128 + lane * 4 + j < i0 + k ? 1u : 0u);
+  }
+#pragma unroll
+  for (int k = 0; k < ITEMS; ++k) {
+    count[k] = __reduce_add_sync(0xffffffffu, count[k]);
+    if (lane == k && i0 + k < n) {
+      ids[count[k]] = me[k];
+      order[count[k]] = i0 + k;
+    }
+  }
+}
 
 // ----------------------------------------------------------------------------- sums
 constexpr int EW_THREADS = 128;
@@ -490,18 +533,14 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return 7;
   if (!configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         ES_WARPS * ES_BINS * 2 + 2 * ES_PER_BLOCK * 8);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(embedding_sort_small_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               ES_WARPS * ES_BINS * 2 + 2 * ES_ALONE * 8);
+    const cudaError_t e = cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               ES_WARPS * ES_BINS * 2 + 2 * ES_PER_BLOCK * 8);
     if (e != cudaSuccess) return 1000 + static_cast<int>(e);
     configured[dev] = true;
   }
   for (long at = 0; at < ntok; at += ES_MOST) {
     const int n = static_cast<int>(ntok - at < ES_MOST ? ntok - at : ES_MOST);
-    const bool alone = n <= ES_ALONE;
-    const int blocks = alone ? 1 : ES_BLOCKS, per = ((n + blocks - 1) / blocks + 31) / 32 * 32;
+    const int per = ((n + ES_BLOCKS - 1) / ES_BLOCKS + 31) / 32 * 32;
     const long list = (4L * n + 255) / 256 * 256;
     EmbeddingSum s;
     uint8_t* base = static_cast<uint8_t*>(work);
@@ -519,9 +558,14 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
     s.H = H;
     s.rows = static_cast<uint32_t>(rows);
     s.scale = scale;
-    const auto sort = alone ? embedding_sort_small_kernel : embedding_sort_kernel;
-    KB_LAUNCH_PDL(sort, blocks, ES_THREADS, ES_WARPS * ES_BINS * 2 + 2 * per * 8, stream, tokens + at, n, per, first, rows,
-                  passes, bits, ids, order);
+    if (n <= ER_MOST) {
+      const int items = n <= ER_TWO ? 2 : 1, per_block = ER_THREADS / 32 * items;
+      KB_LAUNCH_PDL((items == 2 ? embedding_rank_kernel<2> : embedding_rank_kernel<1>), (n + per_block - 1) / per_block, ER_THREADS,
+                    (n + 127) / 128 * 512, stream, tokens + at, n, first, rows, ids, order);
+    } else {
+      KB_LAUNCH_PDL(embedding_sort_kernel, ES_BLOCKS, ES_THREADS, ES_WARPS * ES_BINS * 2 + 2 * per * 8, stream, tokens + at, n, per, first,
+                    rows, passes, bits, ids, order);
+    }
     KB_LAUNCH_PDL((vec ? embedding_window_kernel<true> : embedding_window_kernel<false>), dim3(windows, (H + EW_COLS - 1) / EW_COLS),
                   EW_THREADS, 0, stream, s);
     KB_LAUNCH_PDL((vec ? embedding_join_kernel<true> : embedding_join_kernel<false>),

@@ -225,3 +225,12 @@ def test_gpu_refusals():
 def test_widest_table():
     """A table whose columns the last kernel's grid does not reach is refused before the first one has added to it."""
     assert lib().kb_embedding_bwd_sorted(16, 16, 16, 4, 65535 * 128 + 1, 0, 4, 1.0, 256, 0) == 7
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 2, 3, 127, 128, 129, 1023, 1024, 1025, 2047, 2048, 2049, 4095, 4096, 4097, 65535, 65537])
+@pytest.mark.parametrize("v", [1, 40, 100000])
+def test_borders_of_the_sorts(n, v):
+    """Batches at the sizes where the way of sorting, or of counting, changes; few tokens and many, half of them another shard's."""
+    check(draw(n, v, seed=6), table(v, 24), 0, 1.0)
+    check(draw(n, 2 * v, seed=7), table(v, 24), v, 1.0)
