@@ -14,6 +14,8 @@
 //      the part that goes on after it.
 //   3. Such tokens are put together from their partial sums, in order.
 //
+// Up to 1024 tokens take one kernel for all of it, further below.
+//
 // The order of additions depends on the tokens alone, so the same inputs give the same bits.  Sums are fp32.
 //
 // What bounds it: memory for the lookup and the sums, latency for the sort and the join.  One B200, us: 8192 x 4096 into 128256 rows
@@ -216,15 +218,12 @@ embedding_sort_kernel(const long* __restrict__ tokens, int n, int per, long firs
 }
 
 // The same for small batches, by counting: the place of a token is the number of smaller ones and of equal ones before it.  A block
-// holds all keys, a warp counts for ITEMS consecutive tokens, 128 keys at a time.  What a radix pass takes are its many steps; here is
-// one, of n^2 comparisons, over as many blocks as there are.
-// One B200, us of the gradient of n x 2048, by a cluster / by counting: 64 11.4 / 5.4, 512 12.6 / 7.8, 2048 18.6 / 14.6, 3000 22.0 / 19.0,
-// 4096 24.9 / 23.9; with one token a warp and with two: 512 9.8 / 7.8, 1000 11.5 / 11.5, 1500 14.0 / 15.0, 3000 19.0 / 21.3.
+// holds all keys, a warp counts for one token, 128 keys at a time.  What a radix pass takes are its many steps; here is one, of n^2
+// comparisons, over as many blocks as there are.  One B200, us of the gradient of n x 2048, by a cluster / by counting:
+// 1500 18.2 / 14.0, 2048 18.6 / 14.6, 3000 22.0 / 19.0, 4096 24.9 / 23.9.
 constexpr int ER_MOST = 4096;                  // tokens
-constexpr int ER_TWO = 1024;                   // up to here a warp counts for two
 constexpr int ER_THREADS = 256;
 
-template <int ITEMS>
 __global__ void __launch_bounds__(ER_THREADS)
 embedding_rank_kernel(const long* __restrict__ tokens, int n, long first, long rows, uint32_t* __restrict__ ids,
                       uint32_t* __restrict__ order) {
@@ -238,40 +237,27 @@ embedding_rank_kernel(const long* __restrict__ tokens, int n, long first, long r
     keys[i] = i < n ? static_cast<uint32_t>(id >= 0 && id < rows ? id : rows) : 0xffffffffu;
   }
   __syncthreads();
-  const int i0 = (blockIdx.x * (ER_THREADS / 32) + (threadIdx.x >> 5)) * ITEMS;
-  if (i0 >= n) return;
-  uint32_t me[ITEMS];
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) me[k] = keys[i0 + k];
-  uint32_t count[ITEMS] = {};
-  const auto add = [&](int c, uint32_t equal) {          // equal: 1 where equal keys count too
+  const int item = blockIdx.x * (ER_THREADS / 32) + (threadIdx.x >> 5);
+  if (item >= n) return;
+  const uint32_t me = keys[item];
+  uint32_t count = 0;
+  const auto add = [&](int c, uint32_t below) {
     const uint4 v = sm[c * 32 + lane];
-#pragma unroll
-    for (int k = 0; k < ITEMS; ++k) {
-      const uint32_t below = me[k] + equal;
-      count[k] += (v.x < below) + (v.y < below) + (v.z < below) + (v.w < below);
-    }
+    count += (v.x < below) + (v.y < below) + (v.z < below) + (v.w < below);
   };
-  const int own = i0 / 128;
+  const int own = item / 128;
 #pragma unroll 4
-  for (int c = 0; c < own; ++c) add(c, 1u);
+  for (int c = 0; c < own; ++c) add(c, me + 1);           // equal keys count too
 #pragma unroll 4
-  for (int c = own + 1; c < chunks; ++c) add(c, 0u);
-  {
-    const uint4 v = sm[own * 32 + lane];
-    const uint32_t key[4] = {v.x, v.y, v.z, v.w};
+  for (int c = own + 1; c < chunks; ++c) add(c, me);
+  const uint4 v = sm[own * 32 + lane];
+  const uint32_t key[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int k = 0; k < ITEMS; ++k)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) count[k] += key[j] < me[k] + (own * 128 + lane * 4 + j < i0 + k ? 1u : 0u);
-  }
-#pragma unroll
-  for (int k = 0; k < ITEMS; ++k) {
-    count[k] = __reduce_add_sync(0xffffffffu, count[k]);
-    if (lane == k && i0 + k < n) {
-      ids[count[k]] = me[k];
-      order[count[k]] = i0 + k;
-    }
+  for (int j = 0; j < 4; ++j) count += key[j] < me + (own * 128 + lane * 4 + j < item ? 1u : 0u);
+  count = __reduce_add_sync(0xffffffffu, count);
+  if (lane == 0) {
+    ids[count] = me;
+    order[count] = item;
   }
 }
 
@@ -315,6 +301,25 @@ __device__ __forceinline__ void store_sums(float* dst, const float (&v)[8], int 
   }
 }
 
+// Eight columns of a row of gradients, and their addition to sums.
+template <bool VEC>
+__device__ __forceinline__ uint4 load_row(const __nv_bfloat16* src, int left) {
+  if constexpr (VEC) return __ldcs(reinterpret_cast<const uint4*>(src));
+  uint32_t q[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (k < left) q[k >> 1] |= static_cast<uint32_t>(__bfloat16_as_ushort(src[k])) << (k & 1 ? 16 : 0);
+  return make_uint4(q[0], q[1], q[2], q[3]);
+}
+__device__ __forceinline__ void add_row(float (&acc)[8], uint4 v) {
+  const uint32_t q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    acc[2 * k] += __uint_as_float(q[k] << 16);
+    acc[2 * k + 1] += __uint_as_float(q[k] & 0xffff0000u);
+  }
+}
+
 template <bool VEC>
 __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const EmbeddingSum p) {
   __shared__ uint32_t id[EW_MOST + 2], pos[EW_MOST];      // id[0]: the position before the window
@@ -342,15 +347,7 @@ __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const Embe
       v[j] = make_uint4(0u, 0u, 0u, 0u);
       const uint32_t me = b + j < len ? id[1 + b + j] : NONE;
       if (me < p.rows) {
-        const __nv_bfloat16* src = p.dout + static_cast<size_t>(pos[b + j]) * p.H + col;
-        if constexpr (VEC) {
-          v[j] = __ldcs(reinterpret_cast<const uint4*>(src));
-        } else {
-          uint32_t* q = reinterpret_cast<uint32_t*>(&v[j]);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (k < left) q[k >> 1] |= static_cast<uint32_t>(__bfloat16_as_ushort(src[k])) << (k & 1 ? 16 : 0);
-        }
+        v[j] = load_row<VEC>(p.dout + static_cast<size_t>(pos[b + j]) * p.H + col, left);
         const bool ends = id[2 + b + j] != me;
         if (ends && starts) load_sums<VEC>(p.grad + static_cast<size_t>(me) * p.H + col, old[j], left);
         if (ends) starts = true;
@@ -360,12 +357,7 @@ __global__ void __launch_bounds__(EW_THREADS) embedding_window_kernel(const Embe
     for (int j = 0; j < EW_BATCH; ++j) {
       const uint32_t me = b + j < len ? id[1 + b + j] : NONE;
       if (me < p.rows) {
-        const uint32_t q[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          acc[2 * k] += __uint_as_float(q[k] << 16);
-          acc[2 * k + 1] += __uint_as_float(q[k] & 0xffff0000u);
-        }
+        add_row(acc, v[j]);
         const bool last = b + j == len - 1, ends = id[2 + b + j] != me;
         if (last || ends) {
           float* dst;
@@ -482,6 +474,112 @@ __global__ void __launch_bounds__(EC_THREADS) embedding_join_kernel(const Embedd
   }
 }
 
+// ----------------------------------------------------------------------------- few tokens
+// The whole gradient of a small batch in one launch.  A block for each token lists the positions that hold it.  Up to EW_BATCH of them
+// are summed by the block of the first, groups of threads with columns of their own.  A longer run is spread over the blocks of its
+// tokens by columns, and in a block over groups of threads by rows, whose sums are added in order.
+//
+// What bounds it: latency, of the tokens and then of a few rows.  One B200, us of the gradient of n x 2048, sorted by counting / so: 64
+// tokens 5.2 / 2.5, 512 10.4 / 4.4, nine tenths of them one token 9.9 / 5.3, 1024 12.2 / 7.9; 2048 14.6 / 15.5, since every block goes
+// through all tokens.
+constexpr int EF_MOST = 1024;                  // tokens
+constexpr int EF_THREADS = 256;
+constexpr int EF_COLS = 512;                   // of a group, short runs
+constexpr int EF_LONG_COLS = 128;              // of a block, long runs
+constexpr int EF_GROUPS = EF_THREADS / (EF_COLS / 8), EF_LONG_GROUPS = EF_THREADS / (EF_LONG_COLS / 8);
+
+template <bool VEC>
+__global__ void __launch_bounds__(EF_THREADS)
+embedding_few_kernel(const long* __restrict__ tokens, const __nv_bfloat16* __restrict__ dout, float* __restrict__ grad, int n, int H,
+                     long first, long rows, float scale) {
+  constexpr int TURNS = EF_MOST / EF_THREADS, WARPS = EF_THREADS / 32;
+  __shared__ uint16_t at[EF_MOST];             // the token's positions
+  static_assert(TURNS * WARPS == 32, "a count a lane");
+  __shared__ int found[32];                    // in each 32 positions
+  __shared__ int place;                        // of this block's token among them
+  __shared__ __align__(16) float part[EF_LONG_GROUPS - 1][EF_LONG_COLS];
+  pdl_begin();
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const long me = tokens[t] - first;
+  if (me < 0 || me >= rows) return;
+  uint32_t same[TURNS];                        // lanes of this warp that hold the token
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    const int i = k * EF_THREADS + tid;
+    same[k] = k * EF_THREADS < n ? __ballot_sync(0xffffffffu, i < n && tokens[i] - first == me) : 0u;
+    if (lane == 0) found[k * WARPS + warp] = __popc(same[k]);
+  }
+  __syncthreads();
+  const int mine = found[lane];
+  int before = mine;                           // in the positions before the lane's 32
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    const int o = __shfl_up_sync(0xffffffffu, before, i);
+    if (lane >= i) before += o;
+  }
+  const int len = __shfl_sync(0xffffffffu, before, 31);
+  before -= mine;
+#pragma unroll
+  for (int k = 0; k < TURNS; ++k) {
+    if (k * EF_THREADS >= n) break;
+    const int p = __shfl_sync(0xffffffffu, before, k * WARPS + warp) + __popc(same[k] & ((1u << lane) - 1)), i = k * EF_THREADS + tid;
+    if (same[k] >> lane & 1u) {
+      at[p] = static_cast<uint16_t>(i);
+      if (i == t) place = p;
+    }
+  }
+  __syncthreads();
+  const auto sum = [&](int col, int from, int to, float (&acc)[8]) {
+    for (int b = from; b < to; b += EW_BATCH) {
+      uint4 v[EW_BATCH];
+#pragma unroll
+      for (int j = 0; j < EW_BATCH; ++j)
+        v[j] = b + j < to ? load_row<VEC>(dout + static_cast<size_t>(at[b + j]) * H + col, H - col) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int j = 0; j < EW_BATCH; ++j)
+        if (b + j < to) add_row(acc, v[j]);
+    }
+  };
+  float* const row = grad + me * H;
+  const auto finish = [&](int col, float (&acc)[8], const float (&old)[8]) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = fmaf(acc[k], scale, old[k]);
+    store_sums<VEC>(row + col, acc, H - col);
+  };
+  if (len <= EW_BATCH) {
+    if (place) return;
+    const int group = tid / (EF_COLS / 8), c = tid % (EF_COLS / 8) * 8;
+    for (int col = (blockIdx.y + gridDim.y * group) * EF_COLS + c; col < H; col += gridDim.y * EF_GROUPS * EF_COLS) {
+      float acc[8] = {}, old[8];
+      load_sums<VEC>(row + col, old, H - col);
+      sum(col, 0, len, acc);
+      finish(col, acc, old);
+    }
+    return;
+  }
+  const int group = tid / (EF_LONG_COLS / 8), c = tid % (EF_LONG_COLS / 8) * 8;
+  const int share = (len + EF_LONG_GROUPS - 1) / EF_LONG_GROUPS, from = group * share, to = min(len, from + share);
+  for (int col0 = (place * gridDim.y + blockIdx.y) * EF_LONG_COLS; col0 < H; col0 += len * gridDim.y * EF_LONG_COLS) {
+    const int col = col0 + c;
+    float acc[8] = {}, old[8];
+    if (group == 0 && col < H) load_sums<VEC>(row + col, old, H - col);
+    if (col < H) sum(col, from, to, acc);
+    if (group > 0) store_sums<true>(&part[group - 1][c], acc, 8);
+    __syncthreads();
+    if (group == 0 && col < H) {
+#pragma unroll
+      for (int g = 0; g < EF_LONG_GROUPS - 1; ++g) {
+        float more[8];
+        load_sums<true>(&part[g][c], more, 8);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] += more[k];
+      }
+      finish(col, acc, old);
+    }
+    __syncthreads();                           // the sums have been read
+  }
+}
+
 // ----------------------------------------------------------------------------- host side
 // Sorted positions per block of the sums: 64, fewer where that would be less than 512 windows, whose blocks wait for memory side by
 // side.  More windows leave a frequent token in more parts to be joined.  One B200, us, 8192 x 5120: 64 positions 97, 32 86, 16 83,
@@ -493,6 +591,7 @@ static int sum_window(long n) {
   return w;
 }
 static long chunk_bytes(long n, int H) {
+  if (n <= EF_MOST) return 0;                  // nothing is kept
   const long windows = (n + sum_window(n) - 1) / sum_window(n);
   return (4L * n + 255) / 256 * 256 * 2 + 2L * windows * H * 4;
 }
@@ -511,11 +610,16 @@ extern "C" int kb_embedding_fwd(const long* tokens, const void* w, void* out, lo
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }
 
-// Bytes of workspace (256-byte aligned) of the call below.
+// Bytes of workspace (256-byte aligned) of the call below; 0: it takes none.
 extern "C" long kb_embedding_sorted_bytes(long ntok, int H) {
   if (ntok <= 0 || H <= 0) return 0;
   const long whole = kb::chunk_bytes(kb::ES_MOST, H), rest = kb::chunk_bytes(ntok % kb::ES_MOST ? ntok % kb::ES_MOST : kb::ES_MOST, H);
   return ntok > kb::ES_MOST && whole > rest ? whole : rest;
+}
+// Kernels that it launches.
+extern "C" int kb_embedding_sorted_launches(long ntok) {
+  const long rest = ntok % kb::ES_MOST;
+  return static_cast<int>(ntok / kb::ES_MOST * 3 + (rest == 0 ? 0 : rest <= kb::EF_MOST ? 1 : 3));
 }
 // grad [rows, H] (fp32) += scale * the rows of dout ([ntok, H] bf16) at the tokens' rows; tokens outside first .. first + rows - 1
 // are left out.  Batches beyond 65536 tokens are taken in chunks of that many.
@@ -523,7 +627,9 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
                                        float scale, void* work, cudaStream_t stream) {
   using namespace kb;
   constexpr int MOST = 65535 * EC_COLS;         // columns, one row of blocks for each EC_COLS of them
-  if (ntok <= 0 || H <= 0 || H > MOST || rows <= 0 || rows >= 1L << 31 || !work || reinterpret_cast<uintptr_t>(work) % 256) return 7;
+  if (ntok <= 0 || H <= 0 || H > MOST || rows <= 0 || rows >= 1L << 31 || reinterpret_cast<uintptr_t>(work) % 256 ||
+      (!work && ntok > EF_MOST))
+    return 7;
   const bool vec = H % 8 == 0 && reinterpret_cast<uintptr_t>(dout) % 16 == 0 && reinterpret_cast<uintptr_t>(grad) % 16 == 0;
   int bits_all = 1;
   while ((rows - 1) >> bits_all) ++bits_all;              // keys 0 .. rows - 1
@@ -540,6 +646,13 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
   }
   for (long at = 0; at < ntok; at += ES_MOST) {
     const int n = static_cast<int>(ntok - at < ES_MOST ? ntok - at : ES_MOST);
+    if (n <= EF_MOST) {
+      // blocks of a token: two per SM in all (with four, 64 x 8192 takes 3.9 us instead of 3.1, with eight 4.9)
+      const int strips = (H + EF_COLS - 1) / EF_COLS, most = 2 * device_sm_count() / n;
+      KB_LAUNCH_PDL((vec ? embedding_few_kernel<true> : embedding_few_kernel<false>), dim3(n, strips < most ? strips : most < 1 ? 1 : most),
+                    EF_THREADS, 0, stream, tokens + at, static_cast<const __nv_bfloat16*>(dout) + at * H, grad, n, H, first, rows, scale);
+      continue;
+    }
     const int per = ((n + ES_BLOCKS - 1) / ES_BLOCKS + 31) / 32 * 32;
     const long list = (4L * n + 255) / 256 * 256;
     EmbeddingSum s;
@@ -559,9 +672,9 @@ extern "C" int kb_embedding_bwd_sorted(const long* tokens, const void* dout, flo
     s.rows = static_cast<uint32_t>(rows);
     s.scale = scale;
     if (n <= ER_MOST) {
-      const int items = n <= ER_TWO ? 2 : 1, per_block = ER_THREADS / 32 * items;
-      KB_LAUNCH_PDL((items == 2 ? embedding_rank_kernel<2> : embedding_rank_kernel<1>), (n + per_block - 1) / per_block, ER_THREADS,
-                    (n + 127) / 128 * 512, stream, tokens + at, n, first, rows, ids, order);
+      constexpr int ITEMS = ER_THREADS / 32;
+      KB_LAUNCH_PDL(embedding_rank_kernel, (n + ITEMS - 1) / ITEMS, ER_THREADS, (n + 127) / 128 * 512, stream, tokens + at, n, first,
+                    rows, ids, order);
     } else {
       KB_LAUNCH_PDL(embedding_sort_kernel, ES_BLOCKS, ES_THREADS, ES_WARPS * ES_BINS * 2 + 2 * per * 8, stream, tokens + at, n, per, first,
                     rows, passes, bits, ids, order);

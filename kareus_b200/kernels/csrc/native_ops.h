@@ -16,6 +16,7 @@ int kb_newton_schulz(const void* x, int bf16, int batch, int m, int n, float a, 
 int kb_embedding_fwd(const long* tokens, const void* w, void* out, long ntok, int H, long first, long rows, float scale,
                             cudaStream_t stream);
 long kb_embedding_sorted_bytes(long ntok, int H);
+int kb_embedding_sorted_launches(long ntok);
 int kb_embedding_bwd_sorted(const long* tokens, const void* dout, float* grad, long ntok, int H, long first, long rows, float scale,
                             void* work, cudaStream_t stream);
 }

@@ -188,25 +188,27 @@ PyObject* embedding_fwd(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// embedding_bwd_sorted(dout, tokens, grad, vocab_start, scale, launches)
+// embedding_bwd_sorted(dout, tokens, grad, vocab_start, scale)
 PyObject* embedding_bwd_sorted(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 6 || !PyLong_Check(args[3]) || !PyFloat_Check(args[4])) Py_RETURN_NONE;
+  if (nargs != 5 || !PyLong_Check(args[3]) || !PyFloat_Check(args[4])) Py_RETURN_NONE;
   const at::Tensor *d = plain(args[0], at::kBFloat16), *t = plain(args[1], at::kLong), *g = plain(args[2], at::kFloat);
   if (!d || !lookup(t, g) || d->device() != g->device() || !d->is_contiguous()) Py_RETURN_NONE;
   const int64_t H = g->size(1), rows = g->size(0), n = t->numel();
   if (d->dim() < 1 || d->size(-1) != H || d->numel() != n * H || rows > INT_MAX) Py_RETURN_NONE;
-  const long first = PyLong_AsLong(args[3]), launches = PyLong_AsLong(args[5]);
+  const long first = PyLong_AsLong(args[3]);
   if (PyErr_Occurred()) return nullptr;
   const double scale = PyFloat_AS_DOUBLE(args[4]);
-  at::Tensor work = at::empty({kb_embedding_sorted_bytes(n, H)}, g->options().dtype(at::kByte).requires_grad(false));
+  const long bytes = kb_embedding_sorted_bytes(n, H);
+  at::Tensor work;
+  if (bytes) work = at::empty({bytes}, g->options().dtype(at::kByte).requires_grad(false));
   const long* pt = reinterpret_cast<const long*>(t->data_ptr());
   const void* pd = d->data_ptr();
   float* pg = g->data_ptr<float>();
-  void* pw = work.data_ptr();
+  void* pw = bytes ? work.data_ptr() : nullptr;
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream().stream();
   const int rc = without_gil([&] { return kb_embedding_bwd_sorted(pt, pd, pg, n, H, first, rows, scale, pw, stream); });
-  if (!finish(rc, "embedding_bwd", launches)) return nullptr;
+  if (!finish(rc, "embedding_bwd", kb_embedding_sorted_launches(n))) return nullptr;
   Py_INCREF(args[2]);
   return args[2];
   END_HANDLE_TH_ERRORS

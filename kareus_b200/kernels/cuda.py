@@ -116,6 +116,8 @@ def _declare(L) -> None:
     L.kb_rmsnorm_bwd_scratch_elems.restype = c_long
     L.kb_embedding_sorted_bytes.argtypes = [LNG, I]
     L.kb_embedding_sorted_bytes.restype = c_long
+    L.kb_embedding_sorted_launches.argtypes = [LNG]
+    L.kb_embedding_sorted_launches.restype = c_int
     L.kb_newton_schulz_bytes.argtypes = [LNG, LNG, LNG]
     L.kb_newton_schulz_bytes.restype = c_long
     L.kb_gemm_row_stats_floats.argtypes = [I, I, I]
@@ -750,7 +752,7 @@ def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"
     if order == "sorted":
         from . import _OPS
         if _OPS is not None:
-            r = _OPS.embedding_bwd_sorted(dout, tokens, grad_weight, vocab_start, scale, 3 * -(-tokens.numel() // EMBEDDING_CHUNK))
+            r = _OPS.embedding_bwd_sorted(dout, tokens, grad_weight, vocab_start, scale)
             if r is not None:
                 return r
     if not _bf16(dout) or grad_weight.dtype != torch.float32:
@@ -769,7 +771,7 @@ def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"
         work = torch.empty(L.kb_embedding_sorted_bytes(n, H), dtype=torch.uint8, device=dout.device)
         _check(L.kb_embedding_bwd_sorted(tokens.data_ptr(), dout.data_ptr(), grad_weight.data_ptr(), n, H, int(vocab_start),
                                          grad_weight.shape[0], float(scale), work.data_ptr(), _stream()), "embedding_bwd")
-        _count(3 * -(-n // EMBEDDING_CHUNK))
+        _count(L.kb_embedding_sorted_launches(n))
     else:
         _check(L.kb_embedding_bwd(tokens.data_ptr(), dout.data_ptr(), grad_weight.data_ptr(), n, H,
                                   int(vocab_start), grad_weight.shape[0], _stream()), "embedding_bwd")
@@ -778,7 +780,6 @@ def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"
 
 
 EMBEDDING_ORDERS = ("any", "sorted")
-EMBEDDING_CHUNK = 65536       # tokens that csrc/embedding_sorted.cu sorts at once
 
 
 def _embedding_args(what, tokens, table, *more):

@@ -234,3 +234,27 @@ def test_borders_of_the_sorts(n, v):
     """Batches at the sizes where the way of sorting, or of counting, changes; few tokens and many, half of them another shard's."""
     check(draw(n, v, seed=6), table(v, 24), 0, 1.0)
     check(draw(n, 2 * v, seed=7), table(v, 24), v, 1.0)
+
+
+@gpu
+@pytest.mark.parametrize("H", [1000, 4104, 8191, 20000])
+@pytest.mark.parametrize("n", [5, 9, 300, 1024])
+def test_few_tokens_of_wide_rows(n, H):
+    """Short runs and long ones, whose columns are spread over the blocks of their tokens."""
+    t = draw(n, 60, seed=8)
+    t[: n // 2] = 7
+    t = t[torch.randperm(n, generator=torch.Generator().manual_seed(4)).to(t.device)]
+    check(t, table(40, H), 0, 1.0)
+    check(torch.full((n,), 3, device="cuda"), table(9, H), 2, 0.5)
+
+
+@gpu
+def test_launches_are_counted():
+    from kareus_b200.kernels import launch_count
+    g = torch.zeros(9, 16, device="cuda")
+    for n, launches in ((1024, 1), (1025, 3), (65536, 3), (65537, 4)):
+        d, t = torch.zeros(n, 16, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.int64, device="cuda")
+        for _ in range(2):                                         # the first call goes through the Python statements
+            before = launch_count()
+            K.embedding_bwd(d, t, g, 0, order="sorted")
+            assert launch_count() - before == launches
