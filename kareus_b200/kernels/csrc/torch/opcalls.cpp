@@ -12,14 +12,20 @@ constexpr int64_t FP8_MOST = (int64_t(1) << 31) - 512;     // rows and columns t
 bool current(const at::Tensor& t) { return t.device().index() == c10::cuda::getCurrentCUDAStream().device_index(); }
 bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 
-// Bytes whose rows start on 16, as the kernels read them.
-at::Tensor fp8_rows(int64_t rows, int64_t cols, int fmt, const at::TensorOptions& o) {
-  const int64_t ld = (cols + 15) / 16 * 16;
-  at::Tensor t = at::empty({rows, ld}, o.dtype(FP8[fmt]));
-  return ld == cols ? t : t.as_strided({rows, cols}, {ld, 1});
+// A tensor of part of a storage; without the dispatcher, which takes three times as long as the allocation behind it.
+at::Tensor part(const at::Tensor& base, at::ScalarType type, int64_t offset, c10::IntArrayRef sizes, c10::IntArrayRef strides) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+                                                          c10::scalarTypeToTypeMeta(type));
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides, offset);
+  return t;
 }
-at::Tensor fp8_scales(int64_t rows, int64_t cols, const at::TensorOptions& o) {
-  return at::empty({(rows + 127) / 128, ((cols + 127) / 128 + 3) / 4, 32, 4, 4}, o.dtype(at::kByte));
+// Data and scales of a matrix in one allocation.  Rows start on 16 bytes, as the kernels read them.
+void fp8_matrix(int64_t rows, int64_t cols, int fmt, const at::TensorOptions& o, at::Tensor& data, at::Tensor& scales) {
+  const int64_t ld = (cols + 15) / 16 * 16, blocks = (rows + 127) / 128, groups = ((cols + 127) / 128 + 3) / 4;
+  const int64_t behind = (rows * ld + 511) / 512 * 512;
+  const at::Tensor base = at::empty({behind + blocks * groups * 512}, o.dtype(at::kByte));
+  data = part(base, FP8[fmt], 0, {rows, cols}, {ld, 1});
+  scales = part(base, at::kByte, behind, {blocks, groups, 32, 4, 4}, {groups * 512, 512, 16, 4, 1});
 }
 
 // fp8_quantize(x, rows, cols, square, format) -> (data, scales, data of the transpose, its scales), None for what is not wanted
@@ -37,14 +43,8 @@ PyObject* fp8_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if ((x->stride(1) != 1 && N > 1) || ld < N) Py_RETURN_NONE;
   const auto o = x->options().requires_grad(false);
   at::Tensor t[4];
-  if (rows) {
-    t[0] = fp8_rows(M, N, fmt, o);
-    t[1] = fp8_scales(M, N, o);
-  }
-  if (cols) {
-    t[2] = fp8_rows(N, M, fmt, o);
-    t[3] = fp8_scales(N, M, o);
-  }
+  if (rows) fp8_matrix(M, N, fmt, o, t[0], t[1]);
+  if (cols) fp8_matrix(N, M, fmt, o, t[2], t[3]);
   void* p[4];
   for (int i = 0; i < 4; ++i) p[i] = t[i].defined() ? t[i].data_ptr() : nullptr;
   const void* px = x->data_ptr();

@@ -351,3 +351,34 @@ def test_largest_sizes():
         assert L.kb_fp8_quantize(16, rows, cols, cols, 16, 2 ** 31, 16, 16, 2 ** 31, 16, 0, 0, 0) == 7
     for m, n, k in ((2 ** 31 - 511, 8, 16), (8, 2 ** 31 - 1, 16), (8, 8, 2 ** 31 - 511)):
         assert L.kb_gemm_fp8(16, 16, 0, 2 ** 31, 16, 16, 0, 2 ** 31, 16, 2 ** 31, m, n, k, 0, 0, 0, 0) == 7
+
+
+@gpu
+def test_results_as_tensors():
+    """What the native call returns behaves like any tensor: views, inference mode, autograd's saving, storage of its own."""
+    x = sample(200, 136, "cuda")
+    K.fp8_quantize(x)                                              # the native call takes over from here
+    (r, c), (want, _) = K.fp8_quantize(x, cols=True), K.fp8_quantize(x.cpu())
+    assert r.data.storage_offset() == 0 and r.data.untyped_storage().data_ptr() != c.data.untyped_storage().data_ptr()
+    assert r.scales.is_contiguous() and not r.data.requires_grad and r.data.device == x.device
+    assert torch.equal(r.data.cpu().view(torch.uint8), want.data.view(torch.uint8)) and torch.equal(r.scales.clone().cpu(), want.scales)
+    with torch.inference_mode():
+        y, (inside, _) = x + 0, K.fp8_quantize(x)
+        assert inside.data.is_inference() and torch.equal(inside.scales, r.scales)
+    outside, _ = K.fp8_quantize(y)                                 # an inference tensor as input, its result is none
+    assert not outside.data.is_inference()
+
+    class Keep(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, t):
+            ctx.save_for_backward(outside.data, outside.scales)
+            return t * 2
+
+        @staticmethod
+        def backward(ctx, d):
+            data, scales = ctx.saved_tensors
+            return d * Fp8Matrix(data, scales).dequantize().sum()
+
+    t = torch.ones(1, device="cuda", requires_grad=True)
+    Keep.apply(t).backward()
+    assert torch.equal(t.grad[0], outside.dequantize().sum())
