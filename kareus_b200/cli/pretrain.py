@@ -42,7 +42,8 @@ def main(argv=None) -> int:
                             ("nanobatch" if par.num_nanobatches > 1 else "megatron"))))
     argv2 = ["--method", method, "--model", model.name, "--tp", str(par.tp), "--cp", str(par.cp), "--pp", str(par.pp),
              "--mbs", str(train.micro_batch_size), "--gbs", str(train.global_batch_size), "--seq", str(train.seq_len),
-             "--steps", str(sw.max_steps), "--tp-comm", par.tp_comm, "--clock-mode", a.clock_mode, "--out", a.out]
+             "--steps", str(sw.max_steps), "--tp-comm", par.tp_comm, "--clock-mode", a.clock_mode, "--out", a.out,
+             "--optimizer", train.optimizer, "--muon-momentum", str(train.muon_momentum)]
     if sw.solution_path:
         argv2 += ["--scheds", sw.solution_path]
     if extra.get("freqs"):

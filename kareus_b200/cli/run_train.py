@@ -54,10 +54,12 @@ def main(argv=None) -> int:
                          "are then read in the per-microbatch (forward, backward) pair layout")
     ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"],
                     help="muon: orthogonalised momentum for the layers' weight matrices, AdamW for the rest (tp 1)")
-    ap.add_argument("--linear-precision", default="bf16", choices=["bf16", "fp8"],
-                    help="fp8: the layers' matrix products on 8-bit operands with block scales (tp_comm sp or allreduce)")
-    ap.add_argument("--fp8-grad", default="e4m3", choices=["e4m3", "e5m2"], help="8-bit format of the gradients")
-    ap.add_argument("--embedding-grad", default="any", choices=["any", "sorted"],
+    ap.add_argument("--muon-momentum", type=float, default=None, help="momentum of --optimizer muon (default 0.95)")
+    ap.add_argument("--linear-precision", default=None, choices=["bf16", "fp8"],
+                    help="fp8: the layers' matrix products on 8-bit operands with block scales (tp_comm sp or allreduce); "
+                         "default, as for the two below: what the model's configuration says")
+    ap.add_argument("--fp8-grad", default=None, choices=["e4m3", "e5m2"], help="8-bit format of the gradients")
+    ap.add_argument("--embedding-grad", default=None, choices=["any", "sorted"],
                     help="sorted: the embedding table's gradient is summed in the order of the tokens (the same bits every run)")
     ap.add_argument("--profile-start-step", type=int, default=None,
                     help="open the CUDA profiler capture range at this step (nsys --capture-range=cudaProfilerApi)")
@@ -102,9 +104,11 @@ def main(argv=None) -> int:
     par = ParallelConfig(tp=a.tp, cp=a.cp, pp=a.pp, dp=dp, num_nanobatches=nano, tp_comm=tp_comm,
                          comm_backend=a.comm_backend if cuda else "nccl", recompute=not a.no_recompute)
     mesh = Mesh(tp=a.tp, cp=a.cp, dp=dp, pp=a.pp)
-    cfg = get_model_config(a.model).replace(linear_precision=a.linear_precision, fp8_grad=a.fp8_grad, embedding_grad=a.embedding_grad)
+    given = {k: getattr(a, k) for k in ("linear_precision", "fp8_grad", "embedding_grad") if getattr(a, k) is not None}
+    cfg = get_model_config(a.model).replace(**given)
     tc = TrainConfig(micro_batch_size=a.mbs, global_batch_size=a.gbs, seq_len=a.seq,
-                     dtype="bf16" if cuda else "fp32", optimizer=a.optimizer)
+                     dtype="bf16" if cuda else "fp32", optimizer=a.optimizer,
+                     **({} if a.muon_momentum is None else {"muon_momentum": a.muon_momentum}))
     tag = f"cp{a.cp}_tp{a.tp}_mbs{a.mbs}_seq{a.seq}"
     out = Path(a.run_dir) if a.run_dir else Path(a.out) / a.model / tag / a.method
     out.mkdir(parents=True, exist_ok=True)

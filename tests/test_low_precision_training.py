@@ -268,6 +268,65 @@ trainer: {devices: 1}
     assert train.optimizer == "muon" and train.muon_momentum == 0.9
 
 
+YAML = """name: low_precision_yaml
+trainer: {devices: 1, max_steps: 2}
+model: {micro_batch_size: 2, global_batch_size: 4, encoder_seq_length: 32, num_layers: 2, hidden_size: 64, ffn_hidden_size: 128,
+        num_attention_heads: 4, num_query_groups: 2, vocab_size: 256, %s}
+"""
+
+
+def _built_trainers(monkeypatch):
+    """The trainers that a driver builds from here on."""
+    import kareus_b200.train.trainer as T
+    built = []
+
+    class Kept(T.Trainer):
+        def __init__(self, *a, **kw):
+            super().__init__(*a, **kw)
+            built.append(self)
+
+    monkeypatch.setattr(T, "Trainer", Kept)
+    return built
+
+
+def _settings(tr):
+    cls, layer = type(tr.optimizer).__name__, tr.model.decoder.layers[0]
+    return (cls, tr.cfg.muon_momentum, type(layer.qkv), type(layer.fc2), getattr(layer.fc1, "fp8_grad", None),
+            tr.model.embedding.grad_order, tr.model.embedding.scale)
+
+
+def test_yaml_settings_reach_the_trainer(tmp_path, monkeypatch):
+    """`pretrain` trains with what the run config says."""
+    from kareus_b200.cli import pretrain
+    from kareus_b200.config import MODEL_REGISTRY
+    from kareus_b200.ops.linear import RowParallelLinear
+    monkeypatch.setattr("kareus_b200.config.MODEL_REGISTRY", dict(MODEL_REGISTRY))
+    built = _built_trainers(monkeypatch)
+    low = "fp8: hybrid, embedding_grad: sorted, embedding_scale: 8.0, optim: {name: distributed_muon, momentum: 0.9}"
+    plain = "optim: {name: distributed_fused_adam}"
+    for keys in (low, plain):
+        (tmp_path / "c.yaml").write_text(YAML % keys)
+        assert pretrain.main(["--config", str(tmp_path / "c.yaml"), "--out", str(tmp_path / "exp")]) == 0
+    assert _settings(built[0]) == ("DistributedMuon", 0.9, Fp8ColumnParallelLinear, Fp8RowParallelLinear, "e5m2", "sorted", 8.0)
+    assert _settings(built[1]) == ("DistributedAdamW", 0.95, ColumnParallelLinear, RowParallelLinear, None, "any", 1.0)
+
+
+def test_flags_of_run_train_replace_only_what_they_name(tmp_path, monkeypatch):
+    from kareus_b200.cli import run_train
+    from kareus_b200.config import MODEL_REGISTRY
+    built = _built_trainers(monkeypatch)
+    low = get_model_config("tiny").replace(name="tiny_low", linear_precision="fp8", fp8_grad="e5m2", embedding_grad="sorted")
+    monkeypatch.setitem(MODEL_REGISTRY, "tiny_low", low)
+    args = ["--method", "nanobatch", "--model", "tiny_low", "--mbs", "2", "--gbs", "4", "--seq", "32", "--steps", "1", "--out", str(tmp_path)]
+    for flags, want in (([], ("fp8", "e5m2", "sorted")), (["--fp8-grad", "e4m3"], ("fp8", "e4m3", "sorted")),
+                        (["--linear-precision", "bf16", "--embedding-grad", "any"], ("bf16", "e5m2", "any"))):
+        assert run_train.main(args + flags) == 0
+        c = built[-1].model_cfg
+        assert (c.linear_precision, c.fp8_grad, c.embedding_grad) == want
+    assert run_train.main(args + ["--optimizer", "muon", "--muon-momentum", "0.8"]) == 0
+    assert _settings(built[-1])[:2] == ("DistributedMuon", 0.8)
+
+
 LOW = dict(linear_precision="fp8", embedding_scale=22.627416997969522, embedding_grad="sorted")
 
 
