@@ -64,6 +64,22 @@ def apply_overrides(cfg: dict, overrides: Iterable[str]) -> dict:
     return cfg
 
 
+def _fp8_settings(m: Dict[str, Any]) -> Dict[str, str]:
+    """``linear_precision`` and ``fp8_grad`` of a run config, which says ``fp8: e4m3`` or ``fp8: hybrid`` (gradients in e5m2), or ``fp8:
+    true`` with ``fp8_e4m3`` or ``fp8_hybrid`` (e4m3 where it has neither)."""
+    text = str(m.get("fp8") or "").lower()
+    if text in ("", "none", "false"):
+        return {}
+    if text == "true":
+        e4m3, hybrid = bool(m.get("fp8_e4m3")), bool(m.get("fp8_hybrid"))
+        if e4m3 and hybrid:
+            raise ValueError("model.fp8_e4m3 and model.fp8_hybrid exclude each other")
+        text = "hybrid" if hybrid else "e4m3"
+    if text not in ("e4m3", "hybrid"):
+        raise ValueError(f"bad model.fp8 {m['fp8']!r}: e4m3, hybrid, a truth value or null")
+    return {"linear_precision": "fp8", "fp8_grad": "e5m2" if text == "hybrid" else "e4m3"}
+
+
 def load_run_config(path, overrides: Iterable[str] = (), world_size: Optional[int] = None
                     ) -> Tuple[ModelConfig, ParallelConfig, TrainConfig, RunSwitches]:
     with open(path) as f:
@@ -87,9 +103,7 @@ def load_run_config(path, overrides: Iterable[str] = (), world_size: Optional[in
         tie_embeddings=bool(m.get("share_embeddings_and_output_weights", False)),
         max_seq_len=int(m.get("encoder_seq_length", 4096)), init_std=float(m.get("init_method_std", 0.02)),
         num_layers_in_first_pipeline_stage=m.get("num_layers_in_first_pipeline_stage"),
-        linear_precision="fp8" if m.get("fp8") else "bf16",                     # Megatron's `fp8: e4m3` or `fp8: hybrid`
-        fp8_grad="e5m2" if str(m.get("fp8")).lower() == "hybrid" else "e4m3",
-        embedding_scale=float(m.get("embedding_scale", 1.0)), embedding_grad=str(m.get("embedding_grad", "any")))
+        **_fp8_settings(m), embedding_scale=float(m.get("embedding_scale", 1.0)), embedding_grad=str(m.get("embedding_grad", "any")))
     tp = int(m.get("tensor_model_parallel_size", 1))
     pp = int(m.get("pipeline_model_parallel_size", 1))
     cp = int(m.get("context_parallel_size", 1))

@@ -327,6 +327,28 @@ def test_flags_of_run_train_replace_only_what_they_name(tmp_path, monkeypatch):
     assert _settings(built[-1])[:2] == ("DistributedMuon", 0.8)
 
 
+@pytest.mark.parametrize("keys, want", [
+    ("fp8: e4m3", ("fp8", "e4m3")), ("fp8: E4M3", ("fp8", "e4m3")), ("fp8: hybrid", ("fp8", "e5m2")), ("fp8: Hybrid", ("fp8", "e5m2")),
+    ("fp8: true", ("fp8", "e4m3")), ("fp8: true, fp8_hybrid: true", ("fp8", "e5m2")), ("fp8: true, fp8_e4m3: true", ("fp8", "e4m3")),
+    ("fp8: true, fp8_e4m3: false, fp8_hybrid: true", ("fp8", "e5m2")), ("fp8: false, fp8_hybrid: true", ("bf16", "e4m3")),
+    ("fp8: null", ("bf16", "e4m3")), ("fp8: none", ("bf16", "e4m3")), ("fp8: None", ("bf16", "e4m3")), ("fp8: ''", ("bf16", "e4m3")),
+    ("fp8: 'false'", ("bf16", "e4m3")), ("fp8_hybrid: true", ("bf16", "e4m3"))])
+def test_yaml_fp8_values(tmp_path, keys, want):
+    """The string form of a run config (`fp8: e4m3 | hybrid`) and the one of truth values (`fp8: true` with `fp8_hybrid: true`)."""
+    from kareus_b200.config_yaml import load_run_config
+    (tmp_path / "c.yaml").write_text(YAML % keys)
+    model = load_run_config(tmp_path / "c.yaml")[0]
+    assert (model.linear_precision, model.fp8_grad) == want
+
+
+@pytest.mark.parametrize("keys", ["fp8: e5m2", "fp8: hybird", "fp8: 8", "fp8: true, fp8_e4m3: true, fp8_hybrid: true"])
+def test_yaml_fp8_refusals(tmp_path, keys):
+    from kareus_b200.config_yaml import load_run_config
+    (tmp_path / "c.yaml").write_text(YAML % keys)
+    with pytest.raises(ValueError, match="fp8"):
+        load_run_config(tmp_path / "c.yaml")
+
+
 LOW = dict(linear_precision="fp8", embedding_scale=22.627416997969522, embedding_grad="sorted")
 
 
