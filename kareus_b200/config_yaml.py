@@ -64,6 +64,12 @@ def apply_overrides(cfg: dict, overrides: Iterable[str]) -> dict:
     return cfg
 
 
+def _value(d: Dict[str, Any], key: str, default):
+    """A value of the default's type; the default where the key is missing or null."""
+    v = d.get(key)
+    return default if v is None else type(default)(v)
+
+
 def _fp8_settings(m: Dict[str, Any]) -> Dict[str, str]:
     """``linear_precision`` and ``fp8_grad`` of a run config, which says ``fp8: e4m3`` or ``fp8: hybrid`` (gradients in e5m2), or ``fp8:
     true`` with ``fp8_e4m3`` or ``fp8_hybrid`` (e4m3 where it has neither)."""
@@ -103,7 +109,7 @@ def load_run_config(path, overrides: Iterable[str] = (), world_size: Optional[in
         tie_embeddings=bool(m.get("share_embeddings_and_output_weights", False)),
         max_seq_len=int(m.get("encoder_seq_length", 4096)), init_std=float(m.get("init_method_std", 0.02)),
         num_layers_in_first_pipeline_stage=m.get("num_layers_in_first_pipeline_stage"),
-        **_fp8_settings(m), embedding_scale=float(m.get("embedding_scale", 1.0)), embedding_grad=str(m.get("embedding_grad", "any")))
+        **_fp8_settings(m), embedding_scale=_value(m, "embedding_scale", 1.0), embedding_grad=_value(m, "embedding_grad", "any"))
     tp = int(m.get("tensor_model_parallel_size", 1))
     pp = int(m.get("pipeline_model_parallel_size", 1))
     cp = int(m.get("context_parallel_size", 1))
@@ -121,7 +127,7 @@ def load_run_config(path, overrides: Iterable[str] = (), world_size: Optional[in
                         betas=(float(betas[0]), float(betas[1])), grad_clip=float(tr.get("gradient_clip_val", 1.0)),
                         warmup_steps=int(sched.get("warmup_steps", 500)), max_steps=int(tr.get("max_steps", 30)),
                         seed=int(m.get("seed", 1234)), optimizer="muon" if "muon" in str(opt.get("name", "")).lower() else "adamw",
-                        muon_momentum=float(opt.get("momentum", 0.95)),
+                        muon_momentum=_value(opt, "momentum", 0.95),
                         dtype={"bf16": "bf16", "bf16-mixed": "bf16", 16: "fp16", 32: "fp32"}.get(tr.get("precision", "bf16"), "bf16"))
     sw = RunSwitches(enable_zeus_monitor=bool(m.get("enable_zeus_monitor", False)),
                      enable_power_monitor=bool(m.get("enable_power_monitor", False)),

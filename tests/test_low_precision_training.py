@@ -349,6 +349,22 @@ def test_yaml_fp8_refusals(tmp_path, keys):
         load_run_config(tmp_path / "c.yaml")
 
 
+@pytest.mark.parametrize("keys", ["embedding_scale: null", "embedding_grad: null", "optim: {name: adam, momentum: null}"])
+def test_yaml_keys_without_a_value(tmp_path, keys):
+    """A key that is there without a value (an interpolation's target, say) is one that is not there."""
+    from kareus_b200.config_yaml import load_run_config
+    (tmp_path / "c.yaml").write_text(YAML % keys)
+    model, _, train, _ = load_run_config(tmp_path / "c.yaml")
+    assert (model.embedding_scale, model.embedding_grad, train.muon_momentum) == (1.0, "any", 0.95)
+
+
+def test_yaml_momentum_of_zero_stays(tmp_path):
+    from kareus_b200.config_yaml import load_run_config
+    (tmp_path / "c.yaml").write_text(YAML % "optim: {name: muon, momentum: 0}, embedding_scale: 0.5")
+    model, _, train, _ = load_run_config(tmp_path / "c.yaml")
+    assert train.muon_momentum == 0.0 and model.embedding_scale == 0.5
+
+
 LOW = dict(linear_precision="fp8", embedding_scale=22.627416997969522, embedding_grad="sorted")
 
 
