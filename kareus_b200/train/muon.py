@@ -151,7 +151,8 @@ class DistributedMuon(DistributedAdamW):
         return sd
 
     def load_state_dict(self, sd: dict) -> None:
-        if set(sd.get("muon", {})) != set(self._own):
+        own = sd.get("muon", {})              # a state of AdamW has none; neither has one of a single rank
+        if set(own) != set(self._own):
             raise ValueError("owners of the weight matrices differ from the checkpoint's")
         # the flat master buffer holds no current values of matrices with an owner: their weights stay (another rank's, which come
         # with the model) or follow from the owner's
@@ -159,7 +160,7 @@ class DistributedMuon(DistributedAdamW):
         super().load_state_dict(sd)
         for (off, rows, cols), w in zip(self.matrices, weights):
             self.param_flat[off:off + rows * cols].copy_(w)
-        for i, state in sd["muon"].items():
+        for i, state in own.items():
             off, rows, cols = self.matrices[i]
             for mine, theirs in zip(self._own[i], state):
                 mine.copy_(theirs)

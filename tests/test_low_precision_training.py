@@ -251,6 +251,35 @@ def test_muon_refuses_shards():
         DistributedMuon([q], TrainConfig(), [q])
 
 
+def _flat_state(opt):
+    return {k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in opt.state_dict().items()}
+
+
+def test_muon_takes_the_state_of_adamw():
+    """On one rank the flat buffers hold all of the state, and another optimizer's has no more to say than that."""
+    adamw, tc = _trainer(optimizer="adamw")
+    _steps(adamw, tc, 2)
+    sd = _flat_state(adamw.optimizer)
+    tr, _ = _trainer()
+    _steps(tr, tc, 1)
+    tr.optimizer.load_state_dict(sd)
+    opt = tr.optimizer
+    assert opt.step_count == 2 and torch.equal(opt.param_flat, adamw.optimizer.param_flat)
+    assert torch.equal(opt.m, sd["exp_avg"]) and torch.equal(opt.v, sd["exp_avg_sq"]) and torch.equal(opt.master, sd["master"])
+    assert all(l == l for l in _steps(tr, tc, 1))
+
+
+def test_muon_refuses_states_before_it_takes_any():
+    tr, tc = _trainer()
+    _steps(tr, tc, 1)
+    opt = tr.optimizer
+    before, params = _flat_state(opt), opt.param_flat.clone()
+    sd = {**_flat_state(opt), "step": 9, "muon": {0: (torch.zeros(4), torch.zeros(4))}}
+    with pytest.raises(ValueError, match="owners"):
+        opt.load_state_dict(sd)
+    assert opt.step_count == 1 and torch.equal(opt.param_flat, params) and torch.equal(opt.master, before["master"])
+
+
 # ----------------------------------------------------------------------------- all of them
 def test_drivers(tmp_path):
     from kareus_b200.cli import run_train
