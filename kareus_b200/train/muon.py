@@ -62,6 +62,7 @@ class DistributedMuon(DistributedAdamW):
                 if self.owner[i] == self.dp_rank:
                     w = self.param_flat[off:off + rows * cols]
                     self._own[i] = (torch.zeros(rows * cols, dtype=self.m.dtype, device=w.device), w.to(self.m.dtype).clone())
+        self._apart = set(self._own)
 
     def _state(self, i: int):
         """(momentum, master) of matrix ``i``, flat; the caller owns it."""

@@ -86,6 +86,7 @@ class DistributedAdamW:
             torch.empty(self.shard, dtype=acc, device=dev)
         self.step_count = 0
         self.last_grad_norm: Optional[torch.Tensor] = None
+        self._apart: set = set()              # numbers of the matrices that a subclass keeps state of outside the flat buffers
 
     # ------------------------------------------------------------------
     def zero_grad(self) -> None:
@@ -194,6 +195,8 @@ class DistributedAdamW:
     def load_state_dict(self, sd: dict) -> None:
         if tuple(sd["shard"]) != (self.lo, self.hi) or sd["total"] != self.total:
             raise ValueError("optimizer shard layout differs from the checkpoint")
+        if set(sd.get("muon", {})) - self._apart:
+            raise ValueError("the checkpoint's Muon matrices have masters and momentum apart from the flat buffers")
         self.step_count = int(sd["step"])
         self.master.copy_(sd["master"])
         self.m.copy_(sd["exp_avg"])

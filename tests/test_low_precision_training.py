@@ -280,6 +280,20 @@ def test_muon_refuses_states_before_it_takes_any():
     assert opt.step_count == 1 and torch.equal(opt.param_flat, params) and torch.equal(opt.master, before["master"])
 
 
+def test_adamw_refuses_what_muon_keeps_apart():
+    """Masters of matrices that have an owner are not in the flat buffer, which AdamW would take them from."""
+    tr, tc = _trainer(optimizer="adamw")
+    _steps(tr, tc, 1)
+    opt = tr.optimizer
+    params = opt.param_flat.clone()
+    sd = {**_flat_state(opt), "step": 9, "muon": {0: (torch.zeros(4), torch.zeros(4))}}
+    with pytest.raises(ValueError, match="Muon"):
+        opt.load_state_dict(sd)
+    assert opt.step_count == 1 and torch.equal(opt.param_flat, params)
+    opt.load_state_dict({**sd, "muon": {}})                        # Muon on one rank keeps nothing apart
+    assert opt.step_count == 9
+
+
 # ----------------------------------------------------------------------------- all of them
 def test_drivers(tmp_path):
     from kareus_b200.cli import run_train
