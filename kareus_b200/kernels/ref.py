@@ -337,8 +337,9 @@ def embedding_bwd(dout, tokens, grad_weight, vocab_start: int, scale: float = 1.
     if order == "sorted":
         at = torch.nonzero(inside).flatten()
         d = dout.reshape(-1, dout.shape[-1])[at].to(grad_weight.dtype)
-        grad_weight.index_put_((local[at],), d * scale, accumulate=True)      # adds by sorted index
-        return grad_weight
+        if grad_weight.is_cuda:
+            return grad_weight.index_put_((local[at],), d * scale, accumulate=True)      # adds by sorted index
+        return grad_weight.index_add_(0, local[at], d * scale)                # token after token; the call above adds with atomics here
     d = dout.reshape(-1, dout.shape[-1]).to(grad_weight.dtype) * inside.unsqueeze(-1).to(grad_weight.dtype)
     grad_weight.index_add_(0, local.clamp(0, v - 1), d if scale == 1.0 else d * scale)
     return grad_weight

@@ -258,3 +258,16 @@ def test_launches_are_counted():
             before = launch_count()
             K.embedding_bwd(d, t, g, 0, order="sorted")
             assert launch_count() - before == launches
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_statements_repeat_bit_for_bit(device, dtype):
+    """Also where PyTorch computes it: on the CPU, and fp32 gradients on the GPU.  Enough elements for several threads."""
+    t, d = draw(4000, 3, device=device), table(4000, 64, device).to(dtype)
+    runs = []
+    for _ in range(8):
+        g = torch.zeros(3, 64, device=device)
+        K.embedding_bwd(d, t, g, 0, scale=1.3, order="sorted")
+        runs.append(g)
+    assert all(torch.equal(r, runs[0]) for r in runs)
