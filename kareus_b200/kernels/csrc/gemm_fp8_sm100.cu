@@ -233,7 +233,7 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     constexpr int SLAB = OUT_F32 || NARROW ? 32 : 64;          // output columns of a slab, 64 bytes wide if NARROW, else 128
     constexpr int UNITS = NARROW ? 4 : 8, PER_UNIT = OUT_F32 ? 4 : 8;
     const int swizzle = NARROW ? (lane >> 1) & 3 : lane & 7;   // of the 16-byte units of this thread's row, as TMA expects
-    const int slabs = bn / SLAB, mine = (slabs - h + 1) >> 1;
+    const int slabs = bn / SLAB, mine = (slabs - h + 1) >> 1;  // mine >= 1: no tile has fewer than two slabs
     const uint32_t stg_row = smem_u32(stg) + lane * (UNITS * 16);
     // columns that this warp has read may be overwritten, if a tile comes that does
     const auto hand_over = [&](uint64_t* bar, bool awaited) {
@@ -315,7 +315,6 @@ gemm_fp8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
           tma_store_commit();
         }
       }
-      if (mine == 0) hand_over(&tempty[buf], t + 2 * step < tiles);     // no slab for this warp (narrow tile)
     }
     if (lane == 0) tma_store_wait_read<0>();          // nothing in flight out of shared memory at exit
   }
@@ -416,6 +415,7 @@ extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, c
   if ((rc = make_tmap(&tmSA, SA, 4, 2, da, str, box, 0))) return rc;
   if ((rc = make_tmap(&tmSB, SB, 4, 2, db, str, box, 0))) return rc;
   const uint32_t idesc = make_idesc_mxf8(G8_BM, bn, fmt_a, fmt_b);
+  // bn is a multiple of 64: two slabs of columns a tile at least, of 32 in fp32 and in the narrow form, of 64 in the other
   if (!out_f32 && bn == 64)
     return launch_fp8<false, false, true>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);
   if (!out_f32) return launch_fp8<false, false, false>(tmA, tmB, tmSA, tmSB, C, M, N, ldc, w, bn, idesc, pairs, status, stream);

@@ -278,7 +278,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
     // units are swizzled by row, as TMA expects rows of 64 or 128 bytes
     const auto swizzle = [](int r) { return NARROW ? (r >> 1) & 3 : r & 7; };
     uint8_t* const stg0 = smem + NS_RING + (warp - 2) * 8192;
-    const int slabs = bn / SLAB;
+    const int slabs = bn / SLAB;              // at least two, one for either set of warps
     constexpr bool ADDS = ns_adds(MODE), SYMMETRIC = ns_symmetric(MODE);
     uint4 v[UNITS];                           // the slab that is added, on its way
     float2 d_next = make_float2(0.f, 0.f);    // NS_UPDATE_T: P's diagonal for two of these columns, lane by lane
@@ -303,7 +303,7 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
         }
       }
     };
-    if (ADDS && first < units && h < slabs) fetch(first, h);
+    if (ADDS && first < units) fetch(first, h);
     uint32_t tile_i = 0, slab_i = 0;
     for (int u = first; u < units; u += step, ++tile_i) {
       int pair, z, tm, tn;
@@ -529,11 +529,6 @@ newton_schulz_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_const
             put(o2, &tmC2, &tmM2);
           }
         }
-      }
-      if (slabs <= h) {                              // no slab for this warp (narrow tile): release all the same
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0 && reused) mbar_arrive_cluster(cluster_addr(&tempty[buf], 0));
       }
     }
     if (lane == 0) tma_store_wait_read<0>();         // nothing in flight out of shared memory at exit
@@ -846,7 +841,7 @@ static int ns_product(const NsMatrix& A, const NsMatrix& B, const NsMatrix& C, c
   if (rc) return rc;
   // the output's rows in whole 16-byte units (the padding of the workspace takes zeros); a result with other rows is not stored by TMA
   tmC = tmA;
-  const bool narrow = bn == 64;
+  const bool narrow = bn == 64;                // the others have 128 columns and more: two slabs a tile at least in either form
   const uint32_t slab = narrow ? 32 : 64;
   const int swizzle = narrow ? 2 : 3;
   if (C.ld % 8 == 0 && (rc = ns_map(&tmC, C, C.ld, M, batch, pairs, slab, 32, swizzle))) return rc;
