@@ -359,8 +359,30 @@ static int launch_fp8(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUte
   return e == cudaSuccess ? 0 : 2000 + static_cast<int>(e);
 }
 
+// Rows of A that a CTA loads.
+static int fp8_rows_of_a(int M) { return M < 128 ? (M + 7) / 8 * 8 : 128; }
+// Width of the tiles: clocks of a step of 128 are the larger of the tensor cores' (2 per column) and of the loads' (64 bytes a
+// clock reach an SM: two per row of A, one per column for B), times the tiles that a pair works through.
+static int fp8_tile_columns(int M, int N, int K, int pairs) {
+  const long tiles_m = ((long)M + G8_BM - 1) / G8_BM;
+  const int nk = (K + G8_BK - 1) / G8_BK, a_rows = fp8_rows_of_a(M);
+  int bn = 256;
+  double best = 0;
+  for (int b = 256; b >= 64; b -= 64) {
+    const long tiles = tiles_m * (((long)N + b - 1) / b);
+    const double cost = (double)((tiles + pairs - 1) / pairs) * (nk * (double)(b > 2 * a_rows ? 2 * b : 2 * a_rows + b) + 1500.0);
+    if (b == 256 || cost < best * 0.97) {
+      best = cost;
+      bn = b;
+    }
+  }
+  return bn;
+}
+
 }  // namespace kb
 
+// Width of the tiles that the call below takes on `sms` SMs.
+extern "C" int kb_gemm_fp8_columns(int M, int N, int K, int sms) { return kb::fp8_tile_columns(M, N, K, sms / 2); }
 // C [M, N] = A [M, K] * B [N, K]^T: bytes of format 0 (e4m3) or 1 (e5m2) with rows of lda / ldb bytes (multiples of 16), scales as
 // kb_fp8_quantize lays them out.  C: bf16 or fp32 (out_f32), rows of ldc elements; accumulate (fp32): +=.
 extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, const void* B, const void* SB, int fmt_b, long ldb,
@@ -377,19 +399,8 @@ extern "C" int kb_gemm_fp8(const void* A, const void* SA, int fmt_a, long lda, c
   w.tiles_m = (M + G8_BM - 1) / G8_BM;
   w.nk = (K + G8_BK - 1) / G8_BK;
   w.groups_k = (w.nk + 3) / 4;
-  w.a_rows = M < 128 ? (M + 7) / 8 * 8 : 128;
-  // Width of the tiles: clocks of a step of 128 are the larger of the tensor cores' (2 per column) and of the loads' (64 bytes a
-  // clock reach an SM: two per row of A, one per column for B), times the tiles that a pair works through.
-  int bn = 256;
-  double best = 0;
-  for (int b = 256; b >= 64; b -= 64) {
-    const long tiles = (long)w.tiles_m * ((N + b - 1) / b);
-    const double cost = (double)((tiles + pairs - 1) / pairs) * (w.nk * (double)(b > 2 * w.a_rows ? 2 * b : 2 * w.a_rows + b) + 1500.0);
-    if (b == 256 || cost < best * 0.97) {
-      best = cost;
-      bn = b;
-    }
-  }
+  w.a_rows = fp8_rows_of_a(M);
+  const int bn = fp8_tile_columns(M, N, K, pairs);
   w.tiles_n = (N + bn - 1) / bn;
   const long panel = (long)G8_BM * K;          // m-tiles per group: about 24 MB of A rows, 8 to 16 tiles
   long gm = (24L << 20) / panel;

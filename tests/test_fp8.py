@@ -382,3 +382,40 @@ def test_results_as_tensors():
     t = torch.ones(1, device="cuda", requires_grad=True)
     Keep.apply(t).backward()
     assert torch.equal(t.grad[0], outside.dequantize().sum())
+
+
+#: width of the tiles -> rows and columns of a product that takes it with several tiles a pair of SMs, 74 pairs or a few fewer
+WIDTHS = {64: (60000, 64), 128: (60000, 120), 192: (18984, 552), 256: (18984, 744)}
+
+
+def _columns(M, N, Kd, sms):
+    import ctypes
+    from kareus_b200.kernels import build
+    if not build.LIB.exists():
+        pytest.skip("native library not built")
+    f = ctypes.CDLL(str(build.LIB)).kb_gemm_fp8_columns
+    f.argtypes = [ctypes.c_int] * 4
+    return f(M, N, Kd, sms)
+
+
+@pytest.mark.parametrize("sms", [132, 140, 148])
+def test_sizes_take_every_tile_width(sms):
+    """What the tests of the widths run, and the two borders of the choice: few tiles take narrow ones, many wide ones."""
+    assert all(_columns(*size, 1100, sms) == width for width, size in WIDTHS.items())
+    assert {_columns(148 * 256 // 2 + 40, n, 1100, 148) for w in WIDTHS for n in (w, 3 * w - 24)} == set(WIDTHS)
+    assert _columns(1, 9000, 700, sms) in WIDTHS and _columns(17, 64, 1100, sms) == 64 and _columns(8192, 28672, 4096, sms) == 256
+
+
+@gpu
+@pytest.mark.parametrize("width", sorted(WIDTHS))
+def test_gemm_several_tiles_of_every_width(width):
+    (M, N), Kd = WIDTHS[width], 1100
+    assert _columns(M, N, Kd, torch.cuda.get_device_properties(0).multi_processor_count) == width
+    a, _ = K.fp8_quantize(sample(M, Kd, "cuda", 3))
+    b, _ = K.fp8_quantize(sample(N, Kd, "cuda", 4))
+    y = K.fp8_gemm(a, b)
+    check_product(y, a, b)
+    assert torch.equal(y, K.fp8_gemm(a, b))
+    acc = torch.ones(M, N, device="cuda")
+    K.fp8_gemm(a, b, accumulate=acc)
+    check_product(acc, a, b, torch.ones(M, N, device="cuda"))
