@@ -271,3 +271,148 @@ def test_statements_repeat_bit_for_bit(device, dtype):
         K.embedding_bwd(d, t, g, 0, scale=1.3, order="sorted")
         runs.append(g)
     assert all(torch.equal(r, runs[0]) for r in runs)
+
+
+#: one length for each way a batch is taken: in one kernel, sorted by counting, by the radix sort, in two chunks
+PATHS = [300, 3000, 5000, 70000]
+
+
+@gpu
+@pytest.mark.parametrize("n", [1100, 4096, 4097, 20000])
+@pytest.mark.parametrize("v", [1, 2, 3, 511, 512, 513, 2 ** 17, 2 ** 18 - 1, 2 ** 18, 2 ** 18 + 1])
+def test_digits_of_the_radix_sort(n, v):
+    """Tables at the borders of one, two and three digits, with keys at both ends, beyond 4096 tokens and below."""
+    t = draw(n, v, 3)
+    t[5], t[6], t[-1] = v - 1, 0, v - 1
+    check(t, table(v, 8), 0, 2.0)
+    check(t + v // 2, table(v, 8), 0, 1.0)                         # half of the keys are another shard's
+
+
+@gpu
+def test_four_digits():
+    """More than 2^27 rows.  Whole numbers whose sums fp32 holds."""
+    v, n = 2 ** 27 + 3, 6000
+    t = draw(n, v)
+    t[:50], t[50:99] = v - 1, 2 ** 27 - 1
+    d = torch.randint(-8, 9, (n, 1), generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    grad = torch.zeros(v, 1, device="cuda")
+    K.embedding_bwd(d, t, grad, 0, order="sorted")
+    rows, inverse = torch.unique(t, return_inverse=True)
+    want = torch.zeros(rows.numel(), 1, device="cuda").index_add_(0, inverse, d.float())
+    assert torch.equal(grad[rows], want)
+    grad[rows] = 0
+    assert not bool(grad.any())
+
+
+@gpu
+@pytest.mark.parametrize("n", PATHS[:3])
+@pytest.mark.parametrize("H", [1, 7, 136, 1020, 1024, 1032, 2056, 4096])
+def test_widths_of_every_path(n, H):
+    """One block of columns in the sums and the join, several, a last one of few columns; rows that start on 16 bytes and not."""
+    check(draw(n, 90, 2), table(90, H), 0, 1.0)
+    check(draw(n, 90, seed=4).view(n // 100, 100), table(30, H), 30, 0.5)
+
+
+@gpu
+@pytest.mark.parametrize("n", PATHS)
+def test_tokens_of_no_row_in_every_path(n):
+    w = table(50, 64)
+    far = draw(n, 50)
+    far[::2] += torch.tensor(2 ** 32)
+    far[1::4] = -2 ** 62
+    far[3::8] = 2 ** 62
+    for t in (torch.full((n,), 50), torch.full((n,), -1), far):
+        check(t.cuda(), w, 0, 1.0)
+    check(draw(n, 50), w, 2 ** 40, 1.0)
+
+
+@gpu
+@pytest.mark.parametrize("n", PATHS)
+def test_not_finite_in_every_path(n):
+    t, d = draw(n, 9), torch.ones(n, 24, device="cuda").bfloat16()
+    t[0], t[-1], t[n // 2] = 3, 4, 9
+    d[0, 5], d[-1, 0], d[n // 2, 2] = float("inf"), float("nan"), float("nan")
+    g = torch.zeros(9, 24, device="cuda")
+    K.embedding_bwd(d, t, g, 0, order="sorted")                    # token 9 belongs to another shard
+    assert g[3, 5].isinf() and g[4, 0].isnan() and torch.isfinite(g).sum() == 9 * 24 - 2
+    count = torch.bincount(t, minlength=10)[:9].float()
+    assert torch.equal(g[:, 8], count)                             # sums of ones, 2^24 at most
+
+
+@gpu
+@pytest.mark.parametrize("n", PATHS)
+def test_views_streams_and_graphs_of_every_path(n):
+    """Strided and unaligned gradients, two streams at once (each call has a workspace of its own), two captured graphs that share a
+    pool and take new tokens: the bits of a plain call.  Sums are of whole numbers, which fp32 holds in any order."""
+    H = 72
+    whole = torch.randint(-4, 5, (n, H + 16), generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    d, t = whole[:, 8:8 + H].contiguous(), draw(n, 40, 3)
+
+    def want(t):
+        return torch.zeros(40, H, device="cuda", dtype=torch.float64).index_add_(0, t, d.double()).float()
+
+    zeros = lambda: torch.zeros(40, H, device="cuda")
+    g = zeros()
+    K.embedding_bwd(whole[:, 8:8 + H], t, g, 0, order="sorted")
+    assert torch.equal(g, want(t))
+    flat = torch.zeros(40 * H + 2, device="cuda")
+    K.embedding_bwd(d, t, flat[1:-1].view(40, H), 0, order="sorted")
+    assert torch.equal(flat[1:-1].view(40, H), want(t)) and flat[0].item() == flat[-1].item() == 0
+    tokens = [draw(n, 40, 3, seed=s) for s in (5, 6)]
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [zeros(), zeros()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for s, tok, out in zip(streams, tokens, outs):
+            with torch.cuda.stream(s):
+                out.zero_()
+                K.embedding_bwd(d, tok, out, 0, order="sorted")
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want(tok)) for tok, out in zip(tokens, outs))
+    graphs, pool = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], None
+    for graph, tok, out in zip(graphs, tokens, outs):
+        with torch.cuda.graph(graph, pool=pool):
+            out.zero_()
+            K.embedding_bwd(d, tok, out, 0, order="sorted")
+        pool = graph.pool()
+    for seed in (7, 8):
+        for i, tok in enumerate(tokens):
+            tok.copy_(draw(n, 40, 3, seed=seed + 10 * i))
+        for graph in (graphs[1], graphs[0], graphs[1]):
+            graph.replay()
+        assert all(torch.equal(out, want(tok)) for tok, out in zip(tokens, outs))
+
+
+@gpu
+@pytest.mark.parametrize("n", PATHS[1:3])
+def test_rows_beyond_32_bits_of_every_path(n):
+    """The last rows of a gradient of more than 2^32 bytes, one token on many of them."""
+    v, H = 300000, 4096
+    t = v - 1 - draw(n, 200, 2)
+    t[::7] = v - 1
+    d = torch.randint(-4, 5, (n, H), generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    grad = torch.zeros(v, H, device="cuda")
+    K.embedding_bwd(d, t, grad, 0, order="sorted")
+    want = torch.zeros(200, H, device="cuda", dtype=torch.float64).index_add_(0, t - (v - 200), d.double())
+    assert torch.equal(grad[v - 200:], want.float())
+    assert not bool(grad[:v - 200].any())
+    w = torch.zeros(v, H, dtype=torch.bfloat16, device="cuda")
+    w[v - 200:] = d[:200]
+    assert torch.equal(K.embedding_fwd(t, w, 0), d[t - (v - 200)])
+
+
+@gpu
+def test_batches_beyond_32_bits():
+    """Output and gradient of more than 2^32 bytes, chunk after chunk."""
+    n, H = 2 ** 19 + 20000, 4096
+    t = draw(n, 3000)
+    d = torch.zeros(n, H, dtype=torch.bfloat16, device="cuda")
+    d[-30000:] = torch.randint(-4, 5, (30000, H), generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    grad = torch.zeros(2000, H, device="cuda")
+    K.embedding_bwd(d, t, grad, 1000, order="sorted")              # a shard of the middle
+    want = torch.zeros(3000, H, device="cuda", dtype=torch.float64).index_add_(0, t[-30000:], d[-30000:].double())
+    assert torch.equal(grad, want[1000:].float())
+    w = table(2000, H)
+    out = K.embedding_fwd(t, w, 1000)
+    at = t[-30000:] - 1000
+    inside = (at >= 0) & (at < 2000)
+    assert torch.equal(out[-30000:], w[at.clamp(0, 1999)] * inside[:, None])
