@@ -114,6 +114,108 @@ def test_fp8_tensor_parallel(tp_comm):
     run_distributed(_fp8_tp_worker, 2, tp_comm)
 
 
+class _ShardedProducts:
+    """In the place of a weight of the oracle (``x @ w.t()``): the products of the quantised shards of ``tp`` ranks, in 64 bits, in both
+    directions.  ``axis`` 0: ranks have rows ``shards[r]`` of the weight, 1: columns, whose products are summed."""
+
+    def __init__(self, w, axis, shards):
+        self.w, self.axis, self.shards = w.detach(), axis, shards
+        self.grads = [0.0 for _ in shards]
+
+    def t(self):
+        return self
+
+    @classmethod
+    def __torch_function__(cls, func, types, args=(), kwargs=None):
+        assert func in (torch.Tensor.matmul, torch.Tensor.__matmul__, torch.matmul) and isinstance(args[1], cls)
+        return _ShardedProductsFn.apply(args[0], args[1])
+
+
+def _stands_for(t, square=False):
+    return ref.fp8_dequantize(*ref.fp8_quantize(t.contiguous(), "e4m3", square), dtype=torch.float64)
+
+
+class _ShardedProductsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, op):
+        x2 = x.reshape(-1, x.shape[-1])
+        ctx.op, ctx.shape = op, x.shape
+        ctx.save_for_backward(x2)
+        y = torch.zeros(x2.shape[0], op.w.shape[0], dtype=torch.float64)
+        for at in op.shards:
+            if op.axis == 0:
+                y[:, at] = _stands_for(x2) @ _stands_for(op.w[at], True).t()
+            else:
+                y += _stands_for(x2[:, at]) @ _stands_for(op.w[:, at], True).t()
+        return y.reshape(x.shape[:-1] + (-1,))
+
+    @staticmethod
+    def backward(ctx, dy):
+        op, (x2,) = ctx.op, ctx.saved_tensors
+        dy2, dx = dy.reshape(-1, dy.shape[-1]), torch.zeros_like(x2)
+        for r, at in enumerate(op.shards):
+            if op.axis == 0:
+                dx += _stands_for(dy2[:, at]) @ _stands_for(op.w[at], True)
+                op.grads[r] = op.grads[r] + _stands_for(dy2[:, at].t()) @ _stands_for(x2.t()).t()
+            else:
+                dx[:, at] = _stands_for(dy2) @ _stands_for(op.w[:, at], True)
+                op.grads[r] = op.grads[r] + _stands_for(dy2.t()) @ _stands_for(x2[:, at].t()).t()
+        return dx.reshape(ctx.shape), None
+
+
+def _fp8_tp_products_worker(rank, world, tp_comm):
+    """Loss and the gradients of every shard against a model of one process whose products are those of the quantised shards.
+
+    Both sides have the same operands up to what the order of sums changes, 1e-7 of a value at most.  Of values so close, at most 2 *
+    1e-7 / 2^-4 = 3e-6 lie on different sides of a border between two 8-bit values, which are 2^-3 apart at most: 2^-3 * sqrt(3e-6) =
+    2.2e-4 of an operand as a root mean square, sqrt(28) times that for the operands of two layers; 2.5 times it, 3e-3, is the limit.  A
+    reduction that is left out, or made twice, or a gradient of another shard's rows is off by the size of the gradient."""
+    from test_engine_distributed import _load
+    from kareus_b200.parallel.collectives import CommFactory
+    from kareus_b200.parallel.mesh import Mesh
+    mesh = Mesh(tp=world)
+    cfg = get_model_config("tiny").replace(linear_precision="fp8")
+    model = GPTModel(cfg, ParallelConfig(tp=world, tp_comm=tp_comm, num_nanobatches=2), mesh=mesh, comm=CommFactory(mesh, "nccl"), dtype="fp64")
+    states = [None] * world
+    dist.all_gather_object(states, {k: v.detach() for k, v in model.state_dict().items()})
+    oracle = OracleLlama(cfg)
+    _load(oracle, states, cfg)
+    for l in oracle.layers:
+        for name, axis in (("qkv", 0), ("proj", 1), ("fc1", 0), ("fc2", 1)):
+            w = getattr(l, name)
+            every = torch.arange(w.shape[axis])
+            shards = list(every.chunk(world)) if name != "fc1" else [torch.cat([half.chunk(world)[r] for half in every.chunk(2)])
+                                                                      for r in range(world)]
+            delattr(l, name)
+            setattr(l, name, _ShardedProducts(w, axis, shards))
+    g = torch.Generator().manual_seed(0)
+    tokens, labels = (torch.randint(0, cfg.vocab_size, (2, 32), generator=g) for _ in range(2))
+    want = 0.0
+    for i in range(2):                                             # a nanobatch is quantised on its own
+        part = oracle(tokens[i:i + 1], labels[i:i + 1], torch.ones(1, 32, dtype=torch.float64)) / 2
+        part.backward()
+        want += part.item()
+    loss = model(tokens, labels, torch.ones(2, 32))
+    loss.backward()
+    model.finalize_grads()
+    assert abs(loss.item() - want) < 1e-5 * want
+    pairs = [("emb", model.embedding.weight, oracle.emb.grad.chunk(world)[rank]),
+             ("out", model.output_layer.weight, oracle.out.grad.chunk(world)[rank]),
+             ("final_norm", model.final_norm.weight, oracle.final_norm.grad)]
+    for i, (layer, l) in enumerate(zip(model.decoder.layers, oracle.layers)):
+        pairs += [(f"{i}.{name}", getattr(layer, name).weight, getattr(l, name).grads[rank]) for name in ("qkv", "proj", "fc1", "fc2")]
+        pairs += [(f"{i}.input_norm", layer.input_norm.weight, l.input_norm.grad),
+                  (f"{i}.pre_mlp_norm", layer.pre_mlp_norm.weight, l.pre_mlp_norm.grad)]
+    for name, p, exact in pairs:
+        off = ((p.main_grad - exact).norm() / exact.norm()).item()
+        assert off < 3e-3, (name, off)
+
+
+@pytest.mark.parametrize("tp_comm", ["allreduce", "sp"])
+def test_fp8_tensor_parallel_products(tp_comm):
+    run_distributed(_fp8_tp_products_worker, 2, tp_comm)
+
+
 def test_refused_layouts():
     cfg = get_model_config("tiny").replace(linear_precision="fp8")
     from kareus_b200.models.llama import TransformerLayer
