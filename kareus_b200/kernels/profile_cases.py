@@ -4,6 +4,7 @@
     python -m kareus_b200.kernels.profile_cases attn_fwd    # B4 H3 S4096 d128 causal, 3 launches
     python -m kareus_b200.kernels.profile_cases norm | swiglu | ce | adamw | rope
     python -m kareus_b200.kernels.profile_cases gemm_epilogues   # what GEMM epilogues do besides storing, 5 GEMMs a repetition
+    python -m kareus_b200.kernels.profile_cases fp8 | newton_schulz | embedding   # operators of a low-precision training run
 
 Each case touches more than the 126 MB L2 where DRAM figures matter but holds at most a few GB,
 and launches its kernel a handful of times so a ``--set full`` capture ends within minutes.
@@ -15,6 +16,7 @@ Timing tables (CUDA events, no profiler; L2 flushed between launches):
     python -m kareus_b200.kernels.profile_cases small_table     # small calls: device and host time
     python -m kareus_b200.kernels.profile_cases swiglu_sweep    # drawn layers: SwiGLU in the GEMMs' epilogues or on its own
     python -m kareus_b200.kernels.profile_cases route_sweep     # drawn layers: kernels, widths and K parts of bf16 outputs
+    python -m kareus_b200.kernels.profile_cases low_precision_step   # training steps in bf16 and 8 bits, with AdamW and Muon
     python -m torch.distributed.run --nproc-per-node N --master-addr 127.0.0.1 \
         -m kareus_b200.kernels.profile_cases fused                # the eight fused GEMM+collective kernels at TP N
 """
@@ -243,6 +245,33 @@ def small_table() -> None:
         torch.cuda.synchronize()
         print(f"| training step of tiny128, launch lists {'on' if lists else 'off'} | | {(time.perf_counter() - t0) / 30 * 1e6:.0f} |")
     KC.check_status()
+
+
+def low_precision_step() -> None:
+    """Training steps of 4 layers of the 8B model (16384-row vocabulary, 2 microbatches of 4 x 4096 tokens, recompute): bf16 or 8-bit
+    layers, AdamW or Muon, embedding gradients by atomics or by sorted tokens."""
+    from ..config import ParallelConfig, TrainConfig, get_model_config
+    from ..train.trainer import Trainer, synthetic_batch
+    print("| layers | optimizer | embedding gradient | ms a step | peak GB |\n|---|---|---|---|---|")
+    for precision, optimizer, order in (("bf16", "adamw", "any"), ("bf16", "adamw", "sorted"), ("fp8", "adamw", "any"),
+                                        ("bf16", "muon", "any"), ("fp8", "muon", "sorted")):
+        cfg = get_model_config("llama3.1_8b").replace(num_layers=4, vocab_size=16384, linear_precision=precision, embedding_grad=order)
+        tc = TrainConfig(micro_batch_size=4, global_batch_size=8, seq_len=4096, optimizer=optimizer)
+        torch.cuda.reset_peak_memory_stats()
+        tr = Trainer(cfg, ParallelConfig(num_nanobatches=2, recompute=True), tc, device="cuda")
+        batch = synthetic_batch(cfg, tc, tr.num_microbatches)
+        for _ in range(4):                    # recorded in the second, replayed from the third on
+            tr.train_step(batch)
+        times = []
+        for _ in range(8):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            tr.train_step(batch)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        print(f"| {precision} | {optimizer} | {order} | {sorted(times)[4]:.1f} | {torch.cuda.max_memory_allocated() / 1e9:.1f} |", flush=True)
+        del tr
 
 
 def _in_turn(fns, rounds: int = 5, target_ms: float = 4.0) -> dict:
@@ -550,7 +579,8 @@ def collectives_table() -> None:
 
 # every command of this module: tables (CUDA events) and single-kernel cases (for a profiler capture)
 CASES = ("collectives", "memory_table", "small_table", "wgrad_sweep", "swiglu_sweep", "route_sweep", "gemm_table", "attn_table", "fused", "gemm",
-         "gemm_epilogues", "gemm_one_sm", "gemm_wgrad", "attn_fwd", "attn_bwd", "norm", "swiglu", "rope", "ce", "adamw", "step")
+         "low_precision_step", "gemm_epilogues", "gemm_one_sm", "gemm_wgrad", "attn_fwd", "attn_bwd", "norm", "swiglu", "rope", "ce", "adamw", "fp8", "newton_schulz", "embedding",
+         "step")
 
 
 def main(case: str, reps: int = 3) -> None:
@@ -574,6 +604,8 @@ def main(case: str, reps: int = 3) -> None:
         return attn_table()
     if case == "small_table":
         return small_table()
+    if case == "low_precision_step":
+        return low_precision_step()
     if case == "fused":
         return fused_table()
     if case == "gemm":
@@ -650,6 +682,42 @@ def main(case: str, reps: int = 3) -> None:
         p = w.bfloat16()
         for i in range(reps):
             KC.adamw_step(p, g, m, v, w, 1e-3, 0.9, 0.98, 1e-8, 0.01, i + 1)
+    elif case == "fp8":
+        # gate and up projection of the 8B model over 8192 tokens in both directions (3 quantisations, 3 products), then 17 tokens
+        # through its QKV projection (2 quantisations, a product)
+        import kareus_b200.kernels as K
+        x, w, dy = (torch.randn(*s, device=dev).bfloat16() for s in ((8192, 4096), (28672, 4096), (8192, 28672)))
+        acc, few, qkv = torch.zeros(28672, 4096, device=dev), x[:17], torch.randn(6144, 4096, device=dev).bfloat16()
+        for _ in range(reps):
+            (xr, xc), (wr, wc), (dr, dc) = K.fp8_quantize(x, cols=True), K.fp8_quantize(w, cols=True, square=True), K.fp8_quantize(dy, cols=True)
+            K.fp8_gemm(xr, wr)
+            K.fp8_gemm(dr, wc)
+            K.fp8_gemm(dc, xc, accumulate=acc)
+            K.fp8_gemm(K.fp8_quantize(few)[0], K.fp8_quantize(qkv, square=True)[0])
+    elif case == "newton_schulz":
+        # optimizer steps of the 8B model's QKV and down projections, and an iteration that launches bound
+        import kareus_b200.kernels as K
+        x = torch.randn(2048, 512, device=dev)
+        for rows, cols in ((6144, 4096), (4096, 14336)):
+            g, m, master = (torch.randn(rows, cols, device=dev) * 1e-3 for _ in range(3))
+            p = master.bfloat16()
+            for _ in range(reps):
+                K.muon_step(p, g, m, master, lr=2e-4, weight_decay=0.01)
+        for _ in range(reps):
+            K.orthogonalize(x)
+    elif case == "embedding":
+        # lookup and sorted gradient: text-like tokens into the 8B model's table, a shard of the 1.7B model's with padding, few tokens
+        import kareus_b200.kernels as K
+        gen = torch.Generator(device=dev).manual_seed(0)
+        for n, hidden, rows, first, total, skew, padded in ((8192, 4096, 128256, 0, 128256, 4, 0), (32768, 2048, 18992, 37984, 151936, 2, 10813),
+                                                            (512, 512, 2048, 0, 2048, 1, 0)):
+            tokens = (torch.rand(n, device=dev, generator=gen, dtype=torch.float64) ** skew * total).long()
+            tokens[n - padded:] = first + rows // 2
+            w, dout, grad = torch.randn(rows, hidden, device=dev).bfloat16(), torch.randn(n, hidden, device=dev).bfloat16(), \
+                torch.zeros(rows, hidden, device=dev)
+            for _ in range(reps):
+                K.embedding_fwd(tokens, w, first, scale=64.0)
+                K.embedding_bwd(dout, tokens, grad, first, scale=64.0, order="sorted")
     elif case == "step":
         # one training step of a 2-layer model with the 3B layer shape (1 microbatch of 8 x 4096)
         from ..config import ParallelConfig, TrainConfig, get_model_config
