@@ -317,8 +317,9 @@ def embedding_fwd(tokens, weight, vocab_start, scale=1.0):
 
 def embedding_bwd(dout, tokens, grad_weight, vocab_start, scale=1.0, order="any"):
     """``grad_weight[id] += scale *`` the sum of ``dout`` over the tokens ``id``.  ``order="sorted"``: the rows of a token are summed
-    in the order of the tokens and added once, so the same inputs give the same bits, and tokens that fill much of a batch (padding)
-    cost no more than others; ``"any"``: as they come, with atomic additions (a ``scale`` other than 1 sorts too)."""
+    in an order that the tokens alone decide (partial sums of consecutive rows, put together from front to back; one addition to the
+    table for each 65536 tokens), so the same inputs give the same bits, and tokens that fill much of a batch (padding) cost no more
+    than others; ``"any"``: as they come, with atomic additions on the GPU (there a ``scale`` other than 1 sorts too)."""
     if is_cuda(dout):
         return _cuda().embedding_bwd(dout, tokens, grad_weight, vocab_start, scale, order)
     return ref.embedding_bwd(dout, tokens, grad_weight, vocab_start, scale, order)

@@ -1,6 +1,6 @@
 // Embedding lookup with a scale, and the gradient of the table by sorted tokens.
 //
-//   out[t] = s W[id_t]          G[id] += s * sum of dout[t] over the t with id_t = id, in order of t
+//   out[t] = s W[id_t]          G[id] += s * sum of dout[t] over the t with id_t = id
 //
 // The gradient with atomic additions (elementwise.cu) adds the rows of a token as they come, so its bits change from run to run,
 // and tokens that make up much of a batch (padding, a frequent word) queue up for the same addresses.  Here the tokens are sorted
@@ -16,7 +16,8 @@
 //
 // Up to 1024 tokens take one kernel for all of it, further below.
 //
-// The order of additions depends on the tokens alone, so the same inputs give the same bits.  Sums are fp32.
+// The order of additions depends on the tokens alone, so the same inputs give the same bits.  Sums are fp32: of consecutive rows of
+// a token, which are put together from front to back.  Batches beyond 65536 tokens are taken in chunks, each of which adds to the table.
 //
 // What bounds it: memory for the lookup and the sums, latency for the sort and the join.  One B200, us: 8192 x 4096 into 128256 rows
 // lookup 18, sort 12, sums 39, join 8; 32768 x 2048, a third of it one token, 21, 14, 24, 12 (the atomic form queues for that row).
