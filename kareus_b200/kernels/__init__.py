@@ -335,9 +335,11 @@ def adamw_step(p, g, m, v, master, lr, beta1, beta2, eps, wd, step, grad_scale=1
 def orthogonalize(x, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     """The last two dimensions of ``x`` after ``steps`` Newton-Schulz products, as bf16: ``X = x / (|x|_F + eps)``, then ``G = X Xt;
     X = a X + (b G + c G G) X``.  Singular vectors stay, singular values go to about 1 (0.7 to 1.2 with these coefficients and five
-    steps); ones below about 1e-3 of the largest stay small.  The products run in fp16 with fp32 sums.  A matrix with an infinity, a
-    NaN or a sum of squares beyond fp32 becomes NaN, one of zeros stays zero.  ``eps`` is at least 1e-12; ``coefficients`` that let
-    the iterates leave the range of fp16 are refused."""
+    steps); ones below about 1e-3 of the largest stay small.  On the GPU the products of fp32 and bf16 matrices run in fp16 with fp32
+    sums, which costs 1e-3 to 1e-2 of the result's 2-norm, most where singular values lie decades apart (a few percent for matrices of
+    a few rows that are nearly singular).  A matrix with an infinity, a NaN or squares whose sum is beyond fp32 (on the GPU: the sum of
+    256 of them) becomes NaN, one of zeros stays zero.  ``eps`` is at least 1e-12; on the GPU ``coefficients`` that let the iterates
+    leave the range of fp16 are refused."""
     from .muon import orthogonalize as f
     return f(x, steps, coefficients, eps)
 
